@@ -112,7 +112,7 @@ def _seen(pages, c):
 def _encode(x, fmt):
     """fp32 rows [..., dim] -> codes (as bytes) and scales [...]."""
     scale = (x.abs().amax(-1) / TOP[fmt]).clamp(min=TINY)
-    y = x / scale[..., None]
+    y = x * (1 / scale)[..., None]
     y = y.to(CODES["e4m3"]) if fmt == "e4m3" else y.round().to(torch.int8)
     return y.view(torch.uint8), scale
 
