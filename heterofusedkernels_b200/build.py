@@ -33,7 +33,8 @@ INCLUDE = ROOT / "include"
 
 CAPI_SOURCES = ["hfk_capi.cu", "host_registry.cpp"]
 CAPI_DEPS = ["common.cuh", "kv_swap.cuh", "paged_gather.cuh", "row_gather.cuh", "block_transfer.cuh", "relayout_swap.cuh",
-             "kv_migrate.cuh", "ptr_check.h", "host_util.h"]
+             "kv_migrate.cuh", "kv_format.cuh", "kv_write.cuh", "paged_gather_dequant.cuh", "shared_prefix_attention.cuh",
+             "cache_ops_host.cuh", "ptr_check.h", "host_util.h"]
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
@@ -69,7 +70,7 @@ def build_capi(force: bool = False, verbose: bool = False, ptxas_info: bool = Fa
     if not force and not _stale(out, deps):
         return out
     nvcc = str(_cuda_home() / "bin" / "nvcc")
-    cmd = [nvcc, "-O3", "-std=c++17", "-lineinfo", *ARCH_FLAGS, "-shared", "-Xcompiler",
+    cmd = [nvcc, "-O3", "-std=c++17", "-lineinfo", "-split-compile", "0", *ARCH_FLAGS, "-shared", "-Xcompiler",
            "-fPIC,-Wall", "-cudart", "static"]
     if ptxas_info:
         cmd += ["-Xptxas", "-v"]

@@ -28,6 +28,10 @@ HFK_DEV_BAD_ROW_ID = 0x4
 HFK_DEV_BAD_SEQ_LEN = 0x8
 HFK_DEV_WAIT_TIMEOUT = 0x10
 HFK_DEV_BAD_LAYER_PTR = 0x20
+HFK_DEV_BAD_POSITION = 0x40
+
+HFK_KV_RAW, HFK_KV_E4M3, HFK_KV_INT8 = 0, 1, 2
+HFK_TYPE_BF16, HFK_TYPE_FP16, HFK_TYPE_FP32 = 0, 1, 2
 
 MOVER_AUTO, MOVER_VECTOR, MOVER_BULK = 0, 1, 2
 HFK_MAX_SEQS = 1024
@@ -118,6 +122,79 @@ class PagedGatherDesc(C.Structure):
     ]
 
 
+class Rows(C.Structure):
+    """struct hfk_rows"""
+    _fields_ = [("base", C.c_void_p), ("token_stride", C.c_int64), ("head_stride", C.c_int64)]
+
+
+class KvWriteDesc(C.Structure):
+    """struct hfk_kv_write_desc"""
+    _fields_ = [
+        ("k", Rows),
+        ("v", Rows),
+        ("k_cache", C.c_void_p),
+        ("v_cache", C.c_void_p),
+        ("slot_ids", C.c_void_p),
+        ("ids_are_int64", C.c_int),
+        ("type", C.c_int),
+        ("kv_format", C.c_int),
+        ("kv_heads", C.c_int),
+        ("head_dim", C.c_int),
+        ("tokens", C.c_int64),
+        ("block_size", C.c_int64),
+        ("device_block_stride", C.c_int64),
+        ("num_device_blocks", C.c_int64),
+    ]
+
+
+class NormRopeDesc(C.Structure):
+    """struct hfk_norm_rope_desc"""
+    _fields_ = [
+        ("q", Rows),
+        ("q_out", Rows),
+        ("q_heads", C.c_int),
+        ("rot_dim", C.c_int),
+        ("interleaved", C.c_int),
+        ("positions_are_int64", C.c_int),
+        ("positions", C.c_void_p),
+        ("cos_sin", C.c_void_p),
+        ("max_positions", C.c_int64),
+        ("q_weight", C.c_void_p),
+        ("k_weight", C.c_void_p),
+        ("eps", C.c_float),
+    ]
+
+
+class PrefixAttentionDesc(C.Structure):
+    """struct hfk_prefix_attention_desc"""
+    _fields_ = [
+        ("q", Rows),
+        ("out", Rows),
+        ("lse", C.c_void_p),
+        ("k_cache", C.c_void_p),
+        ("v_cache", C.c_void_p),
+        ("prefix_table", C.c_void_p),
+        ("block_tables", C.c_void_p),
+        ("seq_lens", C.c_void_p),
+        ("ids_are_int64", C.c_int),
+        ("type", C.c_int),
+        ("kv_format", C.c_int),
+        ("kv_heads", C.c_int),
+        ("group", C.c_int),
+        ("head_dim", C.c_int),
+        ("num_seqs", C.c_int64),
+        ("prefix_len", C.c_int64),
+        ("max_blocks_per_seq", C.c_int64),
+        ("block_table_stride", C.c_int64),
+        ("block_size", C.c_int64),
+        ("device_block_stride", C.c_int64),
+        ("num_device_blocks", C.c_int64),
+        ("scale", C.c_float),
+        ("workspace", C.c_void_p),
+        ("workspace_bytes", C.c_size_t),
+    ]
+
+
 # name -> (restype, argtypes); every symbol include/hfk_b200.h declares
 PROTOTYPES = {
     "hfk_strerror": (C.c_char_p, [C.c_int]),
@@ -166,6 +243,12 @@ PROTOTYPES = {
                                   C.c_int, C.c_void_p]),
     "hfk_swap_relayout": (C.c_int, [C.POINTER(RelayoutDesc), C.c_int, C.c_int, C.c_void_p]),
     "hfk_paged_gather": (C.c_int, [C.POINTER(PagedGatherDesc), C.c_int, C.c_int, C.c_void_p]),
+    "hfk_kv_block_bytes": (C.c_size_t, [C.c_int64, C.c_int64, C.c_int64, C.c_int]),
+    "hfk_kv_write": (C.c_int, [C.POINTER(KvWriteDesc), C.c_void_p]),
+    "hfk_qk_norm_rope_write": (C.c_int, [C.POINTER(KvWriteDesc), C.POINTER(NormRopeDesc), C.c_void_p]),
+    "hfk_paged_gather_dequant": (C.c_int, [C.POINTER(PagedGatherDesc), C.c_int, C.c_int, C.c_int, C.c_int, C.c_void_p]),
+    "hfk_prefix_attention_workspace": (C.c_size_t, [C.POINTER(PrefixAttentionDesc), C.c_int]),
+    "hfk_shared_prefix_attention": (C.c_int, [C.POINTER(PrefixAttentionDesc), C.c_int, C.c_void_p]),
 }
 
 _lib = None

@@ -165,6 +165,8 @@ class PagedKVCache:
         self.elt = self.k_caches[0].element_size()
         self.token_bytes = kv_heads * head_dim * self.elt
         self.block_bytes = block_size * self.token_bytes
+        self.page_shape: Tuple[int, ...] = (block_size, kv_heads, head_dim)
+        self.kv_format = _pkg.capi.HFK_KV_RAW
         self.slot_bytes = layers * 2 * self.block_bytes
         self.host_slots = 0
         self.host_pool: Optional[torch.Tensor] = None
@@ -192,7 +194,7 @@ class PagedKVCache:
         self._host_raw = raw
         self.host_slots = host_slots
         flat = raw.view(torch.uint8)[:host_slots * self.slot_bytes].view(self.dtype)
-        chunk = (2, self.block_size, self.kv_heads, self.head_dim)
+        chunk = (2,) + self.page_shape
         if self.pool_layout == "slot_major":
             self.host_pool = flat.view(host_slots, self.layers, *chunk)
         else:
@@ -363,6 +365,39 @@ class PagedKVCache:
                                             self.block_size, self.num_blocks, None, aiv, mover)
         return k_out, v_out
 
+    # -- one attention layer ---------------------------------------------------------
+    def write(self, layer: int, k: torch.Tensor, v: torch.Tensor, slot_ids: torch.Tensor) -> None:
+        """K and V rows of new tokens, ``[tokens, kv_heads, head_dim]``, to their pages of ``layer``.
+        ``slot_ids``: block * block_size + place in the block; a negative one marks a padding row."""
+        torch.ops.pcie_through.kv_write(k, v, self.k_caches[layer], self.v_caches[layer], slot_ids, self.block_size,
+                                        self.kv_format)
+
+    def norm_rope_write(self, layer: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slot_ids: torch.Tensor,
+                        positions: torch.Tensor, cos_sin: torch.Tensor, q_weight: Optional[torch.Tensor] = None,
+                        k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6, interleaved: bool = False,
+                        q_out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """``write`` after the norm of each query and key head (where a weight is given) and the rotation of their
+        first ``cos_sin.shape[1]`` elements; returns the queries.  ``cos_sin``: see ``rope_table``."""
+        if q_out is None:
+            q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        torch.ops.pcie_through.qk_norm_rope_write(q, k, v, q_out, self.k_caches[layer], self.v_caches[layer], slot_ids,
+                                                  positions, cos_sin, self.block_size, self.kv_format, q_weight, k_weight,
+                                                  eps, interleaved)
+        return q_out
+
+    def attend(self, layer: int, q: torch.Tensor, prefix_table: torch.Tensor, prefix_len: int, block_tables: torch.Tensor,
+               seq_lens: torch.Tensor, scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
+               lse: Optional[torch.Tensor] = None, aiv: Optional[int] = None) -> torch.Tensor:
+        """Attention of one new token of each sequence, ``q`` ``[num_seqs, query heads, head_dim]``, over the pages of a
+        prefix that all sequences share (``prefix_len`` tokens, 0 = none) and the pages of each sequence's own tokens
+        (``seq_lens``, the prefix not counted)."""
+        if out is None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        torch.ops.pcie_through.shared_prefix_attention(q, out, self.k_caches[layer], self.v_caches[layer], prefix_table,
+                                                       prefix_len, block_tables, seq_lens, self.block_size, self.kv_heads,
+                                                       self.kv_format, scale, lse, None, aiv)
+        return out
+
     def migrate_to(self, other: "PagedKVCache", src_block_ids, dst_block_ids, aiv: Optional[int] = None,
                    run_on: str = "dst") -> None:
         """other.cache[dst_block] <- self.cache[src_block], every layer, K and V, one launch.
@@ -372,6 +407,7 @@ class PagedKVCache:
         runs the kernel: "dst" pulls (peer loads), "src" pushes (peer stores).  The launch goes to the
         current stream of that GPU."""
         assert other.layers == self.layers and other.block_bytes == self.block_bytes
+        assert other.kv_format == self.kv_format and other.page_shape == self.page_shape
         dev = other.device if run_on == "dst" else self.device
         key = (id(other), dev)
         cached = getattr(self, "_migrate_tabs", None)
@@ -395,6 +431,65 @@ class PagedKVCache:
         GPU, not per cache or stream: quiesce side streams first."""
         with torch.cuda.device(self.device):
             return int(torch.ops.pcie_through.device_status())
+
+
+KV_FORMATS = {"e4m3": _pkg.capi.HFK_KV_E4M3, "int8": _pkg.capi.HFK_KV_INT8}
+
+
+class QuantizedPagedKVCache(PagedKVCache):
+    """A cache that keeps K and V in 8 bits, ``kv_format`` ``"e4m3"`` or ``"int8"``, with an fp32 scale for each token and
+    head: half the pages' memory, and half the bytes of every swap and migration.
+
+    A page is one run of bytes, codes and then scales, so each layer's cache is uint8 ``[num_blocks, page bytes]`` and
+    ``swap_out`` / ``swap_in`` (every mover), ``migrate_to`` and ``LayerwisePrefetcher`` work on it as on any other.
+    ``write`` / ``norm_rope_write`` quantise, ``attend`` reads the codes, ``paged_gather`` returns values of ``dtype``."""
+
+    def __init__(self, layers: int, num_blocks: int, block_size: int, kv_heads: int, head_dim: int, kv_format: str,
+                 device: torch.device | str = "cuda", host_slots: int = 0, dtype: torch.dtype = torch.bfloat16,
+                 host_raw: Optional[torch.Tensor] = None, pool_layout: str = "slot_major"):
+        code = KV_FORMATS[kv_format]
+        page = _pkg.capi.lib().hfk_kv_block_bytes(block_size, kv_heads, head_dim, code)
+        if page == 0:
+            raise ValueError(f"no page of block_size {block_size}, kv_heads {kv_heads}, head_dim {head_dim}")
+        super().__init__(layers, num_blocks, 1, 1, page, torch.uint8, device, 0, pool_layout=pool_layout)
+        self.k_caches = [t.view(num_blocks, page) for t in self.k_caches]
+        self.v_caches = [t.view(num_blocks, page) for t in self.v_caches]
+        self.block_size, self.kv_heads, self.head_dim = block_size, kv_heads, head_dim
+        self.token_bytes = kv_heads * head_dim      # codes of a token
+        self.page_shape = (page,)
+        self.kv_format = code
+        self.value_dtype = dtype
+        if host_raw is not None:
+            self.attach_host_raw(host_raw, host_slots)
+        elif host_slots > 0:
+            self.attach_host_pool(host_slots)
+
+    def paged_gather(self, block_tables: torch.Tensor, seq_lens: torch.Tensor, k_out: Optional[torch.Tensor] = None,
+                     v_out: Optional[torch.Tensor] = None, total_tokens: Optional[int] = None, aiv: Optional[int] = None,
+                     mover: Optional[int] = None):
+        """As for a 16-bit cache, with the values of the codes in ``k_out`` / ``v_out`` (bfloat16, float16 or float32;
+        ``value_dtype`` where they are not given).  There is one mover."""
+        if mover is not None:
+            raise ValueError("an 8-bit cache is read back by one kernel: mover must be None")
+        if k_out is None:
+            if total_tokens is None:
+                total_tokens = int(seq_lens.sum().item())
+            shape = (self.layers, total_tokens, self.kv_heads, self.head_dim)
+            k_out = torch.empty(shape, dtype=self.value_dtype, device=self.device)
+            v_out = torch.empty(shape, dtype=self.value_dtype, device=self.device)
+        torch.ops.pcie_through.paged_gather_dequant(self.k_ptrs, self.v_ptrs, k_out, v_out, block_tables.to(self.device),
+                                                    seq_lens.to(self.device), self.block_size, self.num_blocks,
+                                                    self.kv_format, None, aiv)
+        return k_out, v_out
+
+
+def rope_table(max_positions: int, rot_dim: int, base: float = 10000.0, scale: float = 1.0,
+               device: torch.device | str = "cuda") -> torch.Tensor:
+    """The table of ``norm_rope_write``: float32 ``[max_positions, rot_dim]``, cosines and then sines of
+    ``position / scale * base^(-2i / rot_dim)``, angles in 64 bits (at position 10^6 an fp32 angle is off by 0.03)."""
+    i = torch.arange(0, rot_dim, 2, dtype=torch.float64, device=device)
+    angle = torch.arange(max_positions, dtype=torch.float64, device=device)[:, None] / scale * base ** (-i / rot_dim)
+    return torch.cat([angle.cos(), angle.sin()], 1).float()
 
 
 LayerArg = Union[int, Tuple[int, int], range]

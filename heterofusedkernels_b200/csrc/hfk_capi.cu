@@ -686,6 +686,8 @@ static int transfer_impl(void *const *layer_ptrs, const void *src, int64_t B, in
 
 }  // namespace hfk
 
+#include "cache_ops_host.cuh"
+
 using namespace hfk;
 
 extern "C" {
@@ -871,6 +873,32 @@ int hfk_fused_memcpy_multi_layer_block_transfer(void *const *device_layer_ptrs,
   // ... stage 2: the same kernel, reading the staging buffer (:105)
   return transfer_impl(device_layer_ptrs, staging, block_size, layers, heads, head_dim, elt_size,
                        ctas, stream);
+}
+
+size_t hfk_kv_block_bytes(int64_t block_size, int64_t kv_heads, int64_t head_dim, int kv_format) {
+  return kv_block_bytes(block_size, kv_heads, head_dim, kv_format);
+}
+
+int hfk_kv_write(const hfk_kv_write_desc *desc, hfk_stream_t stream) {
+  return kv_write_impl("kv_write", desc, nullptr, false, stream);
+}
+
+int hfk_qk_norm_rope_write(const hfk_kv_write_desc *desc, const hfk_norm_rope_desc *norm_rope, hfk_stream_t stream) {
+  return kv_write_impl("qk_norm_rope_write", desc, norm_rope, true, stream);
+}
+
+int hfk_paged_gather_dequant(const hfk_paged_gather_desc *gather, int kv_format, int kv_heads, int out_type, int ctas,
+                             hfk_stream_t stream) {
+  return gather_dequant_impl(gather, kv_format, kv_heads, out_type, ctas, stream);
+}
+
+size_t hfk_prefix_attention_workspace(const hfk_prefix_attention_desc *desc, int ctas) {
+  AttnPlan p = {};
+  return plan_attention(desc, ctas, &p) == HFK_OK ? p.bytes() : 0;
+}
+
+int hfk_shared_prefix_attention(const hfk_prefix_attention_desc *desc, int ctas, hfk_stream_t stream) {
+  return attention_impl(desc, ctas, stream);
 }
 
 int hfk_migrate_blocks(const hfk_migrate_desc *desc, int ctas, hfk_stream_t stream) {

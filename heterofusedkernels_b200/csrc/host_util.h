@@ -50,5 +50,9 @@ constexpr int kDefaultStagedLanes = 1;
 constexpr long long kStagedMaxCopyBytes = 64ll << 20;
 // Block migration: 512-thread CTAs per SM (peer loads over NVLink need megabytes in flight).
 constexpr int kMigrateCtasPerSm = 2;
+// Reading an 8-bit cache back: 256-thread CTAs per SM, eight 8-byte loads a lane in flight.
+constexpr int kGatherDequantCtasPerSm = 4;
+// Attention: 128-thread CTAs per SM (about 200 registers a thread).
+constexpr int kAttnCtasPerSm = 2;
 
 }  // namespace hfk

@@ -25,6 +25,8 @@
 #include <cuda_runtime_api.h>
 #include <torch/library.h>
 
+#include <algorithm>
+#include <cmath>
 #include <string>
 
 #include "../../include/hfk_b200.h"
@@ -418,6 +420,259 @@ void migrate_blocks(const at::Tensor &srcKLayerPtrs, const at::Tensor &srcVLayer
   check_rc(hfk_migrate_blocks(&d, ctas, at::cuda::getCurrentCUDAStream().stream()), "migrate_blocks");
 }
 
+// ---------------------------------------------------------------- Group A ---
+// One layer's cache of an attention layer.  A 16-bit cache is [numDeviceBlocks, blockSize, kvHeads, headDim]; an
+// 8-bit cache is uint8 [numDeviceBlocks, at least hfk_kv_block_bytes].  Only the stride between pages is free.
+static int type_code(at::ScalarType t) {
+  return t == at::kBFloat16 ? HFK_TYPE_BF16 : t == at::kHalf ? HFK_TYPE_FP16 : t == at::kFloat ? HFK_TYPE_FP32 : -1;
+}
+
+static void check_cache(const at::Tensor &kCache, const at::Tensor &vCache, at::ScalarType type, int64_t blockSize,
+                        int64_t kvHeads, int64_t headDim, int64_t kvFormat, const char *op) {
+  TORCH_CHECK(kvFormat >= HFK_KV_RAW && kvFormat <= HFK_KV_INT8, op, ": kvFormat must be 0 (16-bit), 1 (e4m3) or 2 (int8)");
+  TORCH_CHECK(kCache.is_cuda() && kCache.device() == vCache.device(), op, ": kCache and vCache must be on one CUDA device");
+  TORCH_CHECK(kCache.sizes() == vCache.sizes() && kCache.strides() == vCache.strides() && kCache.scalar_type() == vCache.scalar_type(),
+              op, ": kCache and vCache must have the same shape, strides and dtype");
+  if (kvFormat == HFK_KV_RAW) {
+    TORCH_CHECK(kCache.scalar_type() == type, op, ": a 16-bit cache must have the dtype of the call, ", c10::toString(type));
+    TORCH_CHECK(kCache.dim() == 4 && kCache.size(1) == blockSize && kCache.size(2) == kvHeads && kCache.size(3) == headDim, op,
+                ": a 16-bit cache must be [numDeviceBlocks, blockSize, kvHeads, headDim]");
+    TORCH_CHECK(kCache.stride(3) == 1 && kCache.stride(2) == headDim && kCache.stride(1) == headDim * kvHeads, op,
+                ": the pages of a 16-bit cache must be contiguous");
+  } else {
+    TORCH_CHECK(kCache.scalar_type() == at::kByte && kCache.dim() == 2 && kCache.stride(1) == 1, op,
+                ": an 8-bit cache must be uint8 [numDeviceBlocks, page bytes] with contiguous pages");
+    const size_t page = hfk_kv_block_bytes(blockSize, kvHeads, headDim, static_cast<int>(kvFormat));
+    TORCH_CHECK(page > 0 && static_cast<size_t>(kCache.size(1)) >= page, op, ": a page of this cache has ", page, " bytes, the tensor's has ",
+                kCache.size(1));
+  }
+}
+
+static hfk_rows rows_of(const at::Tensor &t, const char *op, const char *name) {
+  TORCH_CHECK(t.dim() == 3 && (t.stride(2) == 1 || t.size(2) <= 1), op, ": ", name, " must be [tokens, heads, headDim] with contiguous rows");
+  hfk_rows r;
+  r.base = t.data_ptr();
+  // a dimension of size 1 has no stride that matters
+  r.token_stride = t.size(0) > 1 ? t.stride(0) * t.element_size() : 0;
+  r.head_stride = t.size(1) > 1 ? t.stride(1) * t.element_size() : 0;
+  return r;
+}
+
+static hfk_kv_write_desc write_desc(const at::Tensor &k, const at::Tensor &v, const at::Tensor &kCache, const at::Tensor &vCache,
+                                    const at::Tensor &slotIds, int64_t blockSize, int64_t kvFormat, const char *op) {
+  TORCH_CHECK(k.is_cuda() && k.dim() == 3 && k.sizes() == v.sizes() && k.scalar_type() == v.scalar_type(), op,
+              ": k and v must be device tensors [tokens, kvHeads, headDim] of the same shape and dtype");
+  TORCH_CHECK(k.scalar_type() == at::kBFloat16 || k.scalar_type() == at::kHalf, op, ": k and v must be bfloat16 or float16");
+  check_cache(kCache, vCache, k.scalar_type(), blockSize, k.size(1), k.size(2), kvFormat, op);
+  hfk_kv_write_desc d;
+  d.ids_are_int64 = ids_are_int64(slotIds, op);
+  TORCH_CHECK(slotIds.numel() == k.size(0), op, ": ", slotIds.numel(), " slot ids for ", k.size(0), " tokens");
+  TORCH_CHECK(v.device() == k.device() && kCache.device() == k.device() && slotIds.device() == k.device(), op,
+              ": all tensors must be on one device");
+  TORCH_CHECK(k.size(1) <= INT32_MAX && k.size(2) <= INT32_MAX, op, ": too many heads");
+  d.k = rows_of(k, op, "k");
+  d.v = rows_of(v, op, "v");
+  d.k_cache = kCache.data_ptr();
+  d.v_cache = vCache.data_ptr();
+  d.slot_ids = slotIds.data_ptr();
+  d.type = type_code(k.scalar_type());
+  d.kv_format = static_cast<int>(kvFormat);
+  d.kv_heads = static_cast<int>(k.size(1));
+  d.head_dim = static_cast<int>(k.size(2));
+  d.tokens = k.size(0);
+  d.block_size = blockSize;
+  d.device_block_stride = kCache.stride(0) * kCache.element_size();
+  d.num_device_blocks = kCache.size(0);
+  return d;
+}
+
+void kv_write(const at::Tensor &k, const at::Tensor &v, const at::Tensor &kCache, const at::Tensor &vCache, const at::Tensor &slotIds,
+              int64_t blockSize, int64_t kvFormat) {
+  const hfk_kv_write_desc d = write_desc(k, v, kCache, vCache, slotIds, blockSize, kvFormat, "kv_write");
+  const c10::cuda::CUDAGuard guard(k.device());
+  check_rc(hfk_kv_write(&d, at::cuda::getCurrentCUDAStream().stream()), "kv_write");
+}
+
+static const void *weight_of(const c10::optional<at::Tensor> &w, const at::Tensor &k, const char *name) {
+  if (!w.has_value() || !w->defined()) return nullptr;
+  TORCH_CHECK(w->device() == k.device() && w->scalar_type() == k.scalar_type() && w->is_contiguous() && w->dim() == 1 && w->numel() == k.size(2),
+              "qk_norm_rope_write: ", name, " must be a contiguous [headDim] tensor of k's dtype and device");
+  return w->data_ptr();
+}
+
+void qk_norm_rope_write(const at::Tensor &q, const at::Tensor &k, const at::Tensor &v, const at::Tensor &qOut, const at::Tensor &kCache,
+                        const at::Tensor &vCache, const at::Tensor &slotIds, const at::Tensor &positions, const at::Tensor &cosSin,
+                        int64_t blockSize, int64_t kvFormat, const c10::optional<at::Tensor> &qWeight,
+                        const c10::optional<at::Tensor> &kWeight, double eps, bool interleaved) {
+  const char *op = "qk_norm_rope_write";
+  const hfk_kv_write_desc d = write_desc(k, v, kCache, vCache, slotIds, blockSize, kvFormat, op);
+  TORCH_CHECK(q.dim() == 3 && q.size(0) == k.size(0) && q.size(2) == k.size(2) && q.scalar_type() == k.scalar_type(), op,
+              ": q must be [tokens, qHeads, headDim] of k's dtype");
+  TORCH_CHECK(qOut.sizes() == q.sizes() && qOut.scalar_type() == q.scalar_type(), op, ": qOut must have q's shape and dtype");
+  TORCH_CHECK(q.size(1) <= INT32_MAX, op, ": too many heads");
+  TORCH_CHECK(cosSin.scalar_type() == at::kFloat && cosSin.dim() == 2 && cosSin.is_contiguous(), op,
+              ": cosSin must be a contiguous float32 [maxPositions, rotDim] tensor (cosines, then sines)");
+  hfk_norm_rope_desc n;
+  n.positions_are_int64 = ids_are_int64(positions, op);
+  TORCH_CHECK(positions.numel() == k.size(0), op, ": ", positions.numel(), " positions for ", k.size(0), " tokens");
+  TORCH_CHECK(q.device() == k.device() && qOut.device() == k.device() && positions.device() == k.device() && cosSin.device() == k.device(),
+              op, ": all tensors must be on one device");
+  TORCH_CHECK(cosSin.size(1) <= k.size(2), op, ": rotDim ", cosSin.size(1), " is larger than headDim");
+  n.q = rows_of(q, op, "q");
+  n.q_out = rows_of(qOut, op, "qOut");
+  n.q_heads = static_cast<int>(q.size(1));
+  n.rot_dim = static_cast<int>(cosSin.size(1));
+  n.interleaved = interleaved ? 1 : 0;
+  n.positions = positions.data_ptr();
+  n.cos_sin = cosSin.data_ptr<float>();
+  n.max_positions = cosSin.size(0);
+  n.q_weight = weight_of(qWeight, k, "qWeight");
+  n.k_weight = weight_of(kWeight, k, "kWeight");
+  n.eps = static_cast<float>(eps);
+  const c10::cuda::CUDAGuard guard(k.device());
+  check_rc(hfk_qk_norm_rope_write(&d, &n, at::cuda::getCurrentCUDAStream().stream()), op);
+}
+
+// kOut / vOut: [layers, total_tokens, kvHeads, headDim] of bfloat16, float16 or float32.
+void paged_gather_dequant(const at::Tensor &kLayerPtrs, const at::Tensor &vLayerPtrs, const at::Tensor &kOut, const at::Tensor &vOut,
+                          const at::Tensor &blockTables, const at::Tensor &seqLens, int64_t blockSize, int64_t numDeviceBlocks,
+                          int64_t kvFormat, c10::optional<int64_t> deviceBlockStride, c10::optional<int64_t> aiv) {
+  const char *op = "paged_gather_dequant";
+  const int ctas = cores_from(aiv);
+  TORCH_CHECK(kOut.is_cuda() && kOut.dim() == 4 && kOut.sizes() == vOut.sizes() && kOut.is_contiguous() && vOut.is_contiguous() &&
+                  kOut.scalar_type() == vOut.scalar_type(),
+              op, ": kOut and vOut must be contiguous device tensors [layers, total_tokens, kvHeads, headDim] of equal shape and dtype");
+  const int out_type = type_code(kOut.scalar_type());
+  TORCH_CHECK(out_type >= 0, op, ": kOut must be bfloat16, float16 or float32");
+  TORCH_CHECK(kvFormat == HFK_KV_E4M3 || kvFormat == HFK_KV_INT8, op, ": kvFormat must be 1 (e4m3) or 2 (int8); paged_gather reads a 16-bit cache");
+  TORCH_CHECK(blockTables.scalar_type() == at::kLong || blockTables.scalar_type() == at::kInt, op, ": blockTables must be int64 or int32");
+  TORCH_CHECK(blockTables.dim() == 2 && (blockTables.stride(1) == 1 || blockTables.size(1) <= 1), op,
+              ": blockTables must be [num_seqs, max_blocks] with unit inner stride");
+  TORCH_CHECK(seqLens.dim() == 1 && seqLens.is_contiguous() && seqLens.scalar_type() == blockTables.scalar_type() &&
+                  seqLens.size(0) == blockTables.size(0),
+              op, ": seqLens must be [num_seqs] of the same dtype as blockTables");
+  const auto dev = kOut.device();
+  TORCH_CHECK(vOut.device() == dev && blockTables.device() == dev && seqLens.device() == dev && kLayerPtrs.device() == dev &&
+                  vLayerPtrs.device() == dev,
+              op, ": all tensors must be on one device");
+  hfk_paged_gather_desc d;
+  d.layers = static_cast<int>(kOut.size(0));
+  check_ptr_table(kLayerPtrs, d.layers, "paged_gather_dequant(kLayerPtrs)", true);
+  check_ptr_table(vLayerPtrs, d.layers, "paged_gather_dequant(vLayerPtrs)", true);
+  TORCH_CHECK(kOut.size(2) <= INT32_MAX, op, ": too many heads");
+  d.k_layer_ptrs = reinterpret_cast<void *const *>(kLayerPtrs.data_ptr());
+  d.v_layer_ptrs = reinterpret_cast<void *const *>(vLayerPtrs.data_ptr());
+  d.k_out = kOut.data_ptr();
+  d.v_out = vOut.data_ptr();
+  d.total_tokens = kOut.size(1);
+  if (d.total_tokens == 0) return;  // an empty output has no address
+  d.token_bytes = kOut.size(2) * kOut.size(3);
+  d.out_layer_stride = kOut.stride(0) * kOut.element_size();
+  d.block_tables = blockTables.data_ptr();
+  d.seq_lens = seqLens.data_ptr();
+  d.ids_are_int64 = blockTables.scalar_type() == at::kLong ? 1 : 0;
+  d.num_seqs = blockTables.size(0);
+  d.max_blocks_per_seq = blockTables.size(1);
+  d.block_table_stride = std::max(blockTables.stride(0), blockTables.size(1));
+  d.block_size = blockSize;
+  d.device_block_stride = deviceBlockStride.has_value()
+                              ? deviceBlockStride.value()
+                              : static_cast<int64_t>(hfk_kv_block_bytes(blockSize, kOut.size(2), kOut.size(3), static_cast<int>(kvFormat)));
+  d.num_device_blocks = numDeviceBlocks;
+  const c10::cuda::CUDAGuard guard(dev);
+  check_rc(hfk_paged_gather_dequant(&d, static_cast<int>(kvFormat), static_cast<int>(kOut.size(2)), out_type, ctas,
+                                    at::cuda::getCurrentCUDAStream().stream()),
+           op);
+}
+
+static hfk_prefix_attention_desc attention_desc(const at::Tensor &q, int64_t prefixLen, const at::Tensor &blockTables, int64_t blockSize,
+                                                int64_t kvHeads, int64_t kvFormat, const char *op) {
+  TORCH_CHECK(q.dim() == 3 && (q.scalar_type() == at::kBFloat16 || q.scalar_type() == at::kHalf), op,
+              ": q must be a bfloat16 or float16 tensor [num_seqs, qHeads, headDim]");
+  TORCH_CHECK(kvHeads > 0 && q.size(1) > 0 && q.size(1) % kvHeads == 0 && q.size(1) <= INT32_MAX, op, ": ", q.size(1),
+              " query heads are not a multiple of kvHeads ", kvHeads);
+  TORCH_CHECK(blockTables.dim() == 2, op, ": blockTables must be [num_seqs, max_blocks]");
+  hfk_prefix_attention_desc d = {};
+  d.type = type_code(q.scalar_type());
+  d.kv_format = static_cast<int>(kvFormat);
+  d.kv_heads = static_cast<int>(kvHeads);
+  d.group = static_cast<int>(q.size(1) / kvHeads);
+  d.head_dim = static_cast<int>(std::min<int64_t>(q.size(2), INT32_MAX));
+  d.num_seqs = q.size(0);
+  d.prefix_len = prefixLen;
+  d.max_blocks_per_seq = blockTables.size(1);
+  d.block_table_stride = blockTables.size(0) > 1 ? blockTables.stride(0) : blockTables.size(1);
+  d.block_size = blockSize;
+  return d;
+}
+
+// Bytes of workspace for calls of this shape (a caller that keeps one workspace sizes it for its largest batch).
+int64_t shared_prefix_attention_workspace(const at::Tensor &q, int64_t prefixLen, const at::Tensor &blockTables, int64_t blockSize,
+                                          int64_t kvHeads, c10::optional<int64_t> aiv) {
+  const char *op = "shared_prefix_attention_workspace";
+  const hfk_prefix_attention_desc d = attention_desc(q, prefixLen, blockTables, blockSize, kvHeads, HFK_KV_RAW, op);
+  const c10::cuda::OptionalCUDAGuard guard(q.is_cuda() ? c10::optional<c10::Device>(q.device()) : c10::nullopt);
+  const size_t bytes = hfk_prefix_attention_workspace(&d, cores_from(aiv));
+  TORCH_CHECK(bytes > 0, op, ": ", hfk_last_error_message());
+  return static_cast<int64_t>(bytes);
+}
+
+void shared_prefix_attention(const at::Tensor &q, const at::Tensor &out, const at::Tensor &kCache, const at::Tensor &vCache,
+                             const at::Tensor &prefixTable, int64_t prefixLen, const at::Tensor &blockTables, const at::Tensor &seqLens,
+                             int64_t blockSize, int64_t kvHeads, int64_t kvFormat, c10::optional<double> scale,
+                             const c10::optional<at::Tensor> &lse, const c10::optional<at::Tensor> &workspace, c10::optional<int64_t> aiv) {
+  const char *op = "shared_prefix_attention";
+  const int ctas = cores_from(aiv);
+  hfk_prefix_attention_desc d = attention_desc(q, prefixLen, blockTables, blockSize, kvHeads, kvFormat, op);
+  TORCH_CHECK(q.is_cuda() && out.sizes() == q.sizes() && out.scalar_type() == q.scalar_type(), op,
+              ": q must be a device tensor and out must have its shape and dtype");
+  check_cache(kCache, vCache, q.scalar_type(), blockSize, kvHeads, q.size(2), kvFormat, op);
+  TORCH_CHECK(blockTables.scalar_type() == at::kLong || blockTables.scalar_type() == at::kInt, op, ": blockTables must be int64 or int32");
+  TORCH_CHECK(blockTables.size(0) == q.size(0) && (blockTables.stride(1) == 1 || blockTables.size(1) <= 1), op,
+              ": blockTables must be [num_seqs, max_blocks] with unit inner stride");
+  TORCH_CHECK(seqLens.dim() == 1 && seqLens.is_contiguous() && seqLens.size(0) == q.size(0) && prefixTable.dim() == 1 &&
+                  prefixTable.is_contiguous() && seqLens.scalar_type() == blockTables.scalar_type() &&
+                  prefixTable.scalar_type() == blockTables.scalar_type(),
+              op, ": seqLens must be [num_seqs] and prefixTable 1-D, contiguous, of the same dtype as blockTables");
+  TORCH_CHECK(prefixLen >= 0 && blockSize > 0, op, ": prefixLen must not be negative, blockSize must be positive");
+  TORCH_CHECK(prefixLen == 0 || prefixTable.numel() > (prefixLen - 1) / blockSize, op, ": prefixTable has ", prefixTable.numel(),
+              " pages, a prefix of ", prefixLen, " tokens needs ", prefixLen == 0 ? 0 : (prefixLen - 1) / blockSize + 1);
+  const auto dev = q.device();
+  TORCH_CHECK(out.device() == dev && kCache.device() == dev && prefixTable.device() == dev && blockTables.device() == dev && seqLens.device() == dev,
+              op, ": all tensors must be on one device");
+  d.q = rows_of(q, op, "q");
+  d.out = rows_of(out, op, "out");
+  if (lse.has_value() && lse->defined()) {
+    TORCH_CHECK(lse->device() == dev && lse->scalar_type() == at::kFloat && lse->is_contiguous() && lse->dim() == 2 &&
+                    lse->size(0) == q.size(0) && lse->size(1) == q.size(1),
+                op, ": lse must be a contiguous float32 tensor [num_seqs, qHeads]");
+    d.lse = lse->data_ptr<float>();
+  }
+  d.k_cache = kCache.data_ptr();
+  d.v_cache = vCache.data_ptr();
+  d.prefix_table = prefixTable.data_ptr();
+  d.block_tables = blockTables.data_ptr();
+  d.seq_lens = seqLens.data_ptr();
+  d.ids_are_int64 = blockTables.scalar_type() == at::kLong ? 1 : 0;
+  d.device_block_stride = kCache.stride(0) * kCache.element_size();
+  d.num_device_blocks = kCache.size(0);
+  d.scale = static_cast<float>(scale.has_value() ? scale.value() : 1.0 / std::sqrt(static_cast<double>(q.size(2))));
+  const c10::cuda::CUDAGuard guard(dev);
+  at::Tensor own;  // freed at return, when the work is enqueued: torch's allocator hands it on in stream order
+  if (workspace.has_value() && workspace->defined()) {
+    TORCH_CHECK(workspace->device() == dev && workspace->is_contiguous(), op, ": workspace must be a contiguous device tensor");
+    d.workspace = workspace->data_ptr();
+    d.workspace_bytes = workspace->nbytes();
+  } else {
+    const size_t bytes = hfk_prefix_attention_workspace(&d, ctas);
+    TORCH_CHECK(bytes > 0, op, ": ", hfk_last_error_message());
+    own = at::empty({static_cast<int64_t>(bytes)}, q.options().dtype(at::kByte));
+    d.workspace = own.data_ptr();
+    d.workspace_bytes = bytes;
+  }
+  check_rc(hfk_shared_prefix_attention(&d, ctas, at::cuda::getCurrentCUDAStream().stream()), op);
+}
+
 // Reads and clears the device status word of the current device (bits HFK_DEV_*).
 int64_t device_status() {
   unsigned int bits = 0;
@@ -445,6 +700,11 @@ TORCH_LIBRARY_FRAGMENT(pcie_through, m) {
   m.def("swap_in_relayout(Tensor layerPtrs, Tensor hostPool, Tensor deviceBlockIds, Tensor hostSlotIds, int numDeviceBlocks, int? deviceBlockStride=None, int? aiv=None) -> ()");
   m.def("swap_out_relayout(Tensor layerPtrs, Tensor hostPool, Tensor deviceBlockIds, Tensor hostSlotIds, int numDeviceBlocks, int? deviceBlockStride=None, int? aiv=None) -> ()");
   m.def("migrate_blocks(Tensor srcKLayerPtrs, Tensor srcVLayerPtrs, Tensor dstKLayerPtrs, Tensor dstVLayerPtrs, Tensor srcBlockIds, Tensor dstBlockIds, int blockBytes, int numSrcBlocks, int numDstBlocks, int? srcBlockStride=None, int? dstBlockStride=None, int? aiv=None) -> ()");
+  m.def("kv_write(Tensor k, Tensor v, Tensor kCache, Tensor vCache, Tensor slotIds, int blockSize, int kvFormat) -> ()");
+  m.def("qk_norm_rope_write(Tensor q, Tensor k, Tensor v, Tensor qOut, Tensor kCache, Tensor vCache, Tensor slotIds, Tensor positions, Tensor cosSin, int blockSize, int kvFormat, Tensor? qWeight=None, Tensor? kWeight=None, float eps=1e-6, bool interleaved=False) -> ()");
+  m.def("paged_gather_dequant(Tensor kLayerPtrs, Tensor vLayerPtrs, Tensor kOut, Tensor vOut, Tensor blockTables, Tensor seqLens, int blockSize, int numDeviceBlocks, int kvFormat, int? deviceBlockStride=None, int? aiv=None) -> ()");
+  m.def("shared_prefix_attention(Tensor q, Tensor out, Tensor kCache, Tensor vCache, Tensor prefixTable, int prefixLen, Tensor blockTables, Tensor seqLens, int blockSize, int kvHeads, int kvFormat, float? scale=None, Tensor? lse=None, Tensor? workspace=None, int? aiv=None) -> ()");
+  m.def("shared_prefix_attention_workspace(Tensor q, int prefixLen, Tensor blockTables, int blockSize, int kvHeads, int? aiv=None) -> int");
   m.def("device_status() -> int");
 }
 
@@ -460,6 +720,10 @@ TORCH_LIBRARY_IMPL(pcie_through, CUDA, m) {
   m.impl("swap_in_relayout", TORCH_FN(pciethrough::swap_in_relayout));
   m.impl("swap_out_relayout", TORCH_FN(pciethrough::swap_out_relayout));
   m.impl("migrate_blocks", TORCH_FN(pciethrough::migrate_blocks));
+  m.impl("kv_write", TORCH_FN(pciethrough::kv_write));
+  m.impl("qk_norm_rope_write", TORCH_FN(pciethrough::qk_norm_rope_write));
+  m.impl("paged_gather_dequant", TORCH_FN(pciethrough::paged_gather_dequant));
+  m.impl("shared_prefix_attention", TORCH_FN(pciethrough::shared_prefix_attention));
 }
 
 // all-CPU argument lists dispatch here; there is no CPU implementation of any
@@ -471,4 +735,5 @@ TORCH_LIBRARY_IMPL(pcie_through, CPU, m) {
 
 TORCH_LIBRARY_IMPL(pcie_through, CompositeExplicitAutograd, m) {
   m.impl("device_status", TORCH_FN(pciethrough::device_status));
+  m.impl("shared_prefix_attention_workspace", TORCH_FN(pciethrough::shared_prefix_attention_workspace));
 }

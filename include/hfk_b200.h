@@ -57,6 +57,7 @@ typedef struct CUstream_st *hfk_stream_t;
 #define HFK_DEV_BAD_SEQ_LEN 0x8u         /* sequence longer than its block table row */
 #define HFK_DEV_WAIT_TIMEOUT 0x10u       /* a bounded mbarrier wait gave up; the destination of that call is undefined */
 #define HFK_DEV_BAD_LAYER_PTR 0x20u      /* a layer base in a device pointer table is null or not 16-byte aligned */
+#define HFK_DEV_BAD_POSITION 0x40u       /* token position outside [0, max_positions) */
 
 const char *hfk_strerror(int code);
 const char *hfk_last_error_message(void);
@@ -422,6 +423,127 @@ typedef struct hfk_paged_gather_desc {
  * one launch. */
 int hfk_paged_gather(const hfk_paged_gather_desc *desc, int mover, int ctas,
                      hfk_stream_t stream);
+
+/* ======================================================================== *
+ *  Group A — filling, keeping and reading the cache of an attention layer
+ *  (no counterpart in the reference)
+ * ======================================================================== */
+
+/* What a page of one layer's K (or V) cache holds.
+ *   HFK_KV_RAW   [block_size][kv_heads][head_dim] of the 16-bit type of the call.
+ *   HFK_KV_E4M3, HFK_KV_INT8
+ *                codes [block_size][kv_heads][head_dim] of one byte, then fp32 scales
+ *                [block_size][kv_heads], padded to a multiple of 16 bytes; value = code * scale.
+ *                A page is one run of hfk_kv_block_bytes() bytes, so hfk_swap_out / hfk_swap_in /
+ *                hfk_swap_staged / hfk_migrate_blocks carry it with block_bytes set to that. */
+#define HFK_KV_RAW 0
+#define HFK_KV_E4M3 1
+#define HFK_KV_INT8 2
+
+/* 16-bit and fp32 element types of the calls below. */
+#define HFK_TYPE_BF16 0
+#define HFK_TYPE_FP16 1
+#define HFK_TYPE_FP32 2 /* hfk_paged_gather_dequant's output only */
+
+/* Bytes of one page, 0 when an argument is out of range. */
+size_t hfk_kv_block_bytes(int64_t block_size, int64_t kv_heads, int64_t head_dim, int kv_format);
+
+/* A tensor [tokens][heads][head_dim] with contiguous rows.  Strides in BYTES, multiples of 16, as the base. */
+typedef struct hfk_rows {
+  const void *base;
+  int64_t token_stride;
+  int64_t head_stride;
+} hfk_rows;
+
+typedef struct hfk_kv_write_desc {
+  hfk_rows k; /* [tokens][kv_heads][head_dim] */
+  hfk_rows v;
+  void *k_cache; /* one layer's cache, [num_device_blocks] pages */
+  void *v_cache;
+  const void *slot_ids; /* DEVICE [tokens]: block * block_size + place in the block; negative = padding */
+  int ids_are_int64;
+  int type;      /* HFK_TYPE_BF16 or HFK_TYPE_FP16: of k and v, and of a HFK_KV_RAW cache */
+  int kv_format; /* HFK_KV_* */
+  int kv_heads;
+  int head_dim; /* multiple of 16, at most 256 */
+  int64_t tokens;
+  int64_t block_size;
+  int64_t device_block_stride; /* bytes between pages (>= hfk_kv_block_bytes, multiple of 16) */
+  int64_t num_device_blocks;   /* num_device_blocks * block_size < 2^31 */
+} hfk_kv_write_desc;
+
+/* K and V rows of new tokens go to their pages, one layer.  8-bit formats, for each row (token, head):
+ *   scale = max(max|x| * (1 / top), 2^-126), code = round_to_nearest_even(x * (1 / scale)), top = 448 (e4m3), 127 (int8),
+ *   every step in fp32.
+ * A row with an infinity or a NaN reads back as NaN.  Slots of one call must be distinct.  A slot beyond the
+ * cache sets HFK_DEV_BAD_DEVICE_BLOCK_ID and its token is skipped.  tokens * 2 * kv_heads < 2^31. */
+int hfk_kv_write(const hfk_kv_write_desc *desc, hfk_stream_t stream);
+
+typedef struct hfk_norm_rope_desc {
+  hfk_rows q;     /* [tokens][q_heads][head_dim] */
+  hfk_rows q_out; /* written; may be q itself (same base and strides), must not overlap it otherwise */
+  int q_heads;
+  int rot_dim;              /* leading elements of a head that are rotated: 0, or a multiple of 16 up to head_dim */
+  int interleaved;          /* pairs (2i, 2i+1) instead of (i, i + rot_dim/2) */
+  int positions_are_int64;
+  const void *positions;    /* DEVICE [tokens] */
+  const float *cos_sin;     /* DEVICE [max_positions][rot_dim]: rot_dim/2 cosines, then the sines; 16-byte aligned */
+  int64_t max_positions;
+  const void *q_weight;     /* DEVICE [head_dim] of `type`, or NULL: no norm of the queries */
+  const void *k_weight;     /* the same for the keys */
+  float eps;
+} hfk_norm_rope_desc;
+
+/* hfk_kv_write after the norm of each query and key head (x * rsqrt(mean(x^2) + eps) * weight) and the rotation of
+ * its first rot_dim elements, in fp32 with one rounding at the end; the rotated queries go to q_out, the keys only
+ * to the cache.  A token with a negative slot is padding: neither its q_out row nor a page is written.  A position
+ * outside the table sets HFK_DEV_BAD_POSITION and its token is skipped.
+ * tokens * (q_heads + 2 * kv_heads) < 2^31. */
+int hfk_qk_norm_rope_write(const hfk_kv_write_desc *desc, const hfk_norm_rope_desc *norm_rope, hfk_stream_t stream);
+
+/* hfk_paged_gather of an 8-bit cache: value = code * scale, rounded once to out_type (any HFK_TYPE_*).  `gather` as
+ * for hfk_paged_gather, except that token_bytes is the codes of a token (kv_heads * head_dim), device_block_stride
+ * counts whole pages with their scales, and out_layer_stride is bytes of the output.  head_dim: multiple of 16. */
+int hfk_paged_gather_dequant(const hfk_paged_gather_desc *gather, int kv_format, int kv_heads, int out_type, int ctas,
+                             hfk_stream_t stream);
+
+typedef struct hfk_prefix_attention_desc {
+  hfk_rows q;   /* [num_seqs][kv_heads * group][head_dim] (token_stride = stride between sequences) */
+  hfk_rows out; /* written; the same shape; may be q itself (same base and strides), must not overlap it otherwise */
+  float *lse;   /* DEVICE [num_seqs][kv_heads * group]: log of the sum of exponentials, or NULL */
+  const void *k_cache; /* one layer's cache */
+  const void *v_cache;
+  const void *prefix_table; /* DEVICE: pages of the prefix all sequences share, ceil(prefix_len / block_size) ids */
+  const void *block_tables; /* DEVICE [num_seqs][max_blocks_per_seq]: pages of each sequence's own tokens */
+  const void *seq_lens;     /* DEVICE [num_seqs]: own tokens, the prefix not counted */
+  int ids_are_int64;        /* of the three */
+  int type;                 /* HFK_TYPE_BF16 or HFK_TYPE_FP16: of q and out, and of a HFK_KV_RAW cache */
+  int kv_format;
+  int kv_heads;
+  int group;    /* query heads to a K/V head */
+  int head_dim; /* 64 or 128 */
+  int64_t num_seqs;
+  int64_t prefix_len; /* tokens; 0 = none */
+  int64_t max_blocks_per_seq;
+  int64_t block_table_stride; /* elements */
+  int64_t block_size;
+  int64_t device_block_stride;
+  int64_t num_device_blocks;
+  float scale; /* of the scores; finite */
+  void *workspace; /* DEVICE, 256-byte aligned, hfk_prefix_attention_workspace() bytes; nothing in it needs clearing */
+  size_t workspace_bytes;
+} hfk_prefix_attention_desc;
+
+/* Bytes of workspace a call with this descriptor needs (pointers are not looked at); 0 when the descriptor is not
+ * valid.  Calls that may run at the same time need workspaces of their own. */
+size_t hfk_prefix_attention_workspace(const hfk_prefix_attention_desc *desc, int ctas);
+
+/* One new token of each sequence attends to the shared prefix and to the sequence's own tokens, one layer:
+ *   out[s, h*group + g] = softmax(scale * q . [Kprefix[h]; K_s[h]]) [Vprefix[h]; V_s[h]]
+ * The prefix is read for all sequences together.  A length outside 0 .. max_blocks_per_seq * block_size is clamped and
+ * sets HFK_DEV_BAD_SEQ_LEN; a page id outside the cache sets HFK_DEV_BAD_DEVICE_BLOCK_ID and its keys are left out.
+ * A row without keys is 0, its lse -infinity. */
+int hfk_shared_prefix_attention(const hfk_prefix_attention_desc *desc, int ctas, hfk_stream_t stream);
 
 #ifdef __cplusplus
 }
