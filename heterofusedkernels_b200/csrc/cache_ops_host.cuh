@@ -4,6 +4,7 @@
 
 #include "kv_write.cuh"
 #include "paged_gather_dequant.cuh"
+#include "prefix_tensor.cuh"
 #include "shared_prefix_attention.cuh"
 
 namespace hfk {
@@ -218,11 +219,13 @@ static int gather_dequant_impl(const hfk_paged_gather_desc *d, int kv_format, in
 }
 
 // ---- attention -----------------------------------------------------------------------------------------------------
-// Batches above HFK_MAX_SEQS go out as several pairs of launches, which use the workspace in turn.
+// Batches above HFK_MAX_SEQS go out as several groups of launches, which use the workspace in turn.
 struct AttnPlan {
-  int ctas;
-  size_t cu_bytes, ml_bytes, o_bytes;
-  size_t bytes() const { return cu_bytes + ml_bytes + o_bytes; }
+  bool tensor;      // the prefix goes to prefix_tensor_kernel
+  int splits;       // its runs of key tiles
+  int ctas;         // of the line
+  size_t cu_bytes, ml_bytes, o_bytes, prefix_ml_bytes, prefix_o_bytes;
+  size_t bytes() const { return cu_bytes + ml_bytes + o_bytes + prefix_ml_bytes + prefix_o_bytes; }
 };
 
 static int plan_attention(const hfk_prefix_attention_desc *d, int ctas, AttnPlan *p) {
@@ -236,35 +239,85 @@ static int plan_attention(const hfk_prefix_attention_desc *d, int ctas, AttnPlan
   if (d->block_size > most || d->prefix_len > most || (d->max_blocks_per_seq > 0 && d->max_blocks_per_seq > most / d->block_size))
     return fail(HFK_ERR_TOO_LARGE, "%s: more than 2^31 keys", op);
   if (d->num_seqs >= (int64_t)1 << 30) return fail(HFK_ERR_TOO_LARGE, "%s: too many sequences", op);
+  const int sms = sm_count();
   const int seqs = (int)std::min<int64_t>(d->num_seqs, HFK_MAX_SEQS);
-  p->ctas = ctas > 0 ? std::min(ctas, 65535) : sm_count() * kAttnCtasPerSm;
-  const AttnLine line(seqs, d->kv_heads, d->group, (int)d->prefix_len);
-  const size_t parts = (size_t)p->ctas + (size_t)line.items(seqs);
-  p->cu_bytes = ((size_t)(seqs + 1) * sizeof(int64_t) + 255) & ~(size_t)255;
-  p->ml_bytes = parts * 16 * sizeof(float2);
-  p->o_bytes = parts * 16 * d->head_dim * sizeof(float);
+  const int64_t rows = (int64_t)seqs * d->group;
+  p->tensor = d->prefix_len > 0 && rows > kPrefixTensorMinRows;
+  p->splits = 0;
+  if (p->tensor) {
+    // as many runs as give the least time for the slowest SM: waves of CTAs, each its key tiles and a constant for
+    // filling the pipeline and writing the part
+    const int64_t items = d->kv_heads * ((rows + 255) / 256), tiles = (d->prefix_len + kPtKeys - 1) / kPtKeys;
+    const int64_t room = ctas > 0 ? std::min(ctas, sms) : sms;
+    int64_t best = 0;
+    for (int64_t s = 1; s <= std::min<int64_t>(tiles, std::max<int64_t>(1, 2 * room / items)); ++s) {
+      const int64_t cost = ((items * s + room - 1) / room) * ((tiles + s - 1) / s + kPrefixTileOverhead);
+      if (p->splits == 0 || cost < best) {
+        best = cost;
+        p->splits = (int)s;
+      }
+    }
+  }
+  p->ctas = d->max_blocks_per_seq == 0 && p->tensor ? 0 : ctas > 0 ? std::min(ctas, 65535) : sms * kAttnCtasPerSm;
+  const AttnLine line(seqs, d->kv_heads, d->group, p->tensor ? 0 : (int)d->prefix_len);
+  const size_t parts = p->ctas > 0 ? (size_t)p->ctas + (size_t)line.items(seqs) : 0;
+  const auto round = [](size_t n) { return (n + 255) & ~(size_t)255; };
+  p->cu_bytes = round((size_t)(seqs + 1) * sizeof(int64_t));
+  p->ml_bytes = round(parts * 16 * sizeof(float2));
+  p->o_bytes = round(parts * 16 * d->head_dim * sizeof(float));
+  p->prefix_ml_bytes = round((size_t)p->splits * d->kv_heads * rows * sizeof(float2));
+  p->prefix_o_bytes = round((size_t)p->splits * d->kv_heads * rows * d->head_dim * sizeof(float));
   return HFK_OK;
 }
 
 template <typename T, int kFmt, int D>
-static cudaError_t launch_attention(const AttnArgs &a, int ctas, cudaStream_t s) {
-  const size_t smem = 4 * 16 * (D * sizeof(float) + sizeof(float2)) + (size_t)(a.seqs + 1) * sizeof(int64_t);
-  shared_prefix_attention_kernel<T, kFmt, D><<<ctas, 128, smem, s>>>(a);
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return e;
+static cudaError_t launch_attention(const AttnArgs &a, const AttnPlan &p, unsigned char *w, cudaStream_t s) {
+  JoinArgs join = {};
+  join.a = a;
+  join.grid = p.ctas;
+  join.rows = a.seqs * a.group;
+  join.a.cu = reinterpret_cast<int64_t *>(w);
+  join.a.part_ml = reinterpret_cast<float2 *>(w + p.cu_bytes);
+  join.a.part_o = reinterpret_cast<float *>(w + p.cu_bytes + p.ml_bytes);
+  cudaError_t e;
+  if (p.tensor) {
+    PrefixTensorArgs t = {};
+    t.a = a;
+    t.a.scale_log2 = std::abs(a.scale_log2);
+    t.negate = a.scale_log2 < 0.f;
+    t.rows = join.rows;
+    t.row_blocks = (t.rows + 255) / 256;
+    t.splits = p.splits;
+    t.part_ml = reinterpret_cast<float2 *>(w + p.cu_bytes + p.ml_bytes + p.o_bytes);
+    t.part_o = reinterpret_cast<float *>(w + p.cu_bytes + p.ml_bytes + p.o_bytes + p.prefix_ml_bytes);
+    auto k = prefix_tensor_kernel<T, kFmt, D>;
+    const size_t smem = sizeof(PrefixSmem<D>) + 1024;
+    if ((e = allow_smem(k, smem)) != cudaSuccess) return e;
+    k<<<a.kv_heads * t.row_blocks * t.splits, kPtThreads, smem, s>>>(t);
+    if ((e = cudaGetLastError()) != cudaSuccess) return e;
+    join.a.prefix_len = 0;
+    join.splits = t.splits;
+    join.prefix_ml = t.part_ml;
+    join.prefix_o = t.part_o;
+  }
+  if (p.ctas > 0) {
+    const size_t smem = 4 * 16 * (D * sizeof(float) + sizeof(float2)) + (size_t)(a.seqs + 1) * sizeof(int64_t);
+    shared_prefix_attention_kernel<T, kFmt, D><<<p.ctas, 128, smem, s>>>(join.a);
+    if ((e = cudaGetLastError()) != cudaSuccess) return e;
+  }
   const int rows = a.seqs * a.kv_heads * a.group;
-  shared_prefix_join_kernel<T, D><<<(rows + 3) / 4, 128, 0, s>>>(a, ctas);
+  shared_prefix_join_kernel<T, D><<<(rows + 3) / 4, 128, 0, s>>>(join);
   return cudaGetLastError();
 }
 template <typename T, int kFmt>
-static cudaError_t launch_attention(const AttnArgs &a, int head_dim, int ctas, cudaStream_t s) {
-  return head_dim == 64 ? launch_attention<T, kFmt, 64>(a, ctas, s) : launch_attention<T, kFmt, 128>(a, ctas, s);
+static cudaError_t launch_attention(const AttnArgs &a, int head_dim, const AttnPlan &p, unsigned char *w, cudaStream_t s) {
+  return head_dim == 64 ? launch_attention<T, kFmt, 64>(a, p, w, s) : launch_attention<T, kFmt, 128>(a, p, w, s);
 }
 template <typename T>
-static cudaError_t launch_attention(const AttnArgs &a, int fmt, int head_dim, int ctas, cudaStream_t s) {
-  if (fmt == HFK_KV_E4M3) return launch_attention<T, kFmtE4m3>(a, head_dim, ctas, s);
-  if (fmt == HFK_KV_INT8) return launch_attention<T, kFmtInt8>(a, head_dim, ctas, s);
-  return launch_attention<T, kFmtRaw>(a, head_dim, ctas, s);
+static cudaError_t launch_attention(const AttnArgs &a, int fmt, int head_dim, const AttnPlan &p, unsigned char *w, cudaStream_t s) {
+  if (fmt == HFK_KV_E4M3) return launch_attention<T, kFmtE4m3>(a, head_dim, p, w, s);
+  if (fmt == HFK_KV_INT8) return launch_attention<T, kFmtInt8>(a, head_dim, p, w, s);
+  return launch_attention<T, kFmtRaw>(a, head_dim, p, w, s);
 }
 
 static int attention_impl(const hfk_prefix_attention_desc *d, int ctas, cudaStream_t stream) {
@@ -307,9 +360,6 @@ static int attention_impl(const hfk_prefix_attention_desc *d, int ctas, cudaStre
   a.block = FastDiv::make((uint32_t)d->block_size);
   a.scale_log2 = d->scale * kLog2e;
   unsigned char *w = static_cast<unsigned char *>(d->workspace);
-  a.cu = reinterpret_cast<int64_t *>(w);
-  a.part_ml = reinterpret_cast<float2 *>(w + p.cu_bytes);
-  a.part_o = reinterpret_cast<float *>(w + p.cu_bytes + p.ml_bytes);
   const int64_t id = d->ids_are_int64 ? 8 : 4;
   for (int64_t first = 0; first < d->num_seqs; first += HFK_MAX_SEQS) {
     a.seqs = (int)std::min<int64_t>(HFK_MAX_SEQS, d->num_seqs - first);
@@ -318,8 +368,8 @@ static int attention_impl(const hfk_prefix_attention_desc *d, int ctas, cudaStre
     a.lse = d->lse ? d->lse + first * a.kv_heads * a.group : nullptr;
     a.tables = static_cast<const unsigned char *>(d->block_tables) + first * d->block_table_stride * id;
     a.lens = static_cast<const unsigned char *>(d->seq_lens) + first * id;
-    const cudaError_t e = d->type == HFK_TYPE_BF16 ? launch_attention<__nv_bfloat16>(a, d->kv_format, d->head_dim, p.ctas, stream)
-                                                   : launch_attention<__half>(a, d->kv_format, d->head_dim, p.ctas, stream);
+    const cudaError_t e = d->type == HFK_TYPE_BF16 ? launch_attention<__nv_bfloat16>(a, d->kv_format, d->head_dim, p, w, stream)
+                                                   : launch_attention<__half>(a, d->kv_format, d->head_dim, p, w, stream);
     if (e != cudaSuccess) return cuda_fail(e, "shared_prefix_attention launch");
   }
   return HFK_OK;

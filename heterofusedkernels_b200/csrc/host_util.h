@@ -54,5 +54,9 @@ constexpr int kMigrateCtasPerSm = 2;
 constexpr int kGatherDequantCtasPerSm = 4;
 // Attention: 128-thread CTAs per SM (about 200 registers a thread).
 constexpr int kAttnCtasPerSm = 2;
+// Rows of queries (sequences x query heads of a K/V head) above which the prefix goes to the tensor-core kernel, and
+// what a CTA of it costs beyond its key tiles, in tiles.
+constexpr int kPrefixTensorMinRows = 32;
+constexpr int kPrefixTileOverhead = 3;
 
 }  // namespace hfk

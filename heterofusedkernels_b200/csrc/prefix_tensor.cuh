@@ -1,0 +1,485 @@
+// The shared prefix on the 5th-generation tensor cores: from a few dozen rows of queries on, reading the prefix once
+// for all of them is a pair of matrix products (queries x keys, weights x values) with a softmax between.
+//
+// A CTA takes up to 256 rows of one K/V head (two tiles of 128, one TMEM lane a row) against a run of key tiles
+// of 128, and leaves a partial result (m, l, o).  Thirteen warps:
+//   0-3, 4-7  softmax of tile 0 and of tile 1: one thread a row, so neither the maximum nor the sum needs a shuffle
+//   8-11      bring K and V tiles into shared memory (asynchronous copies; 8-bit codes are widened on the way)
+//   12        issues the matrix products
+// TMEM: scores of the two tiles (128 columns each), o of the two tiles (head_dim columns each).  The 16-bit weights
+// take the place of the scores they came from, and the second product reads them from there.  While one tile is
+// in its softmax, the tensor cores work on the other: per 128 keys and tile, at head_dim 128, both products take about
+// 1024 clocks of the tensor cores and the 128 x 128 exponentials 1024 clocks of the special function units.
+//
+// o is rescaled only where a row's maximum rises by more than 2^8 above the one in use: weights up to 2^8 are as
+// exact as weights up to 1, and l and o stay in the same units, so nothing is lost.
+//
+// Operand layouts: rows of 128 bytes (64 values), 16-byte chunks XORed with the row number mod 8 ("128-byte swizzle"),
+// head_dim 128 as two such halves.  The same bytes serve K (rows = keys, read along the row) and V (rows = keys, read
+// across the rows: the transposed form of the operand).
+#pragma once
+
+#include "shared_prefix_attention.cuh"
+
+namespace hfk {
+
+struct PrefixTensorArgs {
+  AttnArgs a;
+  int rows;          // seqs * group
+  int row_blocks;    // ceil(rows / 256)
+  int splits;        // runs the prefix's key tiles are cut into
+  int negate;        // scale < 0: queries are negated, so the maximum of the scores is that of the products
+  float2 *part_ml;   // [splits][kv_heads * rows]
+  float *part_o;     // [splits][kv_heads * rows][head_dim]
+};
+
+constexpr int kPtThreads = 416, kPtRows = 128, kPtKeys = 128, kPtStages = 4, kPtMeta = 4;
+
+template <int D>
+struct PrefixSmem {
+  static constexpr int kTile = kPtKeys * D * 2;  // bytes of a tile of queries, keys or values
+  unsigned char q[2][kTile];
+  unsigned char ring[kPtStages][kTile];          // K of tile i in stage 2 (i % 2), V in the next
+  int64_t off[kPtMeta][kPtKeys];                 // byte offset of a key's row, -1: leave out
+  alignas(16) float sk[kPtMeta][kPtKeys];         // scales of keys (times scale * log2 e) and of values, 0: leave out
+  alignas(16) float sv[kPtMeta][kPtKeys];
+  uint32_t valid[kPtMeta][4];
+  uint64_t full[kPtStages], empty[kPtStages], meta[kPtMeta], s_full[2], p_full[2], o_full, q_full;
+  uint32_t tmem;
+  int failed;
+};
+
+// ---- tcgen05 ------------------------------------------------------------------------------------------------
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_commit(uint64_t *bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
+}
+// Shared-memory operand, 128-byte swizzle: start, distance of 64-value blocks (only where the operand is read across
+// its rows), distance of 8-row groups (1024 bytes).
+__device__ __forceinline__ uint64_t tc_operand(uint32_t addr, uint32_t block_bytes) {
+  return (uint64_t)((addr >> 4) & 0x3fff) | ((uint64_t)(block_bytes >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+// fp32 accumulators, M = 128; b_across: B is read across its rows.
+template <typename T>
+__device__ __forceinline__ constexpr uint32_t tc_instruction(int n, bool b_across) {
+  const uint32_t type = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+  return (1u << 4) | (type << 7) | (type << 10) | ((b_across ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((128u >> 4) << 24);
+}
+__device__ __forceinline__ void tc_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t instr, bool add) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a),
+               "l"(b), "r"(instr), "r"((uint32_t)add)
+               : "memory");
+}
+__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t instr, bool add) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a),
+               "l"(b), "r"(instr), "r"((uint32_t)add)
+               : "memory");
+}
+// 32 columns of this warp's 32 lanes
+__device__ __forceinline__ void tc_load32(uint32_t addr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,"
+      "%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+        "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
+        "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]),
+        "=r"(r[31])
+      : "r"(addr));
+}
+__device__ __forceinline__ void tc_store32(uint32_t addr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,"
+      "%26,%27,%28,%29,%30,%31};" ::"r"(r[0]),
+      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]),
+      "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]),
+      "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(addr));
+}
+__device__ __forceinline__ void tc_store16(uint32_t addr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]),
+      "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
+      "r"(addr));
+}
+__device__ __forceinline__ void tc_wait_load() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tc_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool ok) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kLeft>
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory"); }
+
+// Byte of 16-byte chunk `chunk` of row `row` in a tile (8 chunks to a 128-byte row, halves behind each other).
+__device__ __forceinline__ uint32_t tile_at(int row, int chunk) {
+  return (uint32_t)((chunk >> 3) * (kPtKeys * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4));
+}
+
+template <typename T, int kFmt, int D>
+__global__ void __launch_bounds__(kPtThreads, 1) prefix_tensor_kernel(const __grid_constant__ PrefixTensorArgs args) {
+  extern __shared__ __align__(128) unsigned char smem_raw[];
+  using Smem = PrefixSmem<D>;
+  // operands want 1024-byte alignment
+  Smem &sm = *reinterpret_cast<Smem *>(smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023));
+  const AttnArgs &a = args.a;
+  constexpr bool kWide = kFmt != kFmtRaw;
+  constexpr bool kUnits = kWide && std::is_same<T, __half>::value;  // see shared_prefix_attention_kernel
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  const int split = blockIdx.x % args.splits;
+  const int item = blockIdx.x / args.splits;
+  const int h = item / args.row_blocks;
+  const int row0 = (item - h * args.row_blocks) * 256;
+  const int rows = min(256, args.rows - row0);
+  const int tiles = rows > kPtRows ? 2 : 1;
+  const int key_tiles = (a.prefix_len + kPtKeys - 1) / kPtKeys;
+  const int first = (int)((int64_t)key_tiles * split / args.splits);
+  const int n = (int)((int64_t)key_tiles * (split + 1) / args.splits) - first;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kPtStages; ++i) {
+      mbar_init(&sm.full[i], 128);
+      mbar_init(&sm.empty[i], 1);
+    }
+    for (int i = 0; i < kPtMeta; ++i) mbar_init(&sm.meta[i], 128);
+    for (int j = 0; j < 2; ++j) {
+      mbar_init(&sm.s_full[j], 1);
+      mbar_init(&sm.p_full[j], 128);
+    }
+    mbar_init(&sm.o_full, 1);
+    mbar_init(&sm.q_full, 128);
+    sm.failed = 0;
+    mbar_fence_init();
+  }
+  if (warp == 12) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&sm.tmem)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    tc_fence_before();
+  }
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(&sm.tmem);
+  auto wait = [&](uint64_t *bar, uint32_t parity) -> bool {
+    if (mbar_wait_bounded(bar, parity)) return true;
+    raise_status(HFK_DEV_WAIT_TIMEOUT);
+    *reinterpret_cast<volatile int *>(&sm.failed) = 1;
+    return false;
+  };
+
+  if (warp >= 8 && warp < 12) {
+    // ---------------------------------------------------------------- loads ---
+    const int p = threadIdx.x - 256;
+    // queries, rows behind the last one zero
+    {
+      const uint32_t flip = args.negate ? 0x80008000u : 0u;
+      for (int c = p; c < tiles * kPtRows * (D / 8); c += 128) {
+        const int row = c / (D / 8), chunk = c % (D / 8);
+        uint4 w = make_uint4(0, 0, 0, 0);
+        if (row < rows) {
+          const int r = row0 + row, s = r / a.group;
+          w = *reinterpret_cast<const uint4 *>(a.q + s * a.q_seq + (int64_t)(h * a.group + r - s * a.group) * a.q_head + chunk * 16);
+          w.x ^= flip;
+          w.y ^= flip;
+          w.z ^= flip;
+          w.w ^= flip;
+        }
+        *reinterpret_cast<uint4 *>(&sm.q[row / kPtRows][tile_at(row % kPtRows, chunk)]) = w;
+      }
+      fence_async_proxy();
+      mbar_arrive(&sm.q_full);
+    }
+    // key p of a tile: where its row is
+    auto page_of = [&](int i) -> int64_t {
+      const int64_t key = (int64_t)(first + i) * kPtKeys + p;
+      return i < n && key < a.prefix_len ? load_id(a.prefix_table, a.ids_are_int64, a.block.div((uint32_t)key)) : -1;
+    };
+    auto write_meta = [&](int i, int64_t id) {
+      const int64_t key = (int64_t)(first + i) * kPtKeys + p;
+      const bool inside = key < a.prefix_len;
+      const bool ok = inside && id >= 0 && id < a.num_blocks;
+      if (inside && !ok) raise_status(HFK_DEV_BAD_DEVICE_BLOCK_ID);
+      const uint32_t row = ((uint32_t)key - a.block.div((uint32_t)key) * a.block.d) * a.kv_heads + h;
+      const int m = i % kPtMeta;
+      sm.off[m][p] = ok ? id * a.block_stride + (int64_t)row * (D * (kWide ? 1 : 2)) : -1;
+      if (kWide) {
+        sm.sk[m][p] = ok ? reinterpret_cast<const float *>(a.k_cache + id * a.block_stride + a.scales_at)[row] * a.scale_log2 : 0.f;
+        sm.sv[m][p] = ok ? reinterpret_cast<const float *>(a.v_cache + id * a.block_stride + a.scales_at)[row] : 0.f;
+      }
+      const uint32_t word = __ballot_sync(0xffffffffu, ok);
+      if (lane == 0) sm.valid[m][p >> 5] = word;
+      mbar_arrive(&sm.meta[m]);
+    };
+    auto producers = [&]() { asm volatile("bar.sync 1, 128;" ::: "memory"); };
+    int64_t next = page_of(0);
+    if constexpr (!kWide) {
+      constexpr int kChunks = D / 8;             // 16-byte chunks of a row
+      constexpr int kRowsPass = 128 / kChunks;   // rows of a pass over the 128 threads
+      const int chunk = p % kChunks, row_in = p / kChunks;
+      int pending = -1;                          // stage whose copies are in flight and not yet announced
+      auto announce = [&]() {
+        fence_async_proxy();
+        mbar_arrive(&sm.full[pending]);
+      };
+      for (int i = 0; i < n; ++i) {
+        write_meta(i, next);
+        next = page_of(i + 1);
+        producers();
+        bool ok = true;
+        for (int v = 0; v < 2 && ok; ++v) {
+          const int stage = (i & 1) * 2 + v;
+          const uint32_t parity = ((i >> 1) & 1) ^ 1;
+          if (!mbar_try_wait(&sm.empty[stage], parity)) {   // nothing free: what has arrived goes out first
+            if (pending >= 0) {
+              cp_async_wait<0>();
+              announce();
+              pending = -1;
+            }
+            ok = wait(&sm.empty[stage], parity);
+            if (!ok) break;
+          }
+          const unsigned char *cache = v ? a.v_cache : a.k_cache;
+          const uint32_t base = smem_addr(sm.ring[stage]);
+#pragma unroll
+          for (int r = 0; r < kPtKeys; r += kRowsPass) {
+            const int64_t off = sm.off[i % kPtMeta][r + row_in];
+            cp_async16(base + tile_at(r + row_in, chunk), cache + (off < 0 ? 0 : off) + chunk * 16, off >= 0);
+          }
+          cp_async_commit();
+          if (pending >= 0) {
+            cp_async_wait<1>();
+            announce();
+          }
+          pending = stage;
+        }
+        if (!ok) break;
+      }
+      cp_async_wait<0>();
+      if (pending >= 0) announce();
+    } else {
+      constexpr int kChunks = D / 16;            // 16-byte chunks of codes of a row
+      constexpr int kRowsPass = 128 / kChunks;
+      constexpr int kPasses = kPtKeys / kRowsPass;
+      const int chunk = p % kChunks, row_in = p / kChunks;
+      uint4 codes[kPasses];
+      auto fetch = [&](int i, int v) {
+        const unsigned char *cache = v ? a.v_cache : a.k_cache;
+#pragma unroll
+        for (int r = 0; r < kPasses; ++r) {
+          const int64_t off = sm.off[i % kPtMeta][r * kRowsPass + row_in];
+          codes[r] = make_uint4(0, 0, 0, 0);
+          if (off >= 0) codes[r] = *reinterpret_cast<const uint4 *>(cache + off + chunk * 16);
+        }
+      };
+      if (n > 0) {
+        write_meta(0, next);
+        next = page_of(1);
+        producers();
+        fetch(0, 0);
+      }
+      for (int u = 0; u < 2 * n; ++u) {
+        const int i = u >> 1, v = u & 1, stage = (i & 1) * 2 + v;
+        if (!wait(&sm.empty[stage], ((i >> 1) & 1) ^ 1)) break;
+        unsigned char *ring = sm.ring[stage];
+#pragma unroll
+        for (int r = 0; r < kPasses; ++r) {
+          const uint32_t w[4] = {codes[r].x, codes[r].y, codes[r].z, codes[r].w};
+          uint32_t x[8];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) codes_to_pairs<T, kFmt>(w[k], x[2 * k], x[2 * k + 1]);
+          const int row = r * kRowsPass + row_in;
+          *reinterpret_cast<uint4 *>(ring + tile_at(row, 2 * chunk)) = make_uint4(x[0], x[1], x[2], x[3]);
+          *reinterpret_cast<uint4 *>(ring + tile_at(row, 2 * chunk + 1)) = make_uint4(x[4], x[5], x[6], x[7]);
+        }
+        fence_async_proxy();
+        mbar_arrive(&sm.full[stage]);
+        if (v == 0) {
+          fetch(i, 1);
+        } else if (i + 1 < n) {
+          write_meta(i + 1, next);
+          next = page_of(i + 2);
+          producers();
+          fetch(i + 1, 0);
+        }
+      }
+    }
+  } else if (warp == 12) {
+    // ------------------------------------------------------------- products ---
+    if (lane == 0 && n > 0) {
+      constexpr uint32_t kScores = tc_instruction<T>(kPtKeys, false), kValues = tc_instruction<T>(D, true);
+      bool ok = wait(&sm.q_full, 0);
+      auto values = [&](int j, int i) {          // o_j += weights_j . V_i
+        const uint32_t v = smem_addr(sm.ring[(i & 1) * 2 + 1]);
+        tc_fence_after();
+#pragma unroll
+        for (int k = 0; k < kPtKeys / 16; ++k)
+          tc_mma_ts(tmem + 256 + j * D, tmem + j * 128 + k * 8, tc_operand(v + k * 2048, kPtKeys * 128), kValues, i > 0 || k > 0);
+      };
+      for (int i = 0; i < n && ok; ++i) {
+        const int stage = (i & 1) * 2;
+        ok = wait(&sm.full[stage], (i >> 1) & 1);
+        if (ok && i > 0) ok = wait(&sm.full[((i - 1) & 1) * 2 + 1], ((i - 1) >> 1) & 1);
+        const uint32_t kk = smem_addr(sm.ring[stage]);
+        for (int j = 0; j < tiles && ok; ++j) {
+          if (i > 0) {
+            ok = wait(&sm.p_full[j], (i - 1) & 1);
+            if (!ok) break;
+            values(j, i - 1);
+          }
+          tc_fence_after();
+          const uint32_t q = smem_addr(sm.q[j]);
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k) {
+            const uint32_t at = (k >> 2) * (kPtKeys * 128) + (k & 3) * 32;
+            tc_mma_ss(tmem + j * 128, tc_operand(q + at, 16), tc_operand(kk + at, 16), kScores, k > 0);
+          }
+          tc_commit(&sm.s_full[j]);
+        }
+        if (!ok) break;
+        tc_commit(&sm.empty[stage]);
+        if (i > 0) tc_commit(&sm.empty[((i - 1) & 1) * 2 + 1]);
+      }
+      if (ok) ok = wait(&sm.full[((n - 1) & 1) * 2 + 1], ((n - 1) >> 1) & 1);
+      for (int j = 0; j < tiles && ok; ++j) {
+        ok = wait(&sm.p_full[j], (n - 1) & 1);
+        if (ok) values(j, n - 1);
+      }
+      tc_commit(&sm.o_full);                     // also after a failure: nothing is in flight when the CTA ends
+      wait(&sm.o_full, 0);
+    }
+    __syncwarp();
+  } else if (warp / 4 < tiles) {
+    // -------------------------------------------------------------- softmax ---
+    const int j = warp / 4;
+    const uint32_t lanes = (uint32_t)(warp % 4) << 21;   // first TMEM lane of this warp, in bits 16 and up
+    const uint32_t s_at = tmem + j * 128 + lanes, o_at = tmem + 256 + j * D + lanes;
+    float m = -INFINITY, l = 0.f, ref = 0.f;
+    bool ok = true;
+    for (int i = 0; i < n; ++i) {
+      const int mt = i % kPtMeta;
+      ok = wait(&sm.meta[mt], (i / kPtMeta) & 1) && wait(&sm.s_full[j], i & 1);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      tc_fence_after();
+      const uint32_t valid[4] = {sm.valid[mt][0], sm.valid[mt][1], sm.valid[mt][2], sm.valid[mt][3]};
+      uint32_t s[32];
+      float top = -INFINITY;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        tc_load32(s_at + c * 32, s);
+        tc_wait_load();
+        const bool all = valid[c] == 0xffffffffu;
+#pragma unroll
+        for (int e = 0; e < 32; e += 4) {
+          float4 f = make_float4(1.f, 1.f, 1.f, 1.f);
+          if (kWide) f = *reinterpret_cast<const float4 *>(&sm.sk[mt][c * 32 + e]);
+          const float x[4] = {__uint_as_float(s[e]) * f.x, __uint_as_float(s[e + 1]) * f.y, __uint_as_float(s[e + 2]) * f.z,
+                              __uint_as_float(s[e + 3]) * f.w};
+          if (all) {
+            top = fmaxf(fmaxf(top, fmaxf(x[0], x[1])), fmaxf(x[2], x[3]));
+          } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              if (valid[c] >> (e + k) & 1) top = fmaxf(top, x[k]);
+          }
+        }
+      }
+      if (!kWide) top *= a.scale_log2;           // not negative; 0 * -inf of a tile without keys is put right below
+      if (!(valid[0] | valid[1] | valid[2] | valid[3])) top = -INFINITY;
+      // the maximum in use, and whether o has to follow
+      float factor = 1.f;
+      if (top > m + 8.f || m == -INFINITY) {
+        factor = m == -INFINITY ? 0.f : ex2(m - top);
+        m = top;
+        l *= factor;
+      }
+      float unit = 1.f;
+      if (kUnits) {
+        float big = max_nan(max_nan(sm.sv[mt][lane], sm.sv[mt][lane + 32]), max_nan(sm.sv[mt][lane + 64], sm.sv[mt][lane + 96]));
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) big = max_nan(big, __shfl_xor_sync(0xffffffffu, big, d));
+        if (!(big <= 4.f * ref)) {               // also a NaN
+          factor *= big == 0.f ? 1.f : ref / big;
+          ref = big;
+        }
+        __syncwarp();
+        unit = ref == 0.f ? 0.f : 1.f / ref;
+      }
+      if (i > 0 && __any_sync(0xffffffffu, factor != 1.f)) {
+        // the product that wrote o last is complete: the scores waited for were issued behind it
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) {
+          tc_load32(o_at + c * 32, s);
+          tc_wait_load();
+#pragma unroll
+          for (int e = 0; e < 32; ++e) s[e] = __float_as_uint(__uint_as_float(s[e]) * factor);
+          tc_store32(o_at + c * 32, s);
+        }
+      }
+      const float safe = m == -INFINITY ? 0.f : m;
+      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        tc_load32(s_at + c * 32, s);
+        tc_wait_load();
+        uint32_t w[16];
+#pragma unroll
+        for (int e = 0; e < 32; e += 4) {
+          float4 f = make_float4(a.scale_log2, a.scale_log2, a.scale_log2, a.scale_log2);
+          if (kWide) f = *reinterpret_cast<const float4 *>(&sm.sk[mt][c * 32 + e]);
+          float x[4] = {ex2(fmaf(__uint_as_float(s[e]), f.x, -safe)), ex2(fmaf(__uint_as_float(s[e + 1]), f.y, -safe)),
+                        ex2(fmaf(__uint_as_float(s[e + 2]), f.z, -safe)), ex2(fmaf(__uint_as_float(s[e + 3]), f.w, -safe))};
+          if (valid[c] != 0xffffffffu) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              if (!(valid[c] >> (e + k) & 1)) x[k] = 0.f;
+          }
+#pragma unroll
+          for (int k = 0; k < 4; ++k) sum[k] += x[k];
+          if (kWide) {
+            const float4 g = *reinterpret_cast<const float4 *>(&sm.sv[mt][c * 32 + e]);
+            x[0] *= kUnits ? g.x * unit : g.x;
+            x[1] *= kUnits ? g.y * unit : g.y;
+            x[2] *= kUnits ? g.z * unit : g.z;
+            x[3] *= kUnits ? g.w * unit : g.w;
+          }
+          w[e / 2] = Pair<T>::pack(x[0], x[1]);
+          w[e / 2 + 1] = Pair<T>::pack(x[2], x[3]);
+        }
+        tc_store16(s_at + c * 16, w);            // over scores that have been read
+      }
+      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      tc_wait_store();
+      tc_fence_before();
+      mbar_arrive(&sm.p_full[j]);
+    }
+    if (ok && n > 0) ok = wait(&sm.o_full, 0);
+    ok = __all_sync(0xffffffffu, ok);
+    if (ok) {
+      tc_fence_after();
+      const int row = j * kPtRows + (warp % 4) * 32 + lane;
+      const int64_t part = (int64_t)split * a.kv_heads * args.rows + (int64_t)h * args.rows + row0 + row;
+      if (row < rows) args.part_ml[part] = make_float2(m, l);
+      uint32_t s[32];
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c) {
+        tc_load32(o_at + c * 32, s);
+        tc_wait_load();
+        if (row < rows) {
+          float4 *dst = reinterpret_cast<float4 *>(args.part_o + part * D + c * 32);
+          const float unit = kUnits ? ref : 1.f;
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            dst[e] = make_float4(__uint_as_float(s[4 * e]) * unit, __uint_as_float(s[4 * e + 1]) * unit, __uint_as_float(s[4 * e + 2]) * unit,
+                                 __uint_as_float(s[4 * e + 3]) * unit);
+        }
+        __syncwarp();
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 12) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+}
+
+}  // namespace hfk

@@ -461,44 +461,69 @@ __global__ void __launch_bounds__(128) shared_prefix_attention_kernel(const __gr
   }
 }
 
-// Joins the parts of every row; one warp a row.
+// Joins the parts of every row; one warp a row.  Up to three lists of parts: of the prefix's item and of the
+// sequence's item on the line, and of the prefix's runs from prefix_tensor_kernel.
+struct JoinArgs {
+  AttnArgs a;               // as the line's kernel had it: prefix_len 0 where the prefix went to the tensor kernel
+  int grid;                 // CTAs of the line, 0: no line
+  int splits, rows;         // of the tensor kernel; splits 0: not used
+  const float2 *prefix_ml;
+  const float *prefix_o;
+};
+
 template <typename T, int D>
-__global__ void __launch_bounds__(128) shared_prefix_join_kernel(const __grid_constant__ AttnArgs a, int grid) {
+__global__ void __launch_bounds__(128) shared_prefix_join_kernel(const __grid_constant__ JoinArgs args) {
+  const AttnArgs &a = args.a;
   const int row = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   const int q_heads = a.kv_heads * a.group;
   if (row >= a.seqs * q_heads) return;
   const int s = row / q_heads, head = row - s * q_heads, h = head / a.group, g = head - h * a.group;
-  const AttnLine line(a.seqs, a.kv_heads, a.group, a.prefix_len);
-  const int64_t in_prefix = (int64_t)line.prefix_items * line.prefix_tiles;
-  const int64_t total = in_prefix + a.cu[a.seqs] * line.per_seq;
-  const int64_t ctas = line_ctas(grid, total);
-  // parts of the row's two items: numbers first..last, row inside the part
-  int64_t first[2], last[2];
-  int place[2];
+  // list k: parts at ml[k] + step_ml i, o[k] + step_o i, i < count[k]
+  int64_t count[3] = {0, 0, 0};
+  const float2 *ml[3] = {nullptr, nullptr, nullptr};
+  const float *o_at[3] = {nullptr, nullptr, nullptr};
+  if (args.grid > 0) {
+    const AttnLine line(a.seqs, a.kv_heads, a.group, a.prefix_len);
+    const int64_t in_prefix = (int64_t)line.prefix_items * line.prefix_tiles;
+    const int64_t total = in_prefix + a.cu[a.seqs] * line.per_seq;
+    const int64_t ctas = line_ctas(args.grid, total);
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    int64_t item, from, tiles;
-    if (k == 0) {
-      const int r = s * a.group + g;
-      item = (int64_t)h * line.row_tiles + r / 16;
-      place[k] = r % 16;
-      from = item * line.prefix_tiles;
-      tiles = line.prefix_tiles;
-    } else {
-      const int hg = h * line.own_tiles + g / 16;
-      place[k] = g % 16;
-      tiles = a.cu[s + 1] - a.cu[s];
-      from = in_prefix + a.cu[s] * line.per_seq + hg * tiles;
-      item = line.prefix_items + (int64_t)s * line.per_seq + hg;
+    for (int k = 0; k < 2; ++k) {
+      int64_t item, from, tiles;
+      int place;
+      if (k == 0) {
+        const int r = s * a.group + g;
+        item = (int64_t)h * line.row_tiles + r / 16;
+        place = r % 16;
+        from = item * line.prefix_tiles;
+        tiles = line.prefix_tiles;
+      } else {
+        const int hg = h * line.own_tiles + g / 16;
+        place = g % 16;
+        tiles = a.cu[s + 1] - a.cu[s];
+        from = in_prefix + a.cu[s] * line.per_seq + hg * tiles;
+        item = line.prefix_items + (int64_t)s * line.per_seq + hg;
+      }
+      if (tiles > 0) {
+        // CTA c has [total c / ctas, total (c+1) / ctas): the one with tile x is floor((ctas (x+1) - 1) / total)
+        const int64_t first = (ctas * (from + 1) - 1) / total, last = (ctas * (from + tiles) - 1) / total;
+        count[k] = last - first + 1;
+        ml[k] = a.part_ml + (first + item) * 16 + place;
+        o_at[k] = a.part_o + ((first + item) * 16 + place) * D;
+      }
     }
-    // CTA c has [total c / ctas, total (c+1) / ctas): the one with tile x is floor((ctas (x+1) - 1) / total)
-    first[k] = tiles > 0 ? (ctas * (from + 1) - 1) / total + item : 0;
-    last[k] = tiles > 0 ? (ctas * (from + tiles) - 1) / total + item : -1;
+  }
+  const int64_t step[3] = {16, 16, (int64_t)a.kv_heads * args.rows};
+  if (args.splits > 0) {
+    const int64_t r = (int64_t)h * args.rows + s * a.group + g;
+    count[2] = args.splits;
+    ml[2] = args.prefix_ml + r;
+    o_at[2] = args.prefix_o + r * D;
   }
   float big = -INFINITY;
 #pragma unroll
-  for (int k = 0; k < 2; ++k)
-    for (int64_t p = first[k] + lane; p <= last[k]; p += 32) big = fmaxf(big, a.part_ml[p * 16 + place[k]].x);
+  for (int k = 0; k < 3; ++k)
+    for (int64_t i = lane; i < count[k]; i += 32) big = fmaxf(big, ml[k][i * step[k]].x);
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, d));
   constexpr int kPer = D / 32;
@@ -506,14 +531,15 @@ __global__ void __launch_bounds__(128) shared_prefix_join_kernel(const __grid_co
 #pragma unroll
   for (int i = 0; i < kPer; ++i) o[i] = 0.f;
 #pragma unroll
-  for (int k = 0; k < 2; ++k)
-    for (int64_t p = first[k]; p <= last[k]; ++p) {
-      const float2 ml = a.part_ml[p * 16 + place[k]];
-      const float f = big == -INFINITY ? 1.f : ex2(ml.x - big);
-      l += ml.y * f;
-      const float *src = a.part_o + (p * 16 + place[k]) * D + lane * kPer;
+  for (int k = 0; k < 3; ++k)
+#pragma unroll 4
+    for (int64_t i = 0; i < count[k]; ++i) {
+      const float2 x = ml[k][i * step[k]];
+      const float f = big == -INFINITY ? 1.f : ex2(x.x - big);
+      l += x.y * f;
+      const float *src = o_at[k] + i * step[k] * D + lane * kPer;
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) o[i] += src[i] * f;
+      for (int e = 0; e < kPer; ++e) o[e] += src[e] * f;
     }
   const float inv = l == 0.f ? 0.f : 1.f / l;   // a NaN stays
   unsigned char *dst = a.out + s * a.out_seq + (int64_t)head * a.out_head + lane * kPer * 2;
