@@ -37,6 +37,7 @@ constexpr int kPtThreads = 416, kPtRows = 128, kPtKeys = 128, kPtStages = 4, kPt
 
 template <int D>
 struct PrefixSmem {
+  // at the end the first bytes take the 256 rows of o, D * 4 + 16 bytes each
   static constexpr int kTile = kPtKeys * D * 2;  // bytes of a tile of queries, keys or values
   unsigned char q[2][kTile];
   unsigned char ring[kPtStages][kTile];          // K of tile i in stage 2 (i % 2), V in the next
@@ -48,6 +49,8 @@ struct PrefixSmem {
   uint32_t tmem;
   int failed;
 };
+static_assert(256 * (128 * 4 + 16) <= 2 * PrefixSmem<128>::kTile + kPtStages * PrefixSmem<128>::kTile, "o fits");
+static_assert(256 * (64 * 4 + 16) <= 2 * PrefixSmem<64>::kTile + kPtStages * PrefixSmem<64>::kTile, "o fits");
 
 // ---- tcgen05 ------------------------------------------------------------------------------------------------
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -116,6 +119,112 @@ __device__ __forceinline__ uint32_t tile_at(int row, int chunk) {
   return (uint32_t)((chunk >> 3) * (kPtKeys * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4));
 }
 
+// ---- the softmax's arithmetic, two columns an instruction ---------------------------------------------------------
+__device__ __forceinline__ uint64_t pair_of(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ float2 of_pair(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) { return fmaxf(fmaxf(a, b), c); }
+
+// o of this warp's rows times a factor of each row
+template <int D>
+__device__ __forceinline__ void rescale(uint32_t o_at, float factor) {
+#pragma unroll 1
+  for (int c = 0; c < D / 32; ++c) {
+    uint32_t s[32];
+    tc_load32(o_at + c * 32, s);
+    tc_wait_load();
+#pragma unroll
+    for (int e = 0; e < 32; ++e) s[e] = __float_as_uint(__uint_as_float(s[e]) * factor);
+    tc_store32(o_at + c * 32, s);
+  }
+}
+
+// Largest score of the tile (in units of log2 e), -inf without a key.
+template <typename T, int kFmt, bool kMask>
+__device__ __forceinline__ float tile_max(uint32_t s_at, const float *sk, float scale, const uint32_t (&valid)[4]) {
+  float top = -INFINITY;
+#pragma unroll 1
+  for (int c = 0; c < 4; ++c) {
+    uint32_t s[32];
+    tc_load32(s_at + c * 32, s);
+    tc_wait_load();
+#pragma unroll
+    for (int e = 0; e < 32; ++e)
+      if (!kMask || (valid[c] >> e & 1)) top = fmaxf(top, __uint_as_float(s[e]) * (kFmt == kFmtRaw ? scale : sk[c * 32 + e]));
+  }
+  return top;
+}
+
+// Weights 2^(score - m) of the tile's 128 keys, packed in pairs, times the values' scales; their sum before that;
+// returns the largest score - m.
+template <typename T, int kFmt, bool kUnits, bool kMask>
+__device__ __forceinline__ float tile_weights(uint32_t s_at, const float *sk, const float *sv, float scale, float m, float unit,
+                                              const uint32_t (&valid)[4], uint32_t (&w)[64], float &sum) {
+  const float safe = m == -INFINITY ? 0.f : m;
+  const uint64_t minus = pair_of(-safe, -safe), factor = pair_of(scale, scale), units = pair_of(unit, unit);
+  uint64_t total[2] = {0, 0};
+  float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    uint32_t s[32];
+    tc_load32(s_at + c * 32, s);
+    tc_wait_load();
+#pragma unroll
+    for (int e = 0; e < 32; e += 4) {
+      float4 f, g;
+      if (kFmt != kFmtRaw) {
+        f = *reinterpret_cast<const float4 *>(sk + c * 32 + e);
+        g = *reinterpret_cast<const float4 *>(sv + c * 32 + e);
+      }
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const uint64_t score = pair_of(__uint_as_float(s[e + 2 * k]), __uint_as_float(s[e + 2 * k + 1]));
+        const uint64_t by = kFmt == kFmtRaw ? factor : k == 0 ? pair_of(f.x, f.y) : pair_of(f.z, f.w);
+        float2 x = of_pair(fma2(score, by, minus));
+        if (kMask) {
+          if (!(valid[c] >> (e + 2 * k) & 1)) x.x = -INFINITY;
+          if (!(valid[c] >> (e + 2 * k + 1) & 1)) x.y = -INFINITY;
+        }
+        top[k] = max3(top[k], x.x, x.y);
+        uint64_t p = pair_of(ex2(x.x), ex2(x.y));
+        total[k] = add2(total[k], p);
+        if (kFmt != kFmtRaw) {
+          uint64_t by_v = k == 0 ? pair_of(g.x, g.y) : pair_of(g.z, g.w);
+          if (kUnits) by_v = mul2(by_v, units);
+          p = mul2(p, by_v);
+        }
+        const float2 y = of_pair(p);
+        w[c * 16 + e / 2 + k] = Pair<T>::pack(y.x, y.y);
+      }
+    }
+  }
+  const float2 t = of_pair(add2(total[0], total[1]));
+  sum = t.x + t.y;
+  return fmaxf(top[0], top[1]);
+}
+
 template <typename T, int kFmt, int D>
 __global__ void __launch_bounds__(kPtThreads, 1) prefix_tensor_kernel(const __grid_constant__ PrefixTensorArgs args) {
   extern __shared__ __align__(128) unsigned char smem_raw[];
@@ -148,7 +257,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) prefix_tensor_kernel(const __gr
       mbar_init(&sm.p_full[j], 128);
     }
     mbar_init(&sm.o_full, 1);
-    mbar_init(&sm.q_full, 128);
+    mbar_init(&sm.q_full, tiles * 128);
     sm.failed = 0;
     mbar_fence_init();
   }
@@ -170,48 +279,46 @@ __global__ void __launch_bounds__(kPtThreads, 1) prefix_tensor_kernel(const __gr
   if (warp >= 8 && warp < 12) {
     // ---------------------------------------------------------------- loads ---
     const int p = threadIdx.x - 256;
-    // queries, rows behind the last one zero
-    {
-      const uint32_t flip = args.negate ? 0x80008000u : 0u;
-      for (int c = p; c < tiles * kPtRows * (D / 8); c += 128) {
-        const int row = c / (D / 8), chunk = c % (D / 8);
-        uint4 w = make_uint4(0, 0, 0, 0);
-        if (row < rows) {
-          const int r = row0 + row, s = r / a.group;
-          w = *reinterpret_cast<const uint4 *>(a.q + s * a.q_seq + (int64_t)(h * a.group + r - s * a.group) * a.q_head + chunk * 16);
-          w.x ^= flip;
-          w.y ^= flip;
-          w.z ^= flip;
-          w.w ^= flip;
-        }
-        *reinterpret_cast<uint4 *>(&sm.q[row / kPtRows][tile_at(row % kPtRows, chunk)]) = w;
-      }
-      fence_async_proxy();
-      mbar_arrive(&sm.q_full);
-    }
     // key p of a tile: where its row is
     auto page_of = [&](int i) -> int64_t {
       const int64_t key = (int64_t)(first + i) * kPtKeys + p;
       return i < n && key < a.prefix_len ? load_id(a.prefix_table, a.ids_are_int64, a.block.div((uint32_t)key)) : -1;
     };
-    auto write_meta = [&](int i, int64_t id) {
+    // ... and what it is multiplied by: loaded a tile ahead of its use
+    struct Key {
+      int64_t off;
+      float sk, sv;
+      bool ok;
+    };
+    auto key_of = [&](int i, int64_t id) -> Key {
       const int64_t key = (int64_t)(first + i) * kPtKeys + p;
-      const bool inside = key < a.prefix_len;
-      const bool ok = inside && id >= 0 && id < a.num_blocks;
-      if (inside && !ok) raise_status(HFK_DEV_BAD_DEVICE_BLOCK_ID);
+      const bool inside = i < n && key < a.prefix_len;
+      Key k;
+      k.ok = inside && id >= 0 && id < a.num_blocks;
+      if (inside && !k.ok) raise_status(HFK_DEV_BAD_DEVICE_BLOCK_ID);
       const uint32_t row = ((uint32_t)key - a.block.div((uint32_t)key) * a.block.d) * a.kv_heads + h;
-      const int m = i % kPtMeta;
-      sm.off[m][p] = ok ? id * a.block_stride + (int64_t)row * (D * (kWide ? 1 : 2)) : -1;
-      if (kWide) {
-        sm.sk[m][p] = ok ? reinterpret_cast<const float *>(a.k_cache + id * a.block_stride + a.scales_at)[row] * a.scale_log2 : 0.f;
-        sm.sv[m][p] = ok ? reinterpret_cast<const float *>(a.v_cache + id * a.block_stride + a.scales_at)[row] : 0.f;
+      k.off = k.ok ? id * a.block_stride + (int64_t)row * (D * (kWide ? 1 : 2)) : -1;
+      k.sk = k.sv = 0.f;
+      if (kWide && k.ok) {
+        k.sk = reinterpret_cast<const float *>(a.k_cache + id * a.block_stride + a.scales_at)[row];
+        k.sv = reinterpret_cast<const float *>(a.v_cache + id * a.block_stride + a.scales_at)[row];
       }
-      const uint32_t word = __ballot_sync(0xffffffffu, ok);
+      return k;
+    };
+    auto write_meta = [&](int i, const Key &k) {
+      const int m = i % kPtMeta;
+      sm.off[m][p] = k.off;
+      if (kWide) {
+        sm.sk[m][p] = k.sk * a.scale_log2;
+        sm.sv[m][p] = k.sv;
+      }
+      const uint32_t word = __ballot_sync(0xffffffffu, k.ok);
       if (lane == 0) sm.valid[m][p >> 5] = word;
       mbar_arrive(&sm.meta[m]);
     };
     auto producers = [&]() { asm volatile("bar.sync 1, 128;" ::: "memory"); };
-    int64_t next = page_of(0);
+    Key key = key_of(0, page_of(0));
+    int64_t next = page_of(1);
     if constexpr (!kWide) {
       constexpr int kChunks = D / 8;             // 16-byte chunks of a row
       constexpr int kRowsPass = 128 / kChunks;   // rows of a pass over the 128 threads
@@ -222,8 +329,9 @@ __global__ void __launch_bounds__(kPtThreads, 1) prefix_tensor_kernel(const __gr
         mbar_arrive(&sm.full[pending]);
       };
       for (int i = 0; i < n; ++i) {
-        write_meta(i, next);
-        next = page_of(i + 1);
+        write_meta(i, key);
+        key = key_of(i + 1, next);
+        next = page_of(i + 2);
         producers();
         bool ok = true;
         for (int v = 0; v < 2 && ok; ++v) {
@@ -261,29 +369,26 @@ __global__ void __launch_bounds__(kPtThreads, 1) prefix_tensor_kernel(const __gr
       constexpr int kRowsPass = 128 / kChunks;
       constexpr int kPasses = kPtKeys / kRowsPass;
       const int chunk = p % kChunks, row_in = p / kChunks;
-      uint4 codes[kPasses];
-      auto fetch = [&](int i, int v) {
+      // codes of the next K and the next V tile in registers: each has a whole tile's time to arrive
+      uint4 codes[2][kPasses];
+      auto fetch = [&](int i, auto which) {
+        constexpr int v = decltype(which)::value;
         const unsigned char *cache = v ? a.v_cache : a.k_cache;
 #pragma unroll
         for (int r = 0; r < kPasses; ++r) {
           const int64_t off = sm.off[i % kPtMeta][r * kRowsPass + row_in];
-          codes[r] = make_uint4(0, 0, 0, 0);
-          if (off >= 0) codes[r] = *reinterpret_cast<const uint4 *>(cache + off + chunk * 16);
+          codes[v][r] = make_uint4(0, 0, 0, 0);
+          if (off >= 0) codes[v][r] = *reinterpret_cast<const uint4 *>(cache + off + chunk * 16);
         }
       };
-      if (n > 0) {
-        write_meta(0, next);
-        next = page_of(1);
-        producers();
-        fetch(0, 0);
-      }
-      for (int u = 0; u < 2 * n; ++u) {
-        const int i = u >> 1, v = u & 1, stage = (i & 1) * 2 + v;
-        if (!wait(&sm.empty[stage], ((i >> 1) & 1) ^ 1)) break;
+      auto widen = [&](int i, auto which) -> bool {
+        constexpr int v = decltype(which)::value;
+        const int stage = (i & 1) * 2 + v;
+        if (!wait(&sm.empty[stage], ((i >> 1) & 1) ^ 1)) return false;
         unsigned char *ring = sm.ring[stage];
 #pragma unroll
         for (int r = 0; r < kPasses; ++r) {
-          const uint32_t w[4] = {codes[r].x, codes[r].y, codes[r].z, codes[r].w};
+          const uint32_t w[4] = {codes[v][r].x, codes[v][r].y, codes[v][r].z, codes[v][r].w};
           uint32_t x[8];
 #pragma unroll
           for (int k = 0; k < 4; ++k) codes_to_pairs<T, kFmt>(w[k], x[2 * k], x[2 * k + 1]);
@@ -293,14 +398,27 @@ __global__ void __launch_bounds__(kPtThreads, 1) prefix_tensor_kernel(const __gr
         }
         fence_async_proxy();
         mbar_arrive(&sm.full[stage]);
-        if (v == 0) {
-          fetch(i, 1);
-        } else if (i + 1 < n) {
-          write_meta(i + 1, next);
-          next = page_of(i + 2);
-          producers();
-          fetch(i + 1, 0);
+        return true;
+      };
+      constexpr std::integral_constant<int, 0> kK{};
+      constexpr std::integral_constant<int, 1> kV{};
+      auto announce_tile = [&](int i) {          // tile i's rows are known to all four warps
+        write_meta(i, key);
+        key = key_of(i + 1, next);
+        next = page_of(i + 2);
+        producers();
+      };
+      announce_tile(0);
+      fetch(0, kK);
+      fetch(0, kV);
+      for (int i = 0; i < n; ++i) {
+        if (!widen(i, kK)) break;
+        if (i + 1 < n) {
+          announce_tile(i + 1);
+          fetch(i + 1, kK);
         }
+        if (!widen(i, kV)) break;
+        if (i + 1 < n) fetch(i + 1, kV);
       }
     }
   } else if (warp == 12) {
@@ -355,6 +473,24 @@ __global__ void __launch_bounds__(kPtThreads, 1) prefix_tensor_kernel(const __gr
     const uint32_t s_at = tmem + j * 128 + lanes, o_at = tmem + 256 + j * D + lanes;
     float m = -INFINITY, l = 0.f, ref = 0.f;
     bool ok = true;
+    {                                            // this thread's row of queries, zero behind the last one
+      const int at = threadIdx.x - j * kPtRows, row = j * kPtRows + at;
+      const uint32_t flip = args.negate ? 0x80008000u : 0u;
+      const int r = row0 + row, sq = r / a.group;
+      const unsigned char *src = a.q + sq * a.q_seq + (int64_t)(h * a.group + r - sq * a.group) * a.q_head;
+      uint4 w[D / 8];
+#pragma unroll
+      for (int c = 0; c < D / 8; ++c) {
+        w[c] = make_uint4(0, 0, 0, 0);
+        if (row < rows) w[c] = *reinterpret_cast<const uint4 *>(src + c * 16);
+      }
+#pragma unroll
+      for (int c = 0; c < D / 8; ++c)
+        *reinterpret_cast<uint4 *>(&sm.q[j][tile_at(at, c)]) = make_uint4(w[c].x ^ flip, w[c].y ^ flip, w[c].z ^ flip, w[c].w ^ flip);
+      fence_async_proxy();
+      mbar_arrive(&sm.q_full);
+      __syncwarp();
+    }
     for (int i = 0; i < n; ++i) {
       const int mt = i % kPtMeta;
       ok = wait(&sm.meta[mt], (i / kPtMeta) & 1) && wait(&sm.s_full[j], i & 1);
@@ -362,93 +498,43 @@ __global__ void __launch_bounds__(kPtThreads, 1) prefix_tensor_kernel(const __gr
       if (!ok) break;
       tc_fence_after();
       const uint32_t valid[4] = {sm.valid[mt][0], sm.valid[mt][1], sm.valid[mt][2], sm.valid[mt][3]};
-      uint32_t s[32];
-      float top = -INFINITY;
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        tc_load32(s_at + c * 32, s);
-        tc_wait_load();
-        const bool all = valid[c] == 0xffffffffu;
-#pragma unroll
-        for (int e = 0; e < 32; e += 4) {
-          float4 f = make_float4(1.f, 1.f, 1.f, 1.f);
-          if (kWide) f = *reinterpret_cast<const float4 *>(&sm.sk[mt][c * 32 + e]);
-          const float x[4] = {__uint_as_float(s[e]) * f.x, __uint_as_float(s[e + 1]) * f.y, __uint_as_float(s[e + 2]) * f.z,
-                              __uint_as_float(s[e + 3]) * f.w};
-          if (all) {
-            top = fmaxf(fmaxf(top, fmaxf(x[0], x[1])), fmaxf(x[2], x[3]));
-          } else {
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              if (valid[c] >> (e + k) & 1) top = fmaxf(top, x[k]);
-          }
-        }
-      }
-      if (!kWide) top *= a.scale_log2;           // not negative; 0 * -inf of a tile without keys is put right below
-      if (!(valid[0] | valid[1] | valid[2] | valid[3])) top = -INFINITY;
-      // the maximum in use, and whether o has to follow
-      float factor = 1.f;
-      if (top > m + 8.f || m == -INFINITY) {
-        factor = m == -INFINITY ? 0.f : ex2(m - top);
-        m = top;
-        l *= factor;
+      const bool all = (valid[0] & valid[1] & valid[2] & valid[3]) == 0xffffffffu;
+      if (__any_sync(0xffffffffu, m == -INFINITY)) {
+        // rows without a maximum yet (the first tile; tiles whose pages are bad)
+        const float top = all ? tile_max<T, kFmt, false>(s_at, sm.sk[mt], a.scale_log2, valid) : tile_max<T, kFmt, true>(s_at, sm.sk[mt], a.scale_log2, valid);
+        if (m == -INFINITY) m = top;
+        __syncwarp();
       }
       float unit = 1.f;
       if (kUnits) {
         float big = max_nan(max_nan(sm.sv[mt][lane], sm.sv[mt][lane + 32]), max_nan(sm.sv[mt][lane + 64], sm.sv[mt][lane + 96]));
 #pragma unroll
         for (int d = 16; d > 0; d >>= 1) big = max_nan(big, __shfl_xor_sync(0xffffffffu, big, d));
-        if (!(big <= 4.f * ref)) {               // also a NaN
-          factor *= big == 0.f ? 1.f : ref / big;
+        if (!(big <= 4.f * ref)) {               // also a NaN; the same for every row
+          if (i > 0) rescale<D>(o_at, ref / big);
           ref = big;
         }
         __syncwarp();
         unit = ref == 0.f ? 0.f : 1.f / ref;
       }
-      if (i > 0 && __any_sync(0xffffffffu, factor != 1.f)) {
-        // the product that wrote o last is complete: the scores waited for were issued behind it
-#pragma unroll
-        for (int c = 0; c < D / 32; ++c) {
-          tc_load32(o_at + c * 32, s);
-          tc_wait_load();
-#pragma unroll
-          for (int e = 0; e < 32; ++e) s[e] = __float_as_uint(__uint_as_float(s[e]) * factor);
-          tc_store32(o_at + c * 32, s);
-        }
+      uint32_t w[64];
+      float sum;
+      float top = all ? tile_weights<T, kFmt, kUnits, false>(s_at, sm.sk[mt], sm.sv[mt], a.scale_log2, m, unit, valid, w, sum)
+                      : tile_weights<T, kFmt, kUnits, true>(s_at, sm.sk[mt], sm.sv[mt], a.scale_log2, m, unit, valid, w, sum);
+      if (__any_sync(0xffffffffu, top > 8.f)) {
+        // a maximum rose too far: o and l follow, and the weights are taken again (the scores are still there)
+        const float rise = top > 8.f ? top : 0.f, factor = ex2(-rise);
+        m = m == -INFINITY ? m : m + rise;
+        l *= factor;
+        if (i > 0) rescale<D>(o_at, factor);
+        if (all)
+          tile_weights<T, kFmt, kUnits, false>(s_at, sm.sk[mt], sm.sv[mt], a.scale_log2, m, unit, valid, w, sum);
+        else
+          tile_weights<T, kFmt, kUnits, true>(s_at, sm.sk[mt], sm.sv[mt], a.scale_log2, m, unit, valid, w, sum);
       }
-      const float safe = m == -INFINITY ? 0.f : m;
-      float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        tc_load32(s_at + c * 32, s);
-        tc_wait_load();
-        uint32_t w[16];
-#pragma unroll
-        for (int e = 0; e < 32; e += 4) {
-          float4 f = make_float4(a.scale_log2, a.scale_log2, a.scale_log2, a.scale_log2);
-          if (kWide) f = *reinterpret_cast<const float4 *>(&sm.sk[mt][c * 32 + e]);
-          float x[4] = {ex2(fmaf(__uint_as_float(s[e]), f.x, -safe)), ex2(fmaf(__uint_as_float(s[e + 1]), f.y, -safe)),
-                        ex2(fmaf(__uint_as_float(s[e + 2]), f.z, -safe)), ex2(fmaf(__uint_as_float(s[e + 3]), f.w, -safe))};
-          if (valid[c] != 0xffffffffu) {
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              if (!(valid[c] >> (e + k) & 1)) x[k] = 0.f;
-          }
-#pragma unroll
-          for (int k = 0; k < 4; ++k) sum[k] += x[k];
-          if (kWide) {
-            const float4 g = *reinterpret_cast<const float4 *>(&sm.sv[mt][c * 32 + e]);
-            x[0] *= kUnits ? g.x * unit : g.x;
-            x[1] *= kUnits ? g.y * unit : g.y;
-            x[2] *= kUnits ? g.z * unit : g.z;
-            x[3] *= kUnits ? g.w * unit : g.w;
-          }
-          w[e / 2] = Pair<T>::pack(x[0], x[1]);
-          w[e / 2 + 1] = Pair<T>::pack(x[2], x[3]);
-        }
-        tc_store16(s_at + c * 16, w);            // over scores that have been read
-      }
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      l += sum;
+      tc_store32(s_at, *reinterpret_cast<uint32_t (*)[32]>(&w[0]));      // the weights take the scores' place
+      tc_store32(s_at + 32, *reinterpret_cast<uint32_t (*)[32]>(&w[32]));
       tc_wait_store();
       tc_fence_before();
       mbar_arrive(&sm.p_full[j]);
@@ -457,23 +543,32 @@ __global__ void __launch_bounds__(kPtThreads, 1) prefix_tensor_kernel(const __gr
     ok = __all_sync(0xffffffffu, ok);
     if (ok) {
       tc_fence_after();
-      const int row = j * kPtRows + (warp % 4) * 32 + lane;
+      // The part's rows lie one behind the other, but a thread that stored its row would touch a line of its own with
+      // every instruction: the row goes to shared memory (the tiles are done with; 16 bytes of skew a row, so eight
+      // lanes hit eight bank groups) and from there as one copy.
+      const int at = threadIdx.x, row = at;
+      unsigned char *mine = sm.q[0] + at * (D * 4 + 16);
       const int64_t part = (int64_t)split * a.kv_heads * args.rows + (int64_t)h * args.rows + row0 + row;
       if (row < rows) args.part_ml[part] = make_float2(m, l);
-      uint32_t s[32];
+      const float unit = kUnits ? ref : 1.f;
+      uint32_t buf[2][32];
+      tc_load32(o_at, buf[0]);
 #pragma unroll
       for (int c = 0; c < D / 32; ++c) {
-        tc_load32(o_at + c * 32, s);
+        uint32_t (&s)[32] = buf[c & 1];
         tc_wait_load();
-        if (row < rows) {
-          float4 *dst = reinterpret_cast<float4 *>(args.part_o + part * D + c * 32);
-          const float unit = kUnits ? ref : 1.f;
+        if (c + 1 < D / 32) tc_load32(o_at + (c + 1) * 32, buf[(c + 1) & 1]);
 #pragma unroll
-          for (int e = 0; e < 8; ++e)
-            dst[e] = make_float4(__uint_as_float(s[4 * e]) * unit, __uint_as_float(s[4 * e + 1]) * unit, __uint_as_float(s[4 * e + 2]) * unit,
-                                 __uint_as_float(s[4 * e + 3]) * unit);
-        }
-        __syncwarp();
+        for (int e = 0; e < 8; ++e)
+          *reinterpret_cast<float4 *>(mine + c * 128 + e * 16) =
+              make_float4(__uint_as_float(s[4 * e]) * unit, __uint_as_float(s[4 * e + 1]) * unit, __uint_as_float(s[4 * e + 2]) * unit,
+                          __uint_as_float(s[4 * e + 3]) * unit);
+      }
+      fence_async_proxy();
+      if (row < rows) {
+        bulk_store(args.part_o + part * D, mine, D * 4);
+        bulk_commit();
+        bulk_wait_all();
       }
     }
   }
