@@ -2,10 +2,13 @@
 // for all of them is a pair of matrix products (queries x keys, weights x values) with a softmax between.
 //
 // A CTA takes up to 256 rows of one K/V head (two tiles of 128, one TMEM lane a row) against a run of key tiles
-// of 128, and leaves a partial result (m, l, o).  Thirteen warps:
+// of 128, and leaves a partial result (m, l, o).  Four groups of four warps:
 //   0-3, 4-7  softmax of tile 0 and of tile 1: one thread a row, so neither the maximum nor the sum needs a shuffle
 //   8-11      bring K and V tiles into shared memory (asynchronous copies; 8-bit codes are widened on the way)
-//   12        issues the matrix products
+//   12        issues the matrix products (13-15 only bring their registers)
+// A thread starts with 128 registers; the softmax keeps the 64 words of its row's weights at once and would spill (what it
+// spilled went to L2, shared memory leaves no L1: 64 us instead of 59 for 2048 rows x 32768 keys), so the groups split
+// the registers 168 + 168 + 120 + 56 = 4 x 128.
 // TMEM: scores of the two tiles (128 columns each), o of the two tiles (head_dim columns each).  The 16-bit weights
 // take the place of the scores they came from, and the second product reads them from there.  While one tile is
 // in its softmax, the tensor cores work on the other: per 128 keys and tile, at head_dim 128, both products take about
@@ -33,7 +36,7 @@ struct PrefixTensorArgs {
   float *part_o;     // [splits][kv_heads * rows][head_dim]
 };
 
-constexpr int kPtThreads = 416, kPtRows = 128, kPtKeys = 128, kPtStages = 4, kPtMeta = 4;
+constexpr int kPtThreads = 512, kPtRows = 128, kPtKeys = 128, kPtStages = 4, kPtMeta = 4;
 
 template <int D>
 struct PrefixSmem {
@@ -55,8 +58,20 @@ static_assert(256 * (64 * 4 + 16) <= 2 * PrefixSmem<64>::kTile + kPtStages * Pre
 // ---- tcgen05 ------------------------------------------------------------------------------------------------
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_commit(uint64_t *bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
+// Products and commits are issued by one lane (`leader`) of a warp whose lanes all run the code around them: operands
+// have to be in uniform registers, and in a branch of one lane every instruction would first move them there (more
+// registers, and spills).
+__device__ __forceinline__ uint32_t elect_leader() {
+  uint32_t leader;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(leader));
+  return leader;
+}
+__device__ __forceinline__ void tc_commit(uint64_t *bar, uint32_t leader) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.u32 q, %1, 0;\n\t@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(
+          smem_addr(bar)),
+      "r"(leader)
+      : "memory");
 }
 // Shared-memory operand, 128-byte swizzle: start, distance of 64-value blocks (only where the operand is read across
 // its rows), distance of 8-row groups (1024 bytes).
@@ -69,15 +84,17 @@ __device__ __forceinline__ constexpr uint32_t tc_instruction(int n, bool b_acros
   const uint32_t type = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
   return (1u << 4) | (type << 7) | (type << 10) | ((b_across ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((128u >> 4) << 24);
 }
-__device__ __forceinline__ void tc_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t instr, bool add) {
-  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a),
-               "l"(b), "r"(instr), "r"((uint32_t)add)
-               : "memory");
+__device__ __forceinline__ void tc_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t instr, bool add, uint32_t leader) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %4, 0;\n\tsetp.ne.u32 q, %5, 0;\n\t@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(instr), "r"((uint32_t)add), "r"(leader)
+      : "memory");
 }
-__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t instr, bool add) {
-  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a),
-               "l"(b), "r"(instr), "r"((uint32_t)add)
-               : "memory");
+__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t instr, bool add, uint32_t leader) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %4, 0;\n\tsetp.ne.u32 q, %5, 0;\n\t@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(instr), "r"((uint32_t)add), "r"(leader)
+      : "memory");
 }
 // 32 columns of this warp's 32 lanes
 __device__ __forceinline__ void tc_load32(uint32_t addr, uint32_t (&r)[32]) {
@@ -105,6 +122,14 @@ __device__ __forceinline__ void tc_store16(uint32_t addr, const uint32_t (&r)[16
       "r"(addr));
 }
 __device__ __forceinline__ void tc_wait_load() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// The same for one tc_load32, whose registers nothing may read earlier; other memory is free to move across.
+__device__ __forceinline__ void tc_wait_load(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]),
+                 "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]),
+                 "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]),
+                 "+r"(r[31]));
+}
 __device__ __forceinline__ void tc_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool ok) {
@@ -186,11 +211,13 @@ __device__ __forceinline__ float tile_weights(uint32_t s_at, const float *sk, co
   const uint64_t minus = pair_of(-safe, -safe), factor = pair_of(scale, scale), units = pair_of(unit, unit);
   uint64_t total[2] = {0, 0};
   float top[2] = {-INFINITY, -INFINITY};
+  uint32_t buf[2][32];                           // the next 32 columns are on their way while these are worked on
+  tc_load32(s_at, buf[0]);
 #pragma unroll
   for (int c = 0; c < 4; ++c) {
-    uint32_t s[32];
-    tc_load32(s_at + c * 32, s);
-    tc_wait_load();
+    uint32_t (&s)[32] = buf[c & 1];
+    tc_wait_load(s);
+    if (c < 3) tc_load32(s_at + (c + 1) * 32, buf[(c + 1) & 1]);
 #pragma unroll
     for (int e = 0; e < 32; e += 4) {
       float4 f, g;
@@ -234,7 +261,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) prefix_tensor_kernel(const __gr
   const AttnArgs &a = args.a;
   constexpr bool kWide = kFmt != kFmtRaw;
   constexpr bool kUnits = kWide && std::is_same<T, __half>::value;  // see shared_prefix_attention_kernel
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;  // uniform for the compiler
 
   const int split = blockIdx.x % args.splits;
   const int item = blockIdx.x / args.splits;
@@ -268,7 +295,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) prefix_tensor_kernel(const __gr
   }
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(&sm.tmem);
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *reinterpret_cast<volatile uint32_t *>(&sm.tmem), 0);
   auto wait = [&](uint64_t *bar, uint32_t parity) -> bool {
     if (mbar_wait_bounded(bar, parity)) return true;
     raise_status(HFK_DEV_WAIT_TIMEOUT);
@@ -276,7 +303,10 @@ __global__ void __launch_bounds__(kPtThreads, 1) prefix_tensor_kernel(const __gr
     return false;
   };
 
+  auto wait_warp = [&](uint64_t *bar, uint32_t parity) -> bool { return __all_sync(0xffffffffu, wait(bar, parity)); };
+
   if (warp >= 8 && warp < 12) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 120;");
     // ---------------------------------------------------------------- loads ---
     const int p = threadIdx.x - 256;
     // key p of a tile: where its row is
@@ -393,8 +423,12 @@ __global__ void __launch_bounds__(kPtThreads, 1) prefix_tensor_kernel(const __gr
 #pragma unroll
           for (int k = 0; k < 4; ++k) codes_to_pairs<T, kFmt>(w[k], x[2 * k], x[2 * k + 1]);
           const int row = r * kRowsPass + row_in;
-          *reinterpret_cast<uint4 *>(ring + tile_at(row, 2 * chunk)) = make_uint4(x[0], x[1], x[2], x[3]);
-          *reinterpret_cast<uint4 *>(ring + tile_at(row, 2 * chunk + 1)) = make_uint4(x[4], x[5], x[6], x[7]);
+          // head_dim 128: lanes of the first half of a row write their even chunk while the others write their odd one, so
+          // that the eight lanes of a row hit eight bank groups
+          const bool swap = D == 128 && chunk >= 4;
+          const uint4 even = make_uint4(x[0], x[1], x[2], x[3]), odd = make_uint4(x[4], x[5], x[6], x[7]);
+          *reinterpret_cast<uint4 *>(ring + tile_at(row, 2 * chunk + (swap ? 1 : 0))) = swap ? odd : even;
+          *reinterpret_cast<uint4 *>(ring + tile_at(row, 2 * chunk + (swap ? 0 : 1))) = swap ? even : odd;
         }
         fence_async_proxy();
         mbar_arrive(&sm.full[stage]);
@@ -421,53 +455,57 @@ __global__ void __launch_bounds__(kPtThreads, 1) prefix_tensor_kernel(const __gr
         if (i + 1 < n) fetch(i + 1, kV);
       }
     }
-  } else if (warp == 12) {
+  } else if (warp >= 12) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     // ------------------------------------------------------------- products ---
-    if (lane == 0 && n > 0) {
+    if (warp == 12 && n > 0) {
+      const uint32_t leader = elect_leader();
       constexpr uint32_t kScores = tc_instruction<T>(kPtKeys, false), kValues = tc_instruction<T>(D, true);
-      bool ok = wait(&sm.q_full, 0);
+      bool ok = wait_warp(&sm.q_full, 0);
       auto values = [&](int j, int i) {          // o_j += weights_j . V_i
-        const uint32_t v = smem_addr(sm.ring[(i & 1) * 2 + 1]);
+        const uint64_t v = tc_operand(smem_addr(sm.ring[(i & 1) * 2 + 1]), kPtKeys * 128);
         tc_fence_after();
 #pragma unroll
-        for (int k = 0; k < kPtKeys / 16; ++k)
-          tc_mma_ts(tmem + 256 + j * D, tmem + j * 128 + k * 8, tc_operand(v + k * 2048, kPtKeys * 128), kValues, i > 0 || k > 0);
+        for (int k = 0; k < kPtKeys / 16; ++k)   // 16 keys: 16 rows of 128 bytes
+          tc_mma_ts(tmem + 256 + j * D, tmem + j * 128 + k * 8, v + k * (2048 >> 4), kValues, i > 0 || k > 0, leader);
       };
       for (int i = 0; i < n && ok; ++i) {
         const int stage = (i & 1) * 2;
-        ok = wait(&sm.full[stage], (i >> 1) & 1);
-        if (ok && i > 0) ok = wait(&sm.full[((i - 1) & 1) * 2 + 1], ((i - 1) >> 1) & 1);
-        const uint32_t kk = smem_addr(sm.ring[stage]);
+        ok = wait_warp(&sm.full[stage], (i >> 1) & 1);
+        if (ok && i > 0) ok = wait_warp(&sm.full[((i - 1) & 1) * 2 + 1], ((i - 1) >> 1) & 1);
+        const uint64_t kk = tc_operand(smem_addr(sm.ring[stage]), 16);
         for (int j = 0; j < tiles && ok; ++j) {
           if (i > 0) {
-            ok = wait(&sm.p_full[j], (i - 1) & 1);
+            ok = wait_warp(&sm.p_full[j], (i - 1) & 1);
             if (!ok) break;
             values(j, i - 1);
           }
           tc_fence_after();
-          const uint32_t q = smem_addr(sm.q[j]);
+          const uint64_t q = tc_operand(smem_addr(sm.q[j]), 16);
 #pragma unroll
-          for (int k = 0; k < D / 16; ++k) {
-            const uint32_t at = (k >> 2) * (kPtKeys * 128) + (k & 3) * 32;
-            tc_mma_ss(tmem + j * 128, tc_operand(q + at, 16), tc_operand(kk + at, 16), kScores, k > 0);
+          for (int k = 0; k < D / 16; ++k) {     // 16 values of each row: 32 bytes on, or the other half
+            const uint32_t at = ((k >> 2) * (kPtKeys * 128) + (k & 3) * 32) >> 4;
+            tc_mma_ss(tmem + j * 128, q + at, kk + at, kScores, k > 0, leader);
           }
-          tc_commit(&sm.s_full[j]);
+          tc_commit(&sm.s_full[j], leader);
         }
         if (!ok) break;
-        tc_commit(&sm.empty[stage]);
-        if (i > 0) tc_commit(&sm.empty[((i - 1) & 1) * 2 + 1]);
+        tc_commit(&sm.empty[stage], leader);
+        if (i > 0) tc_commit(&sm.empty[((i - 1) & 1) * 2 + 1], leader);
       }
-      if (ok) ok = wait(&sm.full[((n - 1) & 1) * 2 + 1], ((n - 1) >> 1) & 1);
+      if (ok) ok = wait_warp(&sm.full[((n - 1) & 1) * 2 + 1], ((n - 1) >> 1) & 1);
       for (int j = 0; j < tiles && ok; ++j) {
-        ok = wait(&sm.p_full[j], (n - 1) & 1);
+        ok = wait_warp(&sm.p_full[j], (n - 1) & 1);
         if (ok) values(j, n - 1);
       }
-      tc_commit(&sm.o_full);                     // also after a failure: nothing is in flight when the CTA ends
-      wait(&sm.o_full, 0);
+      tc_commit(&sm.o_full, leader);                     // also after a failure: nothing is in flight when the CTA ends
+      wait_warp(&sm.o_full, 0);
     }
     __syncwarp();
-  } else if (warp / 4 < tiles) {
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
     // -------------------------------------------------------------- softmax ---
+    if (warp / 4 < tiles) {
     const int j = warp / 4;
     const uint32_t lanes = (uint32_t)(warp % 4) << 21;   // first TMEM lane of this warp, in bits 16 and up
     const uint32_t s_at = tmem + j * 128 + lanes, o_at = tmem + 256 + j * D + lanes;
@@ -571,6 +609,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) prefix_tensor_kernel(const __gr
         bulk_wait_all();
       }
     }
+  }
   }
   tc_fence_before();
   __syncthreads();
