@@ -260,7 +260,7 @@ static int plan_attention(const hfk_prefix_attention_desc *d, int ctas, AttnPlan
   }
   p->ctas = d->max_blocks_per_seq == 0 && p->tensor ? 0 : ctas > 0 ? std::min(ctas, 65535) : sms * kAttnCtasPerSm;
   const AttnLine line(seqs, d->kv_heads, d->group, p->tensor ? 0 : (int)d->prefix_len);
-  const size_t parts = p->ctas > 0 ? (size_t)p->ctas + (size_t)line.items(seqs) : 0;
+  const size_t parts = p->ctas > 0 ? (size_t)p->ctas * kLineWarps + (size_t)line.items(seqs) : 0;
   const auto round = [](size_t n) { return (n + 255) & ~(size_t)255; };
   p->cu_bytes = round((size_t)(seqs + 1) * sizeof(int64_t));
   p->ml_bytes = round(parts * 16 * sizeof(float2));
@@ -268,6 +268,23 @@ static int plan_attention(const hfk_prefix_attention_desc *d, int ctas, AttnPlan
   p->prefix_ml_bytes = round((size_t)p->splits * d->kv_heads * rows * sizeof(float2));
   p->prefix_o_bytes = round((size_t)p->splits * d->kv_heads * rows * d->head_dim * sizeof(float));
   return HFK_OK;
+}
+
+// A launch that may start while the kernel launched before it in the same stream still runs (`early`, where that
+// is one of ours and says so with launch_next).
+template <typename Args>
+static cudaError_t launch_behind(void (*kernel)(const Args), bool early, int ctas, int threads, size_t smem, cudaStream_t s, const Args &args) {
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(ctas);
+  config.blockDim = dim3(threads);
+  config.dynamicSmemBytes = smem;
+  config.stream = s;
+  cudaLaunchAttribute attr = {};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = &attr;
+  config.numAttrs = early ? 1 : 0;
+  return cudaLaunchKernelEx(&config, kernel, args);
 }
 
 template <typename T, int kFmt, int D>
@@ -301,13 +318,13 @@ static cudaError_t launch_attention(const AttnArgs &a, const AttnPlan &p, unsign
     join.prefix_o = t.part_o;
   }
   if (p.ctas > 0) {
-    const size_t smem = 4 * 16 * (D * sizeof(float) + sizeof(float2)) + (size_t)(a.seqs + 1) * sizeof(int64_t);
-    shared_prefix_attention_kernel<T, kFmt, D><<<p.ctas, 128, smem, s>>>(join.a);
-    if ((e = cudaGetLastError()) != cudaSuccess) return e;
+    const size_t smem = kLineWarps * sizeof(LineRing<kFmt, D>) + (size_t)(a.seqs + 1 + kLineWarps) * sizeof(int64_t);
+    auto k = shared_prefix_attention_kernel<T, kFmt, D>;
+    if ((e = allow_smem(k, smem)) != cudaSuccess) return e;
+    if ((e = launch_behind(k, p.tensor, p.ctas, kLineWarps * 32, smem, s, join.a)) != cudaSuccess) return e;
   }
   const int rows = a.seqs * a.kv_heads * a.group;
-  shared_prefix_join_kernel<T, D><<<(rows + 3) / 4, 128, 0, s>>>(join);
-  return cudaGetLastError();
+  return launch_behind(shared_prefix_join_kernel<T, D>, true, (rows + 3) / 4, 128, 0, s, join);
 }
 template <typename T, int kFmt>
 static cudaError_t launch_attention(const AttnArgs &a, int head_dim, const AttnPlan &p, unsigned char *w, cudaStream_t s) {

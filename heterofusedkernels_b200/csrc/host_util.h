@@ -52,8 +52,8 @@ constexpr long long kStagedMaxCopyBytes = 64ll << 20;
 constexpr int kMigrateCtasPerSm = 2;
 // Reading an 8-bit cache back: 256-thread CTAs per SM, eight 8-byte loads a lane in flight.
 constexpr int kGatherDequantCtasPerSm = 4;
-// Attention: 128-thread CTAs per SM (about 200 registers a thread).
-constexpr int kAttnCtasPerSm = 2;
+// Attention: CTAs of eight warps per SM (their rings take its shared memory).
+constexpr int kAttnCtasPerSm = 1;
 // Rows of queries (sequences x query heads of a K/V head) above which the prefix goes to the tensor-core kernel, and
 // what a CTA of it costs beyond its key tiles, in tiles.
 constexpr int kPrefixTensorMinRows = 32;

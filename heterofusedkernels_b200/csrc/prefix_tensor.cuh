@@ -132,13 +132,6 @@ __device__ __forceinline__ void tc_wait_load(uint32_t (&r)[32]) {
 }
 __device__ __forceinline__ void tc_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool ok) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int kLeft>
-__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory"); }
-
 // Byte of 16-byte chunk `chunk` of row `row` in a tile (8 chunks to a 128-byte row, halves behind each other).
 __device__ __forceinline__ uint32_t tile_at(int row, int chunk) {
   return (uint32_t)((chunk >> 3) * (kPtKeys * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4));
@@ -263,6 +256,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) prefix_tensor_kernel(const __gr
   constexpr bool kUnits = kWide && std::is_same<T, __half>::value;  // see shared_prefix_attention_kernel
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;  // uniform for the compiler
 
+  launch_next();
   const int split = blockIdx.x % args.splits;
   const int item = blockIdx.x / args.splits;
   const int h = item / args.row_blocks;

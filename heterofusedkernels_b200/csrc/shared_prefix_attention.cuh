@@ -100,16 +100,17 @@ __device__ __forceinline__ void codes_to_pairs(uint32_t w, uint32_t &lo, uint32_
 
 // ---- how the work is laid out -------------------------------------------------------------------------------
 // An ITEM is 16 rows of queries against one range of keys: for the prefix a (K/V head, 16 of the seqs * group
-// rows), for a sequence's own keys a (sequence, K/V head, 16 of the group's rows).  Keys go by tiles of 64.
+// rows), for a sequence's own keys a (sequence, K/V head, 16 of the group's rows).  Keys go by tiles of 16.
 // All tiles of all items form one line, items of the prefix first, that is cut into equal pieces, one to a
-// CTA: no CTA has more than one tile more than another, whatever the lengths are (they are known on the
-// device only).  A piece may end one item and begin the next.  The part of CTA c of item i has the number
-// c + i: along the line either grows, so no two parts share a number and there are at most CTAs + items.
-constexpr int kTileKeys = 64;
+// WARP: none has more than one tile more than another, whatever the lengths are (they are known on the
+// device only).  A piece may end one item and begin the next.  The part of warp w of item i has the number
+// w + i: along the line either grows, so no two parts share a number and there are at most warps + items.
+constexpr int kTileKeys = 16;
+constexpr int kLineWarps = 8;   // of a CTA
 
 struct AttnLine {
   int row_tiles, own_tiles;       // tiles of 16 rows: of the prefix's rows, of a group
-  int prefix_items, prefix_tiles; // tiles of 64 keys of an item
+  int prefix_items, prefix_tiles; // tiles of 16 keys of an item
   int per_seq;                    // items of a sequence
   __host__ __device__ AttnLine(int seqs, int kv_heads, int group, int prefix_len) {
     row_tiles = (seqs * group + 15) / 16;
@@ -121,8 +122,12 @@ struct AttnLine {
   __host__ __device__ int64_t items(int seqs) const { return prefix_items + (int64_t)seqs * per_seq; }
 };
 
-// CTAs that take part: with fewer tiles than CTAs one tile each, so that none of them is without a part.
-__device__ __forceinline__ int64_t line_ctas(int64_t grid, int64_t total) { return min(grid, total); }
+// Warps that take part: each at least kLeastTiles tiles (a part costs a start-up and a place in the join), and with
+// fewer tiles than that one warp; so none of them is without a tile.
+constexpr int kLeastTiles = 2;
+__device__ __forceinline__ int64_t line_warps(int64_t warps, int64_t total) {
+  return max((int64_t)min((int64_t)1, total), min(warps, total / kLeastTiles));
+}
 
 // Clamped length of sequence s.
 __device__ __forceinline__ int64_t own_length(const AttnArgs &a, int s, bool report) {
@@ -134,106 +139,212 @@ __device__ __forceinline__ int64_t own_length(const AttnArgs &a, int s, bool rep
   return len;
 }
 
-// First tiles of the sequences (per item of the sequence), by warp 0.
-__device__ __forceinline__ void scan_tiles(const AttnArgs &a, int64_t *cu) {
-  if (threadIdx.x >= 32) return;
-  const int lane = threadIdx.x;
-  int64_t carry = 0;
-  for (int base = 0; base < a.seqs; base += 32) {
-    const int s = base + lane;
-    const int64_t n = s < a.seqs ? (own_length(a, s, blockIdx.x == 0) + kTileKeys - 1) / kTileKeys : 0;
-    int64_t inc = n;
+// First tiles of the sequences (per item of a sequence) in shared memory, cu[seqs] the sum; all threads of the CTA,
+// each a run of sequences, so that the lengths are one round of loads.
+__device__ __forceinline__ void scan_tiles(const AttnArgs &a, int64_t *cu, int64_t *warp_sums) {
+  constexpr int kThreads = kLineWarps * 32;
+  constexpr int kMost = HFK_MAX_SEQS / kThreads;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int per = (a.seqs + kThreads - 1) / kThreads;
+  const int s0 = threadIdx.x * per;
+  int64_t n[kMost], sum = 0;
 #pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const int64_t v = __shfl_up_sync(0xffffffffu, inc, d);
-      if (lane >= d) inc += v;
-    }
-    if (s < a.seqs) cu[s] = carry + inc - n;
-    carry += __shfl_sync(0xffffffffu, inc, 31);
+  for (int k = 0; k < kMost; ++k) {
+    n[k] = k < per && s0 + k < a.seqs ? (own_length(a, s0 + k, blockIdx.x == 0) + kTileKeys - 1) / kTileKeys : 0;
+    sum += n[k];
   }
-  if (lane == 0) cu[a.seqs] = carry;
+  int64_t inc = sum;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int64_t v = __shfl_up_sync(0xffffffffu, inc, d);
+    if (lane >= d) inc += v;
+  }
+  if (lane == 31) warp_sums[warp] = inc;
+  __syncthreads();
+  int64_t before = inc - sum;
+  for (int w = 0; w < warp; ++w) before += warp_sums[w];
+#pragma unroll
+  for (int k = 0; k < kMost; ++k) {
+    if (k < per && s0 + k < a.seqs) cu[s0 + k] = before;
+    before += n[k];
+  }
+  if (threadIdx.x == kThreads - 1) cu[a.seqs] = before;
+  __syncthreads();
 }
 
+// The item at a place of the line.
+struct LineItem {
+  int64_t ordinal;
+  int h, row0, rows, seq;   // its rows of queries: row0 .. row0 + rows of the prefix's rows, or of the sequence's group
+  int len;                  // keys
+  int tile, tiles;          // the place's tile of the item's tiles
+  const void *table;        // its page ids start at table[table_at]
+  int64_t table_at;
+};
+__device__ __forceinline__ LineItem line_item(const AttnArgs &a, const AttnLine &line, const int64_t *cu, int64_t at) {
+  const int64_t in_prefix = (int64_t)line.prefix_items * line.prefix_tiles;
+  LineItem x;
+  if (at < in_prefix) {
+    x.ordinal = at / line.prefix_tiles;
+    x.tile = (int)(at - x.ordinal * line.prefix_tiles);
+    x.tiles = line.prefix_tiles;
+    x.h = (int)x.ordinal / line.row_tiles;
+    x.row0 = ((int)x.ordinal - x.h * line.row_tiles) * 16;
+    x.rows = min(16, a.seqs * a.group - x.row0);
+    x.seq = 0;
+    x.len = a.prefix_len;
+    x.table = a.prefix_table;
+    x.table_at = 0;
+  } else {
+    const int64_t u = at - in_prefix;
+    int lo = 0, hi = a.seqs;
+    while (lo < hi) {         // number of sequences that end at or before u
+      const int mid = (lo + hi) >> 1;
+      if (cu[mid + 1] * line.per_seq <= u) lo = mid + 1; else hi = mid;
+    }
+    x.seq = lo;
+    const int64_t v = u - cu[lo] * line.per_seq;
+    x.tiles = (int)(cu[lo + 1] - cu[lo]);
+    const int hg = (int)(v / x.tiles);
+    x.tile = (int)(v - (int64_t)hg * x.tiles);
+    x.ordinal = line.prefix_items + (int64_t)lo * line.per_seq + hg;
+    x.h = hg / line.own_tiles;
+    x.row0 = (hg - x.h * line.own_tiles) * 16;
+    x.rows = min(16, a.group - x.row0);
+    x.len = (int)own_length(a, lo, false);
+    x.table = a.tables;
+    x.table_at = (int64_t)lo * a.table_stride;
+  }
+  return x;
+}
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool ok) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void *src, bool ok) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(ok ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kLeft>
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory"); }
+// A kernel launched behind another one of the same call may start while that one runs; its results are there
+// after launch_wait.
+__device__ __forceinline__ void launch_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void launch_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+// Ring of a warp: kStages tiles of 16 keys, K rows, V rows, and for an 8-bit cache their scales.
+template <int kFmt, int D>
+struct alignas(128) LineRing {
+  static constexpr int kRow = D * (kFmt == kFmtRaw ? 2 : 1);
+  static constexpr int kStages = kRow >= 256 ? 3 : kRow >= 128 ? 5 : 8;
+  unsigned char k[kStages][16 * kRow], v[kStages][16 * kRow];
+  float scales[kStages][32];      // of 16 keys, of 16 values
+  uint32_t valid[kStages + (kStages & 1)];
+};
+
 // ---- the kernel ------------------------------------------------------------------------------------------------
-// Four warps; each takes 16 of a tile's 64 keys and keeps (m, l, o) of its own over the whole piece, so the
-// warps meet only at the end of a piece.  K and V go from global memory straight into the registers of the
-// matrix product: the order of the products over head_dim, and of the columns of o, is free, so a lane takes
-// 16 contiguous bytes of a row where the operand layout would have it take two.
+// Every warp works for itself: it keeps (m, l, o) of its piece, and brings its keys and values into a ring of its own
+// with asynchronous copies that run ahead over the ends of items; nothing in the CTA waits for anything else.
+// In the ring the 16-byte chunks of a row are XORed with bits of the row's number, so that the fragments' reads
+// (K: four neighbouring chunks of two rows; V: two neighbouring chunks of four rows, two apart) hit all banks.
+// The order of the products over head_dim, and of the columns of o, is free, so a lane takes 16 contiguous bytes of
+// a row where the operand layout would have it take two, and V needs no transposition: a lane that holds the same
+// columns of four rows packs its operands with byte permutations.
+//
+// Bound by HBM for long sequences.  Eight warps of one CTA an SM hold 2 x 8 KB each in flight (16-bit, head_dim 128).
 template <typename T, int kFmt, int D>
-__global__ void __launch_bounds__(128) shared_prefix_attention_kernel(const __grid_constant__ AttnArgs a) {
+__global__ void __launch_bounds__(kLineWarps * 32, 1) shared_prefix_attention_kernel(const __grid_constant__ AttnArgs a) {
+  using Ring = LineRing<kFmt, D>;
   constexpr int kElt = kFmt == kFmtRaw ? 2 : 1;
-  constexpr int kRow = D * kElt;
+  constexpr int kRow = Ring::kRow, kStages = Ring::kStages;
   constexpr int kKc = kRow / 64;                          // 16-byte chunks of a K row per lane
   constexpr int kVb = kRow / 8 < 16 ? kRow / 8 : 16;      // bytes of a V chunk
   constexpr int kVc = kRow / 8 / kVb;                     // V chunks of a row per lane
   constexpr int kVe = kVb / kElt;                         // values of a V chunk
   constexpr int kE = 16 / kElt;                           // values of a K chunk
+  constexpr int kCpr = kRow / 16, kRowsPass = 32 / kCpr;  // copies: chunks of a row, rows of a warp's pass
+  constexpr bool kUnits = kFmt != kFmtRaw && std::is_same<T, __half>::value;
   extern __shared__ __align__(128) unsigned char smem_raw[];
-  float *sm_o = reinterpret_cast<float *>(smem_raw);                      // [4][16][D]
-  float2 *sm_ml = reinterpret_cast<float2 *>(sm_o + 4 * 16 * D);          // [4][16]
-  int64_t *cu = reinterpret_cast<int64_t *>(sm_ml + 4 * 16);              // [seqs + 1]
-
-  scan_tiles(a, cu);
-  __syncthreads();
-  const AttnLine line(a.seqs, a.kv_heads, a.group, a.prefix_len);
-  const int64_t in_prefix = (int64_t)line.prefix_items * line.prefix_tiles;
-  const int64_t total = in_prefix + cu[a.seqs] * line.per_seq;
-  if (blockIdx.x == 0)
-    for (int s = threadIdx.x; s <= a.seqs; s += blockDim.x) a.cu[s] = cu[s];
-  const int64_t ctas = line_ctas(gridDim.x, total);
-  const int64_t begin = blockIdx.x < ctas ? total * blockIdx.x / ctas : total;
-  const int64_t end = blockIdx.x < ctas ? total * (blockIdx.x + 1) / ctas : total;
-
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  for (int64_t at = begin; at < end;) {
-    // the item at this place of the line, and the tiles of it that are ours
-    int64_t ordinal, item_begin, item_tiles;
-    int h, row0, rows, seq;     // rows of queries: row0 .. row0 + rows of the item's row space
-    int64_t len;
-    const void *table;
-    int64_t table_at;
-    if (at < in_prefix) {
-      ordinal = at / line.prefix_tiles;
-      item_begin = ordinal * line.prefix_tiles;
-      item_tiles = line.prefix_tiles;
-      h = (int)(ordinal / line.row_tiles);
-      row0 = (int)(ordinal - (int64_t)h * line.row_tiles) * 16;
-      rows = min(16, a.seqs * a.group - row0);
-      seq = 0;
-      len = a.prefix_len;
-      table = a.prefix_table;
-      table_at = 0;
-    } else {
-      const int64_t u = at - in_prefix;
-      int lo = 0, hi = a.seqs;
-      while (lo < hi) {         // number of sequences that end at or before u
-        const int mid = (lo + hi) >> 1;
-        if (cu[mid + 1] * line.per_seq <= u) lo = mid + 1; else hi = mid;
+  Ring &ring = reinterpret_cast<Ring *>(smem_raw)[warp];
+  int64_t *cu = reinterpret_cast<int64_t *>(smem_raw + kLineWarps * sizeof(Ring));   // [seqs + 1]
+  int64_t *warp_sums = cu + a.seqs + 1;
+
+  launch_next();
+  scan_tiles(a, cu, warp_sums);
+  if (blockIdx.x == 0)
+    for (int s = threadIdx.x; s <= a.seqs; s += kLineWarps * 32) a.cu[s] = cu[s];
+  const AttnLine line(a.seqs, a.kv_heads, a.group, a.prefix_len);
+  const int64_t total = (int64_t)line.prefix_items * line.prefix_tiles + cu[a.seqs] * line.per_seq;
+  const int64_t warps = line_warps((int64_t)gridDim.x * kLineWarps, total);
+  // neighbouring pieces go to different SMs: a batch of few tiles is spread over all of them
+  const int64_t me = (int64_t)warp * gridDim.x + blockIdx.x;
+  const int64_t begin = me < warps ? total * me / warps : total, end = me < warps ? total * (me + 1) / warps : total;
+
+  // ---- loads: tile `load_at` of the line is the next to be brought in; its page ids are here already
+  LineItem in = {};
+  int64_t load_at = begin;
+  int64_t id = -1;            // of key (lane & 15) of the tile
+  auto fetch_id = [&]() {
+    const int key = in.tile * kTileKeys + (lane & 15);
+    id = key < in.len ? load_id(in.table, a.ids_are_int64, in.table_at + a.block.div((uint32_t)key)) : -1;
+  };
+  if (begin < end) {
+    in = line_item(a, line, cu, begin);
+    fetch_id();
+  }
+  int load_stage = 0;
+  auto load_tile = [&]() {
+    if (load_at < end) {
+      const int key = in.tile * kTileKeys + (lane & 15);
+      const bool inside = key < in.len;
+      const bool ok = inside && id >= 0 && id < a.num_blocks;
+      if (inside && !ok) raise_status(HFK_DEV_BAD_DEVICE_BLOCK_ID);
+      const uint32_t row = ((uint32_t)key - a.block.div((uint32_t)key) * a.block.d) * a.kv_heads + in.h;
+      const int64_t page = ok ? id * a.block_stride : 0;
+      const int64_t off = ok ? page + (int64_t)row * kRow : -1;
+      if (kFmt != kFmtRaw)    // lanes 0-15 the scales of the keys, 16-31 those of the values
+        cp_async4(smem_addr(&ring.scales[load_stage][lane]),
+                  (lane < 16 ? a.k_cache : a.v_cache) + page + a.scales_at + (ok ? (int64_t)row * 4 : 0), ok);
+      const uint32_t mask = __ballot_sync(0xffffffffu, ok) & 0xffffu;
+      if (lane == 0) ring.valid[load_stage] = mask;
+      const uint32_t kb = smem_addr(ring.k[load_stage]), vb = smem_addr(ring.v[load_stage]);
+      const int chunk = lane % kCpr;
+#pragma unroll
+      for (int r = 0; r < 16; r += kRowsPass) {
+        const int at = r + lane / kCpr;
+        const int64_t o = __shfl_sync(0xffffffffu, off, at);
+        const int64_t from = (o < 0 ? 0 : o) + chunk * 16;
+        const int kc = kCpr >= 8 ? chunk ^ ((at & 1) << 2) : chunk;
+        const int vc = kCpr >= 8 ? chunk ^ (((at >> 1) & 3) << 1) : chunk ^ ((at >> 1) & 3);
+        cp_async16(kb + at * kRow + kc * 16, a.k_cache + from, o >= 0);
+        cp_async16(vb + at * kRow + vc * 16, a.v_cache + from, o >= 0);
       }
-      seq = lo;
-      item_tiles = cu[seq + 1] - cu[seq];
-      const int64_t v = u - cu[seq] * line.per_seq;
-      const int hg = (int)(v / item_tiles);
-      item_begin = in_prefix + cu[seq] * line.per_seq + hg * item_tiles;
-      ordinal = line.prefix_items + (int64_t)seq * line.per_seq + hg;
-      h = hg / line.own_tiles;
-      row0 = (hg - h * line.own_tiles) * 16;
-      rows = min(16, a.group - row0);
-      len = own_length(a, seq, false);
-      table = a.tables;
-      table_at = (int64_t)seq * a.table_stride;
+      ++load_at;
+      if (load_at < end) {
+        if (++in.tile == in.tiles) in = line_item(a, line, cu, load_at);
+        fetch_id();
+      }
+      load_stage = load_stage + 1 == kStages ? 0 : load_stage + 1;
     }
-    const int64_t stop = min(end, item_begin + item_tiles);
-    const int64_t tile_a = at - item_begin, tile_b = stop - item_begin;
+    cp_async_commit();        // one group a tile, empty behind the last one
+  };
+#pragma unroll
+  for (int i = 0; i < kStages - 1; ++i) load_tile();
+
+  int stage = 0;
+  for (int64_t at = begin; at < end;) {
+    const LineItem x = line_item(a, line, cu, at);
+    const int64_t stop = min(end, at + (x.tiles - x.tile));
 
     // queries: rows g and g + 8, the chunks this lane also takes of K
     uint32_t qf[D / 16][4];
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
-      const int r = row0 + g + 8 * half;
-      const bool ok = g + 8 * half < rows;
-      const int s = seq + (ok ? r / a.group : 0);
-      const unsigned char *qp = a.q + s * a.q_seq + (int64_t)(h * a.group + (ok ? r % a.group : 0)) * a.q_head;
+      const int r = x.row0 + g + 8 * half;
+      const bool ok = g + 8 * half < x.rows;
+      const int s = x.seq + (ok ? r / a.group : 0);
+      const unsigned char *qp = a.q + s * a.q_seq + (int64_t)(x.h * a.group + (ok ? r % a.group : 0)) * a.q_head;
 #pragma unroll
       for (int c = 0; c < kKc; ++c)
 #pragma unroll
@@ -253,61 +364,24 @@ __global__ void __launch_bounds__(128) shared_prefix_attention_kernel(const __gr
 #pragma unroll
     for (int j = 0; j < D / 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
 
-    for (int64_t tile = tile_a; tile < tile_b; ++tile) {
-      const int64_t key0 = tile * kTileKeys + warp * 16;
-      if (key0 >= len) continue;
-      // where the lane's rows are: K of keys g and g + 8, V of keys 2t, 2t + 1, 2t + 8, 2t + 9
-      auto locate = [&](int i, int64_t &page, uint32_t &row) -> bool {
-        const int64_t key = key0 + i;
-        if (key >= len) return false;
-        const uint32_t b = a.block.div((uint32_t)key);
-        const int64_t id = load_id(table, a.ids_are_int64, table_at + b);
-        if (id < 0 || id >= a.num_blocks) {
-          raise_status(HFK_DEV_BAD_DEVICE_BLOCK_ID);
-          return false;
-        }
-        page = id * a.block_stride;
-        row = ((uint32_t)key - b * a.block.d) * a.kv_heads + h;
-        return true;
-      };
-      uint4 kr[2][kKc], vr[4][kVc];
-      float sk[4], sv[4];
-      bool live[4];
+    for (; at < stop; ++at) {
+      cp_async_wait<kStages - 2>();
+      __syncwarp();           // every lane's copies of this tile have arrived, and the stage before it has been read
+      load_tile();
+      const unsigned char *ks = ring.k[stage], *vs = ring.v[stage];
+      const uint32_t valid = ring.valid[stage];
+      const bool live[4] = {(valid >> (2 * t) & 1) != 0, (valid >> (2 * t + 1) & 1) != 0, (valid >> (2 * t + 8) & 1) != 0,
+                            (valid >> (2 * t + 9) & 1) != 0};
+      float sk[4] = {0.f, 0.f, 0.f, 0.f}, sv[4] = {0.f, 0.f, 0.f, 0.f};
+      if (kFmt != kFmtRaw) {
+        const float *sc = ring.scales[stage];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        int64_t page = 0;
-        uint32_t row = 0;
-        const bool ok = locate(g + 8 * i, page, row);
-        const unsigned char *p = a.k_cache + page + (int64_t)row * kRow;
-#pragma unroll
-        for (int c = 0; c < kKc; ++c) {
-          kr[i][c] = make_uint4(0, 0, 0, 0);
-          if (ok) kr[i][c] = *reinterpret_cast<const uint4 *>(p + (c * 4 + t) * 16);
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        int64_t page = 0;
-        uint32_t row = 0;
-        live[i] = locate(2 * t + (i & 1) + 8 * (i >> 1), page, row);
-        const unsigned char *p = a.v_cache + page + (int64_t)row * kRow;
-        sk[i] = sv[i] = 0.f;
-        if (kFmt != kFmtRaw && live[i]) {
-          sk[i] = reinterpret_cast<const float *>(a.k_cache + page + a.scales_at)[row];
-          sv[i] = reinterpret_cast<const float *>(a.v_cache + page + a.scales_at)[row];
-        }
-#pragma unroll
-        for (int c = 0; c < kVc; ++c) {
-          vr[i][c] = make_uint4(0, 0, 0, 0);
-          if (live[i]) {
-            if constexpr (kVb == 16) {
-              vr[i][c] = *reinterpret_cast<const uint4 *>(p + (c * 8 + g) * 16);
-            } else {
-              const uint2 w = *reinterpret_cast<const uint2 *>(p + (c * 8 + g) * 8);
-              vr[i][c].x = w.x;
-              vr[i][c].y = w.y;
-            }
-          }
+        for (int i = 0; i < 2; ++i) {
+          const float2 f = *reinterpret_cast<const float2 *>(sc + 8 * i + 2 * t), h2 = *reinterpret_cast<const float2 *>(sc + 16 + 8 * i + 2 * t);
+          sk[2 * i] = f.x;
+          sk[2 * i + 1] = f.y;
+          sv[2 * i] = h2.x;
+          sv[2 * i + 1] = h2.y;
         }
       }
 
@@ -316,9 +390,12 @@ __global__ void __launch_bounds__(128) shared_prefix_attention_kernel(const __gr
 #pragma unroll
       for (int n = 0; n < 2; ++n) {
         s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+        const int kr = g + 8 * n;
 #pragma unroll
         for (int c = 0; c < kKc; ++c) {
-          const uint32_t w[4] = {kr[n][c].x, kr[n][c].y, kr[n][c].z, kr[n][c].w};
+          const int chunk = kCpr >= 8 ? (c * 4 + t) ^ ((kr & 1) << 2) : c * 4 + t;
+          const uint4 kw = *reinterpret_cast<const uint4 *>(ks + kr * kRow + chunk * 16);
+          const uint32_t w[4] = {kw.x, kw.y, kw.z, kw.w};
           if constexpr (kFmt == kFmtRaw) {
             mma16816<T>(s[n], qf[2 * c], w[0], w[1]);
             mma16816<T>(s[n], qf[2 * c + 1], w[2], w[3]);
@@ -352,7 +429,7 @@ __global__ void __launch_bounds__(128) shared_prefix_attention_kernel(const __gr
       // fp16 weights of an 8-bit cache: weight * scale may leave fp16's range, so o is kept in units of the
       // largest scale of a value so far
       float grow = 1.f, unit = 1.f;
-      if (kFmt != kFmtRaw && std::is_same<T, __half>::value) {
+      if (kUnits) {
         float big = max_nan(max_nan(sv[0], sv[1]), max_nan(sv[2], sv[3]));
         big = max_nan(big, __shfl_xor_sync(0xffffffffu, big, 1));
         big = max_nan(big, __shfl_xor_sync(0xffffffffu, big, 2));
@@ -394,21 +471,33 @@ __global__ void __launch_bounds__(128) shared_prefix_attention_kernel(const __gr
       // o column q (0..7) of block j = c * kVe + e holds value (c * 8 + q) * kVe + e of the head
 #pragma unroll
       for (int c = 0; c < kVc; ++c) {
-        const uint32_t w0[4] = {vr[0][c].x, vr[0][c].y, vr[0][c].z, vr[0][c].w};
-        const uint32_t w1[4] = {vr[1][c].x, vr[1][c].y, vr[1][c].z, vr[1][c].w};
-        const uint32_t w2[4] = {vr[2][c].x, vr[2][c].y, vr[2][c].z, vr[2][c].w};
-        const uint32_t w3[4] = {vr[3][c].x, vr[3][c].y, vr[3][c].z, vr[3][c].w};
+        uint32_t w[4][4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int vr = 2 * t + (i & 1) + 8 * (i >> 1);
+          if constexpr (kVb == 16) {
+            const uint4 x4 = *reinterpret_cast<const uint4 *>(vs + vr * kRow + (((c * 8 + g) ^ (((vr >> 1) & 3) << 1)) * 16));
+            w[i][0] = x4.x;
+            w[i][1] = x4.y;
+            w[i][2] = x4.z;
+            w[i][3] = x4.w;
+          } else {
+            const uint2 x2 = *reinterpret_cast<const uint2 *>(vs + vr * kRow + (((g >> 1) ^ ((vr >> 1) & 3)) * 16) + (g & 1) * 8);
+            w[i][0] = x2.x;
+            w[i][1] = x2.y;
+          }
+        }
 #pragma unroll
         for (int i = 0; i < kVb / 4; ++i) {
           if constexpr (kFmt == kFmtRaw) {
-            mma16816<T>(o[c * kVe + 2 * i], pf, __byte_perm(w0[i], w1[i], 0x5410), __byte_perm(w2[i], w3[i], 0x5410));
-            mma16816<T>(o[c * kVe + 2 * i + 1], pf, __byte_perm(w0[i], w1[i], 0x7632), __byte_perm(w2[i], w3[i], 0x7632));
+            mma16816<T>(o[c * kVe + 2 * i], pf, __byte_perm(w[0][i], w[1][i], 0x5410), __byte_perm(w[2][i], w[3][i], 0x5410));
+            mma16816<T>(o[c * kVe + 2 * i + 1], pf, __byte_perm(w[0][i], w[1][i], 0x7632), __byte_perm(w[2][i], w[3][i], 0x7632));
           } else {
             uint32_t x0, x1, x2, x3, y0, y1, y2, y3;
-            codes_to_pairs<T, kFmt>(__byte_perm(w0[i], w1[i], 0x5140), x0, x1);
-            codes_to_pairs<T, kFmt>(__byte_perm(w0[i], w1[i], 0x7362), x2, x3);
-            codes_to_pairs<T, kFmt>(__byte_perm(w2[i], w3[i], 0x5140), y0, y1);
-            codes_to_pairs<T, kFmt>(__byte_perm(w2[i], w3[i], 0x7362), y2, y3);
+            codes_to_pairs<T, kFmt>(__byte_perm(w[0][i], w[1][i], 0x5140), x0, x1);
+            codes_to_pairs<T, kFmt>(__byte_perm(w[0][i], w[1][i], 0x7362), x2, x3);
+            codes_to_pairs<T, kFmt>(__byte_perm(w[2][i], w[3][i], 0x5140), y0, y1);
+            codes_to_pairs<T, kFmt>(__byte_perm(w[2][i], w[3][i], 0x7362), y2, y3);
             mma16816<T>(o[c * kVe + 4 * i], pf, x0, y0);
             mma16816<T>(o[c * kVe + 4 * i + 1], pf, x1, y1);
             mma16816<T>(o[c * kVe + 4 * i + 2], pf, x2, y2);
@@ -416,49 +505,35 @@ __global__ void __launch_bounds__(128) shared_prefix_attention_kernel(const __gr
           }
         }
       }
+      stage = stage + 1 == kStages ? 0 : stage + 1;
     }
 
-    // join the four warps
+    // this warp's part of the item: lane (g, t) has columns 2t and 2t + 1 of every block, which is, for a chunk c, kVe
+    // values in a row of the head each
+    const int64_t part = me + x.ordinal;
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
       l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-      if (t == 0) sm_ml[warp * 16 + g + 8 * r] = make_float2(m[r], l[r]);
-    }
-    __syncthreads();
-    float big[2], factor[2];
+      const int row = g + 8 * r;
+      if (row < x.rows) {
+        if (t == 0) a.part_ml[part * 16 + row] = make_float2(m[r], l[r]);
+        const float unit = kUnits ? ref : 1.f;
+        float *dst = a.part_o + (part * 16 + row) * D;
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      big[r] = -INFINITY;
-      for (int w = 0; w < 4; ++w) big[r] = fmaxf(big[r], sm_ml[w * 16 + g + 8 * r].x);
-      factor[r] = big[r] == -INFINITY ? 0.f : ex2(m[r] - big[r]);
-      if (kFmt != kFmtRaw && std::is_same<T, __half>::value) factor[r] *= ref;
-    }
+        for (int c = 0; c < kVc; ++c)
 #pragma unroll
-    for (int j = 0; j < D / 8; ++j) {
-      const int c = j / kVe, e = j % kVe;
+          for (int y = 0; y < 2; ++y)
 #pragma unroll
-      for (int r = 0; r < 2; ++r)
-#pragma unroll
-        for (int x = 0; x < 2; ++x)
-          sm_o[(warp * 16 + g + 8 * r) * D + (c * 8 + 2 * t + x) * kVe + e] = o[j][2 * r + x] * factor[r];
-    }
-    __syncthreads();
-    const int64_t part = blockIdx.x + ordinal;
-    for (int i = threadIdx.x; i < rows * D; i += 128)
-      a.part_o[part * 16 * D + i] = (sm_o[i] + sm_o[16 * D + i]) + (sm_o[32 * D + i] + sm_o[48 * D + i]);
-    if (threadIdx.x < rows) {
-      float mm = -INFINITY, ll = 0.f;
-      for (int w = 0; w < 4; ++w) mm = fmaxf(mm, sm_ml[w * 16 + threadIdx.x].x);
-      for (int w = 0; w < 4; ++w) {
-        const float2 x = sm_ml[w * 16 + threadIdx.x];
-        ll += mm == -INFINITY ? x.y : x.y * ex2(x.x - mm);
+            for (int e = 0; e < kVe; e += 4)
+              *reinterpret_cast<float4 *>(dst + (c * 8 + 2 * t + y) * kVe + e) =
+                  make_float4(o[c * kVe + e][2 * r + y] * unit, o[c * kVe + e + 1][2 * r + y] * unit, o[c * kVe + e + 2][2 * r + y] * unit,
+                              o[c * kVe + e + 3][2 * r + y] * unit);
       }
-      a.part_ml[part * 16 + threadIdx.x] = make_float2(mm, ll);
     }
-    __syncthreads();
-    at = stop;
   }
+  cp_async_wait<0>();
+  launch_wait();              // the join is launched behind this kernel and also reads what was launched before it
 }
 
 // Joins the parts of every row; one warp a row.  Up to three lists of parts: of the prefix's item and of the
@@ -475,6 +550,7 @@ template <typename T, int D>
 __global__ void __launch_bounds__(128) shared_prefix_join_kernel(const __grid_constant__ JoinArgs args) {
   const AttnArgs &a = args.a;
   const int row = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  launch_wait();
   const int q_heads = a.kv_heads * a.group;
   if (row >= a.seqs * q_heads) return;
   const int s = row / q_heads, head = row - s * q_heads, h = head / a.group, g = head - h * a.group;
@@ -486,7 +562,7 @@ __global__ void __launch_bounds__(128) shared_prefix_join_kernel(const __grid_co
     const AttnLine line(a.seqs, a.kv_heads, a.group, a.prefix_len);
     const int64_t in_prefix = (int64_t)line.prefix_items * line.prefix_tiles;
     const int64_t total = in_prefix + a.cu[a.seqs] * line.per_seq;
-    const int64_t ctas = line_ctas(args.grid, total);
+    const int64_t warps = line_warps((int64_t)args.grid * kLineWarps, total);
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       int64_t item, from, tiles;
@@ -505,8 +581,8 @@ __global__ void __launch_bounds__(128) shared_prefix_join_kernel(const __grid_co
         item = line.prefix_items + (int64_t)s * line.per_seq + hg;
       }
       if (tiles > 0) {
-        // CTA c has [total c / ctas, total (c+1) / ctas): the one with tile x is floor((ctas (x+1) - 1) / total)
-        const int64_t first = (ctas * (from + 1) - 1) / total, last = (ctas * (from + tiles) - 1) / total;
+        // warp w has [total w / warps, total (w+1) / warps): the one with tile x is floor((warps (x+1) - 1) / total)
+        const int64_t first = (warps * (from + 1) - 1) / total, last = (warps * (from + tiles) - 1) / total;
         count[k] = last - first + 1;
         ml[k] = a.part_ml + (first + item) * 16 + place;
         o_at[k] = a.part_o + ((first + item) * 16 + place) * D;
