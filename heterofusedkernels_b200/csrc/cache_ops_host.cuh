@@ -219,11 +219,12 @@ static int gather_dequant_impl(const hfk_paged_gather_desc *d, int kv_format, in
 }
 
 // ---- attention -----------------------------------------------------------------------------------------------------
-// Batches above HFK_MAX_SEQS go out as several groups of launches, which use the workspace in turn.
+// Large batches (above HFK_MAX_SEQS sequences) go out as several groups of launches, which use the workspace in turn.
 struct AttnPlan {
   bool tensor;      // the prefix goes to prefix_tensor_kernel
   int splits;       // its runs of key tiles
-  int ctas;         // of the line
+  int ctas, warps;  // of the line
+  int seqs;         // sequences a group of launches takes
   size_t cu_bytes, ml_bytes, o_bytes, prefix_ml_bytes, prefix_o_bytes;
   size_t bytes() const { return cu_bytes + ml_bytes + o_bytes + prefix_ml_bytes + prefix_o_bytes; }
 };
@@ -240,7 +241,13 @@ static int plan_attention(const hfk_prefix_attention_desc *d, int ctas, AttnPlan
     return fail(HFK_ERR_TOO_LARGE, "%s: more than 2^31 keys", op);
   if (d->num_seqs >= (int64_t)1 << 30) return fail(HFK_ERR_TOO_LARGE, "%s: too many sequences", op);
   const int sms = sm_count();
-  const int seqs = (int)std::min<int64_t>(d->num_seqs, HFK_MAX_SEQS);
+  // at most HFK_MAX_SEQS at a time, and so few that the line's tiles are counted in 32 bits
+  int seqs = (int)std::min<int64_t>(d->num_seqs, HFK_MAX_SEQS);
+  const int64_t cap = d->max_blocks_per_seq * d->block_size;
+  while (seqs > 1 && AttnLine(seqs, d->kv_heads, d->group, (int)d->prefix_len).most_tiles(seqs, cap) > INT32_MAX / 2) seqs = (seqs + 1) / 2;
+  if (AttnLine(seqs, d->kv_heads, d->group, (int)d->prefix_len).most_tiles(seqs, cap) > INT32_MAX / 2)
+    return fail(HFK_ERR_TOO_LARGE, "%s: K/V heads times keys of one sequence exceed 2^34", op);
+  p->seqs = seqs;
   const int64_t rows = (int64_t)seqs * d->group;
   p->tensor = d->prefix_len > 0 && rows > kPrefixTensorMinRows;
   p->splits = 0;
@@ -260,9 +267,12 @@ static int plan_attention(const hfk_prefix_attention_desc *d, int ctas, AttnPlan
   }
   p->ctas = d->max_blocks_per_seq == 0 && p->tensor ? 0 : ctas > 0 ? std::min(ctas, 65535) : sms * kAttnCtasPerSm;
   const AttnLine line(seqs, d->kv_heads, d->group, p->tensor ? 0 : (int)d->prefix_len);
-  const size_t parts = p->ctas > 0 ? (size_t)p->ctas * kLineWarps + (size_t)line.items(seqs) : 0;
+  p->warps = p->ctas * (d->kv_format == HFK_KV_RAW ? LineWarps<kFmtRaw>::kCount : LineWarps<kFmtE4m3>::kCount);
+  // the size does not depend on the format: one workspace serves caches of either
+  const size_t most_warps = (size_t)p->ctas * std::max(LineWarps<kFmtRaw>::kCount, LineWarps<kFmtE4m3>::kCount);
+  const size_t parts = p->ctas > 0 ? most_warps + (size_t)line.items(seqs) : 0;
   const auto round = [](size_t n) { return (n + 255) & ~(size_t)255; };
-  p->cu_bytes = round((size_t)(seqs + 1) * sizeof(int64_t));
+  p->cu_bytes = round((size_t)(seqs + 1) * sizeof(int));
   p->ml_bytes = round(parts * 16 * sizeof(float2));
   p->o_bytes = round(parts * 16 * d->head_dim * sizeof(float));
   p->prefix_ml_bytes = round((size_t)p->splits * d->kv_heads * rows * sizeof(float2));
@@ -291,9 +301,9 @@ template <typename T, int kFmt, int D>
 static cudaError_t launch_attention(const AttnArgs &a, const AttnPlan &p, unsigned char *w, cudaStream_t s) {
   JoinArgs join = {};
   join.a = a;
-  join.grid = p.ctas;
+  join.warps = p.warps;
   join.rows = a.seqs * a.group;
-  join.a.cu = reinterpret_cast<int64_t *>(w);
+  join.a.cu = reinterpret_cast<int *>(w);
   join.a.part_ml = reinterpret_cast<float2 *>(w + p.cu_bytes);
   join.a.part_o = reinterpret_cast<float *>(w + p.cu_bytes + p.ml_bytes);
   cudaError_t e;
@@ -318,13 +328,13 @@ static cudaError_t launch_attention(const AttnArgs &a, const AttnPlan &p, unsign
     join.prefix_o = t.part_o;
   }
   if (p.ctas > 0) {
-    const size_t smem = kLineWarps * sizeof(LineRing<kFmt, D>) + (size_t)(a.seqs + 1 + kLineWarps) * sizeof(int64_t);
+    constexpr int kLineWarps = LineWarps<kFmt>::kCount;
+    const size_t smem = kLineWarps * sizeof(LineRing<kFmt, D>) + (size_t)(a.seqs + 1 + kLineWarps) * sizeof(int);
     auto k = shared_prefix_attention_kernel<T, kFmt, D>;
     if ((e = allow_smem(k, smem)) != cudaSuccess) return e;
     if ((e = launch_behind(k, p.tensor, p.ctas, kLineWarps * 32, smem, s, join.a)) != cudaSuccess) return e;
   }
-  const int rows = a.seqs * a.kv_heads * a.group;
-  return launch_behind(shared_prefix_join_kernel<T, D>, true, (rows + 3) / 4, 128, 0, s, join);
+  return launch_behind(shared_prefix_join_kernel<T, D>, true, a.seqs * a.kv_heads * a.group, kJoinWarps * 32, 0, s, join);
 }
 template <typename T, int kFmt>
 static cudaError_t launch_attention(const AttnArgs &a, int head_dim, const AttnPlan &p, unsigned char *w, cudaStream_t s) {
@@ -375,11 +385,12 @@ static int attention_impl(const hfk_prefix_attention_desc *d, int ctas, cudaStre
   a.kv_heads = d->kv_heads;
   a.group = d->group;
   a.block = FastDiv::make((uint32_t)d->block_size);
+  a.per_group = FastDiv::make((uint32_t)d->group);
   a.scale_log2 = d->scale * kLog2e;
   unsigned char *w = static_cast<unsigned char *>(d->workspace);
   const int64_t id = d->ids_are_int64 ? 8 : 4;
-  for (int64_t first = 0; first < d->num_seqs; first += HFK_MAX_SEQS) {
-    a.seqs = (int)std::min<int64_t>(HFK_MAX_SEQS, d->num_seqs - first);
+  for (int64_t first = 0; first < d->num_seqs; first += p.seqs) {
+    a.seqs = (int)std::min<int64_t>(p.seqs, d->num_seqs - first);
     a.q = static_cast<const unsigned char *>(d->q.base) + first * a.q_seq;
     a.out = static_cast<unsigned char *>(const_cast<void *>(d->out.base)) + first * a.out_seq;
     a.lse = d->lse ? d->lse + first * a.kv_heads * a.group : nullptr;

@@ -329,9 +329,10 @@ __global__ void __launch_bounds__(kPtThreads, 1) prefix_tensor_kernel(const __gr
       }
       return k;
     };
-    auto write_meta = [&](int i, const Key &k) {
+    // The rows' places go out first, so that the copies can start; the scales and which keys count follow.
+    auto write_places = [&](int i, const Key &k) { sm.off[i % kPtMeta][p] = k.off; };
+    auto write_scales = [&](int i, const Key &k) {
       const int m = i % kPtMeta;
-      sm.off[m][p] = k.off;
       if (kWide) {
         sm.sk[m][p] = k.sk * a.scale_log2;
         sm.sv[m][p] = k.sv;
@@ -353,7 +354,8 @@ __global__ void __launch_bounds__(kPtThreads, 1) prefix_tensor_kernel(const __gr
         mbar_arrive(&sm.full[pending]);
       };
       for (int i = 0; i < n; ++i) {
-        write_meta(i, key);
+        write_places(i, key);
+        write_scales(i, key);
         key = key_of(i + 1, next);
         next = page_of(i + 2);
         producers();
@@ -430,21 +432,22 @@ __global__ void __launch_bounds__(kPtThreads, 1) prefix_tensor_kernel(const __gr
       };
       constexpr std::integral_constant<int, 0> kK{};
       constexpr std::integral_constant<int, 1> kV{};
-      auto announce_tile = [&](int i) {          // tile i's rows are known to all four warps
-        write_meta(i, key);
+      auto announce_tile = [&](int i, auto fetches) {
+        const Key now = key;
+        write_places(i, now);
+        producers();
+        fetches();
         key = key_of(i + 1, next);
         next = page_of(i + 2);
-        producers();
+        write_scales(i, now);
       };
-      announce_tile(0);
-      fetch(0, kK);
-      fetch(0, kV);
+      announce_tile(0, [&]() {
+        fetch(0, kK);
+        fetch(0, kV);
+      });
       for (int i = 0; i < n; ++i) {
         if (!widen(i, kK)) break;
-        if (i + 1 < n) {
-          announce_tile(i + 1);
-          fetch(i + 1, kK);
-        }
+        if (i + 1 < n) announce_tile(i + 1, [&]() { fetch(i + 1, kK); });
         if (!widen(i, kV)) break;
         if (i + 1 < n) fetch(i + 1, kV);
       }
@@ -505,20 +508,26 @@ __global__ void __launch_bounds__(kPtThreads, 1) prefix_tensor_kernel(const __gr
     const uint32_t s_at = tmem + j * 128 + lanes, o_at = tmem + 256 + j * D + lanes;
     float m = -INFINITY, l = 0.f, ref = 0.f;
     bool ok = true;
-    {                                            // this thread's row of queries, zero behind the last one
-      const int at = threadIdx.x - j * kPtRows, row = j * kPtRows + at;
+    {                                            // this warp's 32 rows of queries, zero behind the last one
+      constexpr int kChunks = D / 8, kRowsPass = 32 / kChunks;
       const uint32_t flip = args.negate ? 0x80008000u : 0u;
-      const int r = row0 + row, sq = r / a.group;
-      const unsigned char *src = a.q + sq * a.q_seq + (int64_t)(h * a.group + r - sq * a.group) * a.q_head;
-      uint4 w[D / 8];
+      const int chunk = lane % kChunks;
 #pragma unroll
-      for (int c = 0; c < D / 8; ++c) {
-        w[c] = make_uint4(0, 0, 0, 0);
-        if (row < rows) w[c] = *reinterpret_cast<const uint4 *>(src + c * 16);
+      for (int half = 0; half < 2; ++half) {
+        uint4 w[16 / kRowsPass];
+#pragma unroll
+        for (int k = 0; k < 16 / kRowsPass; ++k) {
+          const int row = warp * 32 + half * 16 + k * kRowsPass + lane / kChunks, r = row0 + row;
+          const int sq = (int)a.per_group.div((uint32_t)r);
+          w[k] = make_uint4(0, 0, 0, 0);
+          if (row < rows) w[k] = *reinterpret_cast<const uint4 *>(a.q + sq * a.q_seq + (int64_t)(h * a.group + r - sq * a.group) * a.q_head + chunk * 16);
+        }
+#pragma unroll
+        for (int k = 0; k < 16 / kRowsPass; ++k) {
+          const int at = (warp % 4) * 32 + half * 16 + k * kRowsPass + lane / kChunks;
+          *reinterpret_cast<uint4 *>(&sm.q[j][tile_at(at, chunk)]) = make_uint4(w[k].x ^ flip, w[k].y ^ flip, w[k].z ^ flip, w[k].w ^ flip);
+        }
       }
-#pragma unroll
-      for (int c = 0; c < D / 8; ++c)
-        *reinterpret_cast<uint4 *>(&sm.q[j][tile_at(at, c)]) = make_uint4(w[c].x ^ flip, w[c].y ^ flip, w[c].z ^ flip, w[c].w ^ flip);
       fence_async_proxy();
       mbar_arrive(&sm.q_full);
       __syncwarp();

@@ -37,10 +37,10 @@ struct AttnArgs {
   int prefix_len;
   int64_t own_cap;                // max_blocks * block_size: longest length the tables can name
   int seqs, kv_heads, group;
-  FastDiv block;
+  FastDiv block, per_group;       // block size; group
   float scale_log2;               // scale * log2 e
   // partial results (workspace)
-  int64_t *cu;                    // [seqs + 1] first tile of each sequence, per (K/V head, row tile)
+  int *cu;                        // [seqs + 1] first tile of each sequence, per (K/V head, row tile)
   float2 *part_ml;                // [parts][16]  (m, l)
   float *part_o;                  // [parts][16][head_dim]
 };
@@ -106,7 +106,6 @@ __device__ __forceinline__ void codes_to_pairs(uint32_t w, uint32_t &lo, uint32_
 // device only).  A piece may end one item and begin the next.  The part of warp w of item i has the number
 // w + i: along the line either grows, so no two parts share a number and there are at most warps + items.
 constexpr int kTileKeys = 16;
-constexpr int kLineWarps = 8;   // of a CTA
 
 struct AttnLine {
   int row_tiles, own_tiles;       // tiles of 16 rows: of the prefix's rows, of a group
@@ -120,14 +119,19 @@ struct AttnLine {
     per_seq = kv_heads * own_tiles;
   }
   __host__ __device__ int64_t items(int seqs) const { return prefix_items + (int64_t)seqs * per_seq; }
+  // Most tiles the line can have; the host takes so few sequences at a time that they number less than 2^31.
+  __host__ __device__ int64_t most_tiles(int seqs, int64_t own_cap) const {
+    return (int64_t)prefix_items * prefix_tiles + (int64_t)seqs * per_seq * ((own_cap + kTileKeys - 1) / kTileKeys);
+  }
 };
 
 // Warps that take part: each at least kLeastTiles tiles (a part costs a start-up and a place in the join), and with
 // fewer tiles than that one warp; so none of them is without a tile.
 constexpr int kLeastTiles = 2;
-__device__ __forceinline__ int64_t line_warps(int64_t warps, int64_t total) {
-  return max((int64_t)min((int64_t)1, total), min(warps, total / kLeastTiles));
-}
+__device__ __forceinline__ int line_warps(int warps, int total) { return max(min(1, total), min(warps, total / kLeastTiles)); }
+// The first tile of warp w, and the warp that has tile x: w has [total w / warps, total (w + 1) / warps).
+__device__ __forceinline__ int first_tile(int w, int warps, int total) { return (int)((int64_t)total * w / warps); }
+__device__ __forceinline__ int warp_of_tile(int x, int warps, int total) { return (int)(((int64_t)warps * (x + 1) - 1) / total); }
 
 // Clamped length of sequence s.
 __device__ __forceinline__ int64_t own_length(const AttnArgs &a, int s, bool report) {
@@ -141,27 +145,27 @@ __device__ __forceinline__ int64_t own_length(const AttnArgs &a, int s, bool rep
 
 // First tiles of the sequences (per item of a sequence) in shared memory, cu[seqs] the sum; all threads of the CTA,
 // each a run of sequences, so that the lengths are one round of loads.
-__device__ __forceinline__ void scan_tiles(const AttnArgs &a, int64_t *cu, int64_t *warp_sums) {
-  constexpr int kThreads = kLineWarps * 32;
-  constexpr int kMost = HFK_MAX_SEQS / kThreads;
+template <int kThreads>
+__device__ __forceinline__ void scan_tiles(const AttnArgs &a, int *cu, int *warp_sums) {
+  constexpr int kMost = (HFK_MAX_SEQS + kThreads - 1) / kThreads;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int per = (a.seqs + kThreads - 1) / kThreads;
   const int s0 = threadIdx.x * per;
-  int64_t n[kMost], sum = 0;
+  int n[kMost], sum = 0;
 #pragma unroll
   for (int k = 0; k < kMost; ++k) {
-    n[k] = k < per && s0 + k < a.seqs ? (own_length(a, s0 + k, blockIdx.x == 0) + kTileKeys - 1) / kTileKeys : 0;
+    n[k] = k < per && s0 + k < a.seqs ? (int)((own_length(a, s0 + k, blockIdx.x == 0) + kTileKeys - 1) / kTileKeys) : 0;
     sum += n[k];
   }
-  int64_t inc = sum;
+  int inc = sum;
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
-    const int64_t v = __shfl_up_sync(0xffffffffu, inc, d);
+    const int v = __shfl_up_sync(0xffffffffu, inc, d);
     if (lane >= d) inc += v;
   }
   if (lane == 31) warp_sums[warp] = inc;
   __syncthreads();
-  int64_t before = inc - sum;
+  int before = inc - sum;
   for (int w = 0; w < warp; ++w) before += warp_sums[w];
 #pragma unroll
   for (int k = 0; k < kMost; ++k) {
@@ -174,40 +178,40 @@ __device__ __forceinline__ void scan_tiles(const AttnArgs &a, int64_t *cu, int64
 
 // The item at a place of the line.
 struct LineItem {
-  int64_t ordinal;
+  int ordinal;
   int h, row0, rows, seq;   // its rows of queries: row0 .. row0 + rows of the prefix's rows, or of the sequence's group
   int len;                  // keys
   int tile, tiles;          // the place's tile of the item's tiles
   const void *table;        // its page ids start at table[table_at]
   int64_t table_at;
 };
-__device__ __forceinline__ LineItem line_item(const AttnArgs &a, const AttnLine &line, const int64_t *cu, int64_t at) {
-  const int64_t in_prefix = (int64_t)line.prefix_items * line.prefix_tiles;
+__device__ __forceinline__ LineItem line_item(const AttnArgs &a, const AttnLine &line, const int *cu, int at) {
+  const int in_prefix = line.prefix_items * line.prefix_tiles;
   LineItem x;
   if (at < in_prefix) {
     x.ordinal = at / line.prefix_tiles;
-    x.tile = (int)(at - x.ordinal * line.prefix_tiles);
+    x.tile = at - x.ordinal * line.prefix_tiles;
     x.tiles = line.prefix_tiles;
-    x.h = (int)x.ordinal / line.row_tiles;
-    x.row0 = ((int)x.ordinal - x.h * line.row_tiles) * 16;
+    x.h = x.ordinal / line.row_tiles;
+    x.row0 = (x.ordinal - x.h * line.row_tiles) * 16;
     x.rows = min(16, a.seqs * a.group - x.row0);
     x.seq = 0;
     x.len = a.prefix_len;
     x.table = a.prefix_table;
     x.table_at = 0;
   } else {
-    const int64_t u = at - in_prefix;
+    const int u = at - in_prefix;
     int lo = 0, hi = a.seqs;
     while (lo < hi) {         // number of sequences that end at or before u
       const int mid = (lo + hi) >> 1;
       if (cu[mid + 1] * line.per_seq <= u) lo = mid + 1; else hi = mid;
     }
     x.seq = lo;
-    const int64_t v = u - cu[lo] * line.per_seq;
-    x.tiles = (int)(cu[lo + 1] - cu[lo]);
-    const int hg = (int)(v / x.tiles);
-    x.tile = (int)(v - (int64_t)hg * x.tiles);
-    x.ordinal = line.prefix_items + (int64_t)lo * line.per_seq + hg;
+    const int v = u - cu[lo] * line.per_seq;
+    x.tiles = cu[lo + 1] - cu[lo];
+    const int hg = v / x.tiles;
+    x.tile = v - hg * x.tiles;
+    x.ordinal = line.prefix_items + lo * line.per_seq + hg;
     x.h = hg / line.own_tiles;
     x.row0 = (hg - x.h * line.own_tiles) * 16;
     x.rows = min(16, a.group - x.row0);
@@ -232,11 +236,18 @@ __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_gr
 __device__ __forceinline__ void launch_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void launch_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
+// Warps of a CTA.  A 16-bit cache of long sequences is bound by HBM with 8 (two tiles of 8 KB in flight each, 355 us for
+// 2.4 GB); an 8-bit cache has half the bytes and more arithmetic to a tile, and 12 hide its latencies better.
+template <int kFmt>
+struct LineWarps {
+  static constexpr int kCount = kFmt == kFmtRaw ? 8 : 12;
+};
+
 // Ring of a warp: kStages tiles of 16 keys, K rows, V rows, and for an 8-bit cache their scales.
 template <int kFmt, int D>
 struct alignas(128) LineRing {
   static constexpr int kRow = D * (kFmt == kFmtRaw ? 2 : 1);
-  static constexpr int kStages = kRow >= 256 ? 3 : kRow >= 128 ? 5 : 8;
+  static constexpr int kStages = kRow >= 256 ? 3 : kRow >= 128 ? 4 : 8;
   unsigned char k[kStages][16 * kRow], v[kStages][16 * kRow];
   float scales[kStages][32];      // of 16 keys, of 16 values
   uint32_t valid[kStages + (kStages & 1)];
@@ -251,9 +262,9 @@ struct alignas(128) LineRing {
 // a row where the operand layout would have it take two, and V needs no transposition: a lane that holds the same
 // columns of four rows packs its operands with byte permutations.
 //
-// Bound by HBM for long sequences.  Eight warps of one CTA an SM hold 2 x 8 KB each in flight (16-bit, head_dim 128).
+// Bound by HBM for long sequences; for short ones by the chain from a sequence's length over its page ids to its rows.
 template <typename T, int kFmt, int D>
-__global__ void __launch_bounds__(kLineWarps * 32, 1) shared_prefix_attention_kernel(const __grid_constant__ AttnArgs a) {
+__global__ void __launch_bounds__(LineWarps<kFmt>::kCount * 32, 1) shared_prefix_attention_kernel(const __grid_constant__ AttnArgs a) {
   using Ring = LineRing<kFmt, D>;
   constexpr int kElt = kFmt == kFmtRaw ? 2 : 1;
   constexpr int kRow = Ring::kRow, kStages = Ring::kStages;
@@ -264,87 +275,117 @@ __global__ void __launch_bounds__(kLineWarps * 32, 1) shared_prefix_attention_ke
   constexpr int kE = 16 / kElt;                           // values of a K chunk
   constexpr int kCpr = kRow / 16, kRowsPass = 32 / kCpr;  // copies: chunks of a row, rows of a warp's pass
   constexpr bool kUnits = kFmt != kFmtRaw && std::is_same<T, __half>::value;
+  constexpr int kLineWarps = LineWarps<kFmt>::kCount;
   extern __shared__ __align__(128) unsigned char smem_raw[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   Ring &ring = reinterpret_cast<Ring *>(smem_raw)[warp];
-  int64_t *cu = reinterpret_cast<int64_t *>(smem_raw + kLineWarps * sizeof(Ring));   // [seqs + 1]
-  int64_t *warp_sums = cu + a.seqs + 1;
+  int *cu = reinterpret_cast<int *>(smem_raw + kLineWarps * sizeof(Ring));   // [seqs + 1]
+  int *warp_sums = cu + a.seqs + 1;
 
   launch_next();
-  scan_tiles(a, cu, warp_sums);
+  scan_tiles<kLineWarps * 32>(a, cu, warp_sums);
   if (blockIdx.x == 0)
     for (int s = threadIdx.x; s <= a.seqs; s += kLineWarps * 32) a.cu[s] = cu[s];
   const AttnLine line(a.seqs, a.kv_heads, a.group, a.prefix_len);
-  const int64_t total = (int64_t)line.prefix_items * line.prefix_tiles + cu[a.seqs] * line.per_seq;
-  const int64_t warps = line_warps((int64_t)gridDim.x * kLineWarps, total);
+  const int total = line.prefix_items * line.prefix_tiles + cu[a.seqs] * line.per_seq;
+  const int warps = line_warps((int)gridDim.x * kLineWarps, total);
   // neighbouring pieces go to different SMs: a batch of few tiles is spread over all of them
-  const int64_t me = (int64_t)warp * gridDim.x + blockIdx.x;
-  const int64_t begin = me < warps ? total * me / warps : total, end = me < warps ? total * (me + 1) / warps : total;
+  const int me = warp * (int)gridDim.x + (int)blockIdx.x;
+  const int begin = me < warps ? first_tile(me, warps, total) : total, end = me < warps ? first_tile(me + 1, warps, total) : total;
 
-  // ---- loads: tile `load_at` of the line is the next to be brought in; its page ids are here already
+  // ---- loads: tile `load_at` of the line is the next to be brought in
   LineItem in = {};
-  int64_t load_at = begin;
-  int64_t id = -1;            // of key (lane & 15) of the tile
-  auto fetch_id = [&]() {
-    const int key = in.tile * kTileKeys + (lane & 15);
+  int load_at = begin;
+  // Pages of a multiple of 16 tokens: a tile lies in one page, and lane j holds the id of the page of tile ids_from + j of
+  // the item.  Other pages: lane j holds the id of the page of key j & 15 of the tile.
+  const bool whole = a.block.d % kTileKeys == 0;
+  int64_t id = -1;
+  int ids_from = 0;
+  auto fetch_ids = [&]() {
+    const int key = whole ? (in.tile + lane) * kTileKeys : in.tile * kTileKeys + (lane & 15);
     id = key < in.len ? load_id(in.table, a.ids_are_int64, in.table_at + a.block.div((uint32_t)key)) : -1;
+    ids_from = in.tile;
   };
-  if (begin < end) {
-    in = line_item(a, line, cu, begin);
-    fetch_id();
-  }
   int load_stage = 0;
+  const int chunk = lane % kCpr, sub = lane / kCpr;
   auto load_tile = [&]() {
     if (load_at < end) {
-      const int key = in.tile * kTileKeys + (lane & 15);
-      const bool inside = key < in.len;
-      const bool ok = inside && id >= 0 && id < a.num_blocks;
-      if (inside && !ok) raise_status(HFK_DEV_BAD_DEVICE_BLOCK_ID);
-      const uint32_t row = ((uint32_t)key - a.block.div((uint32_t)key) * a.block.d) * a.kv_heads + in.h;
-      const int64_t page = ok ? id * a.block_stride : 0;
-      const int64_t off = ok ? page + (int64_t)row * kRow : -1;
-      if (kFmt != kFmtRaw)    // lanes 0-15 the scales of the keys, 16-31 those of the values
-        cp_async4(smem_addr(&ring.scales[load_stage][lane]),
-                  (lane < 16 ? a.k_cache : a.v_cache) + page + a.scales_at + (ok ? (int64_t)row * 4 : 0), ok);
-      const uint32_t mask = __ballot_sync(0xffffffffu, ok) & 0xffffu;
-      if (lane == 0) ring.valid[load_stage] = mask;
+      const int key0 = in.tile * kTileKeys;
       const uint32_t kb = smem_addr(ring.k[load_stage]), vb = smem_addr(ring.v[load_stage]);
-      const int chunk = lane % kCpr;
+      const uint32_t sb = smem_addr(&ring.scales[load_stage][lane]);
+      uint32_t mask;
+      if (whole) {
+        const int64_t page_id = __shfl_sync(0xffffffffu, id, in.tile - ids_from);
+        const bool ok = page_id >= 0 && page_id < a.num_blocks;
+        if (!ok && lane == 0) raise_status(HFK_DEV_BAD_DEVICE_BLOCK_ID);
+        const int64_t page = ok ? page_id * a.block_stride : 0;
+        const int left = ok ? in.len - key0 : 0;            // rows behind the last key are zero
+        mask = left >= 16 ? 0xffffu : (1u << max(left, 0)) - 1u;
+        // row of the page of the tile's first key
+        const uint32_t b = a.block.div((uint32_t)key0);
+        const uint32_t row = ((uint32_t)key0 - b * a.block.d) * a.kv_heads + in.h;
+        const int64_t from = page + (int64_t)(row + sub * a.kv_heads) * kRow + chunk * 16;
+        const int step = kRowsPass * a.kv_heads * kRow;     // bytes from pass to pass, less than a page
+        const unsigned char *kp = a.k_cache + from, *vp = a.v_cache + from;
+        if (kFmt != kFmtRaw) {  // lanes 0-15 the scales of the keys, 16-31 those of the values
+          const bool mine = (lane & 15) < left;
+          cp_async4(sb, (lane < 16 ? a.k_cache : a.v_cache) + page + a.scales_at + (mine ? (int64_t)(row + (lane & 15) * a.kv_heads) * 4 : 0), mine);
+        }
 #pragma unroll
-      for (int r = 0; r < 16; r += kRowsPass) {
-        const int at = r + lane / kCpr;
-        const int64_t o = __shfl_sync(0xffffffffu, off, at);
-        const int64_t from = (o < 0 ? 0 : o) + chunk * 16;
-        const int kc = kCpr >= 8 ? chunk ^ ((at & 1) << 2) : chunk;
-        const int vc = kCpr >= 8 ? chunk ^ (((at >> 1) & 3) << 1) : chunk ^ ((at >> 1) & 3);
-        cp_async16(kb + at * kRow + kc * 16, a.k_cache + from, o >= 0);
-        cp_async16(vb + at * kRow + vc * 16, a.v_cache + from, o >= 0);
+        for (int r = 0; r < 16; r += kRowsPass) {
+          const int at = r + sub;
+          const bool mine = at < left;
+          const int kc = kCpr >= 8 ? chunk ^ ((at & 1) << 2) : chunk;
+          const int vc = kCpr >= 8 ? chunk ^ (((at >> 1) & 3) << 1) : chunk ^ ((at >> 1) & 3);
+          const int64_t on = (int64_t)(r / kRowsPass) * step;
+          cp_async16(kb + at * kRow + kc * 16, mine ? kp + on : a.k_cache, mine);
+          cp_async16(vb + at * kRow + vc * 16, mine ? vp + on : a.v_cache, mine);
+        }
+      } else {
+        const int key = key0 + (lane & 15);
+        const bool inside = key < in.len;
+        const bool ok = inside && id >= 0 && id < a.num_blocks;
+        if (inside && !ok) raise_status(HFK_DEV_BAD_DEVICE_BLOCK_ID);
+        const uint32_t row = ((uint32_t)key - a.block.div((uint32_t)key) * a.block.d) * a.kv_heads + in.h;
+        const int64_t page = ok ? id * a.block_stride : 0;
+        const int64_t off = ok ? page + (int64_t)row * kRow : -1;
+        if (kFmt != kFmtRaw)
+          cp_async4(sb, (lane < 16 ? a.k_cache : a.v_cache) + page + a.scales_at + (ok ? (int64_t)row * 4 : 0), ok);
+        mask = __ballot_sync(0xffffffffu, ok) & 0xffffu;
+#pragma unroll
+        for (int r = 0; r < 16; r += kRowsPass) {
+          const int at = r + sub;
+          const int64_t o = __shfl_sync(0xffffffffu, off, at);
+          const int64_t from = (o < 0 ? 0 : o) + chunk * 16;
+          const int kc = kCpr >= 8 ? chunk ^ ((at & 1) << 2) : chunk;
+          const int vc = kCpr >= 8 ? chunk ^ (((at >> 1) & 3) << 1) : chunk ^ ((at >> 1) & 3);
+          cp_async16(kb + at * kRow + kc * 16, a.k_cache + from, o >= 0);
+          cp_async16(vb + at * kRow + vc * 16, a.v_cache + from, o >= 0);
+        }
       }
+      if (lane == 0) ring.valid[load_stage] = mask;
       ++load_at;
       if (load_at < end) {
-        if (++in.tile == in.tiles) in = line_item(a, line, cu, load_at);
-        fetch_id();
+        if (++in.tile == in.tiles) {
+          in = line_item(a, line, cu, load_at);
+          fetch_ids();
+        } else if (!whole || in.tile - ids_from == 32) {
+          fetch_ids();
+        }
       }
       load_stage = load_stage + 1 == kStages ? 0 : load_stage + 1;
     }
     cp_async_commit();        // one group a tile, empty behind the last one
   };
-#pragma unroll
-  for (int i = 0; i < kStages - 1; ++i) load_tile();
-
-  int stage = 0;
-  for (int64_t at = begin; at < end;) {
-    const LineItem x = line_item(a, line, cu, at);
-    const int64_t stop = min(end, at + (x.tiles - x.tile));
-
-    // queries: rows g and g + 8, the chunks this lane also takes of K
-    uint32_t qf[D / 16][4];
+  // queries: rows g and g + 8, the chunks this lane also takes of K
+  uint32_t qf[D / 16][4];
+  auto load_queries = [&](const LineItem &x) {
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
       const int r = x.row0 + g + 8 * half;
       const bool ok = g + 8 * half < x.rows;
-      const int s = x.seq + (ok ? r / a.group : 0);
-      const unsigned char *qp = a.q + s * a.q_seq + (int64_t)(x.h * a.group + (ok ? r % a.group : 0)) * a.q_head;
+      const int s = x.seq + (ok ? (int)a.per_group.div((uint32_t)r) : 0);
+      const unsigned char *qp = a.q + s * a.q_seq + (int64_t)(x.h * a.group + (ok ? r - (s - x.seq) * a.group : 0)) * a.q_head;
 #pragma unroll
       for (int c = 0; c < kKc; ++c)
 #pragma unroll
@@ -358,6 +399,23 @@ __global__ void __launch_bounds__(kLineWarps * 32, 1) shared_prefix_attention_ke
           qf[ks + 1][half + 2] = w.w;
         }
     }
+  };
+  if (begin < end) {
+    in = line_item(a, line, cu, begin);
+    fetch_ids();
+    load_queries(in);         // under way while the first tiles are asked for
+  }
+  LineItem x = in;
+#pragma unroll
+  for (int i = 0; i < kStages - 1; ++i) load_tile();
+
+  int stage = 0;
+  for (int at = begin; at < end;) {
+    if (at != begin) {
+      x = line_item(a, line, cu, at);
+      load_queries(x);
+    }
+    const int stop = min(end, at + (x.tiles - x.tile));
 
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, ref = 0.f;
     float o[D / 8][4];
@@ -510,7 +568,7 @@ __global__ void __launch_bounds__(kLineWarps * 32, 1) shared_prefix_attention_ke
 
     // this warp's part of the item: lane (g, t) has columns 2t and 2t + 1 of every block, which is, for a chunk c, kVe
     // values in a row of the head each
-    const int64_t part = me + x.ordinal;
+    const int64_t part = (int64_t)me + x.ordinal;
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
@@ -536,93 +594,138 @@ __global__ void __launch_bounds__(kLineWarps * 32, 1) shared_prefix_attention_ke
   launch_wait();              // the join is launched behind this kernel and also reads what was launched before it
 }
 
-// Joins the parts of every row; one warp a row.  Up to three lists of parts: of the prefix's item and of the
-// sequence's item on the line, and of the prefix's runs from prefix_tensor_kernel.
+// Joins the parts of every row.  Up to three lists of parts: of the prefix's item and of the sequence's item on the
+// line, and of the prefix's runs from prefix_tensor_kernel.
 struct JoinArgs {
   AttnArgs a;               // as the line's kernel had it: prefix_len 0 where the prefix went to the tensor kernel
-  int grid;                 // CTAs of the line, 0: no line
+  int warps;                // warps of the line, 0: no line
   int splits, rows;         // of the tensor kernel; splits 0: not used
   const float2 *prefix_ml;
   const float *prefix_o;
 };
 
+// Four warps a row, each with every fourth part and up to eight loads of a part under way: the parts (some dozens of a
+// row) are in L2, and the time is that of the chain of their loads.
+constexpr int kJoinWarps = 4, kJoinAhead = 8;
 template <typename T, int D>
-__global__ void __launch_bounds__(128) shared_prefix_join_kernel(const __grid_constant__ JoinArgs args) {
+__global__ void __launch_bounds__(kJoinWarps * 32) shared_prefix_join_kernel(const __grid_constant__ JoinArgs args) {
+  __shared__ float sums[kJoinWarps][D + 1];
   const AttnArgs &a = args.a;
-  const int row = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  launch_wait();
+  const int row = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int q_heads = a.kv_heads * a.group;
-  if (row >= a.seqs * q_heads) return;
-  const int s = row / q_heads, head = row - s * q_heads, h = head / a.group, g = head - h * a.group;
-  // list k: parts at ml[k] + step_ml i, o[k] + step_o i, i < count[k]
-  int64_t count[3] = {0, 0, 0};
-  const float2 *ml[3] = {nullptr, nullptr, nullptr};
-  const float *o_at[3] = {nullptr, nullptr, nullptr};
-  if (args.grid > 0) {
+  const int s = row / q_heads, head = row - s * q_heads, h = (int)a.per_group.div((uint32_t)head), g = head - h * a.group;
+  launch_wait();
+  // list k: parts first[k] + step[k] i in rows of (m, l) and of o, i < count[k]
+  int count[3] = {0, 0, 0};
+  int64_t first[3] = {0, 0, 0};
+  if (args.warps > 0) {
     const AttnLine line(a.seqs, a.kv_heads, a.group, a.prefix_len);
-    const int64_t in_prefix = (int64_t)line.prefix_items * line.prefix_tiles;
-    const int64_t total = in_prefix + a.cu[a.seqs] * line.per_seq;
-    const int64_t warps = line_warps((int64_t)args.grid * kLineWarps, total);
+    const int in_prefix = line.prefix_items * line.prefix_tiles;
+    const int before = a.cu[s], behind = a.cu[s + 1];
+    const int total = in_prefix + a.cu[a.seqs] * line.per_seq;
+    const int warps = line_warps(args.warps, total);
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      int64_t item, from, tiles;
-      int place;
+      int item, from, tiles, place;
       if (k == 0) {
         const int r = s * a.group + g;
-        item = (int64_t)h * line.row_tiles + r / 16;
+        item = h * line.row_tiles + r / 16;
         place = r % 16;
         from = item * line.prefix_tiles;
         tiles = line.prefix_tiles;
       } else {
         const int hg = h * line.own_tiles + g / 16;
         place = g % 16;
-        tiles = a.cu[s + 1] - a.cu[s];
-        from = in_prefix + a.cu[s] * line.per_seq + hg * tiles;
-        item = line.prefix_items + (int64_t)s * line.per_seq + hg;
+        tiles = behind - before;
+        from = in_prefix + before * line.per_seq + hg * tiles;
+        item = line.prefix_items + s * line.per_seq + hg;
       }
       if (tiles > 0) {
-        // warp w has [total w / warps, total (w+1) / warps): the one with tile x is floor((warps (x+1) - 1) / total)
-        const int64_t first = (warps * (from + 1) - 1) / total, last = (warps * (from + tiles) - 1) / total;
-        count[k] = last - first + 1;
-        ml[k] = a.part_ml + (first + item) * 16 + place;
-        o_at[k] = a.part_o + ((first + item) * 16 + place) * D;
+        const int w0 = warp_of_tile(from, warps, total), w1 = warp_of_tile(from + tiles - 1, warps, total);
+        count[k] = w1 - w0 + 1;
+        first[k] = ((int64_t)w0 + item) * 16 + place;
       }
     }
   }
-  const int64_t step[3] = {16, 16, (int64_t)a.kv_heads * args.rows};
+  const int64_t stride = (int64_t)a.kv_heads * args.rows;
   if (args.splits > 0) {
-    const int64_t r = (int64_t)h * args.rows + s * a.group + g;
     count[2] = args.splits;
-    ml[2] = args.prefix_ml + r;
-    o_at[2] = args.prefix_o + r * D;
+    first[2] = (int64_t)h * args.rows + s * a.group + g;
   }
+  const int parts = count[0] + count[1] + count[2];
+  auto part_of = [&](int i, const float2 *&ml, const float *&o) {
+    const bool p0 = i < count[0], p1 = i < count[0] + count[1];
+    const int64_t at = p0 ? first[0] + (int64_t)i * 16 : p1 ? first[1] + (int64_t)(i - count[0]) * 16 : first[2] + (i - count[0] - count[1]) * stride;
+    ml = (p1 ? a.part_ml : args.prefix_ml) + at;
+    o = (p1 ? a.part_o : args.prefix_o) + at * D;
+  };
+  // the largest maximum: every warp looks at all
   float big = -INFINITY;
-#pragma unroll
-  for (int k = 0; k < 3; ++k)
-    for (int64_t i = lane; i < count[k]; i += 32) big = fmaxf(big, ml[k][i * step[k]].x);
+  for (int i = lane; i < parts; i += 32) {
+    const float2 *ml;
+    const float *o;
+    part_of(i, ml, o);
+    big = fmaxf(big, ml->x);
+  }
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, d));
   constexpr int kPer = D / 32;
-  float l = 0.f, o[kPer];
+  float l = 0.f, sum[kPer];
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) o[i] = 0.f;
+  for (int e = 0; e < kPer; ++e) sum[e] = 0.f;
+  for (int i0 = warp; i0 < parts; i0 += kJoinWarps * kJoinAhead) {
+    float2 ml[kJoinAhead];
+    float o[kJoinAhead][kPer];
 #pragma unroll
-  for (int k = 0; k < 3; ++k)
-#pragma unroll 4
-    for (int64_t i = 0; i < count[k]; ++i) {
-      const float2 x = ml[k][i * step[k]];
-      const float f = big == -INFINITY ? 1.f : ex2(x.x - big);
-      l += x.y * f;
-      const float *src = o_at[k] + i * step[k] * D + lane * kPer;
+    for (int u = 0; u < kJoinAhead; ++u) {
+      const int i = i0 + u * kJoinWarps;
+      ml[u] = make_float2(-INFINITY, 0.f);
 #pragma unroll
-      for (int e = 0; e < kPer; ++e) o[e] += src[e] * f;
+      for (int e = 0; e < kPer; ++e) o[u][e] = 0.f;
+      if (i < parts) {
+        const float2 *mp;
+        const float *op;
+        part_of(i, mp, op);
+        ml[u] = *mp;
+        if constexpr (kPer == 4) {
+          const float4 x = *reinterpret_cast<const float4 *>(op + lane * 4);
+          o[u][0] = x.x;
+          o[u][1] = x.y;
+          o[u][2] = x.z;
+          o[u][3] = x.w;
+        } else {
+          const float2 x = *reinterpret_cast<const float2 *>(op + lane * 2);
+          o[u][0] = x.x;
+          o[u][1] = x.y;
+        }
+      }
     }
-  const float inv = l == 0.f ? 0.f : 1.f / l;   // a NaN stays
-  unsigned char *dst = a.out + s * a.out_seq + (int64_t)head * a.out_head + lane * kPer * 2;
 #pragma unroll
-  for (int i = 0; i < kPer; i += 2)
-    *reinterpret_cast<uint32_t *>(dst + i * 2) = Pair<T>::pack(o[i] * inv, o[i + 1] * inv);
-  if (a.lse != nullptr && lane == 0) a.lse[(int64_t)s * q_heads + head] = l == 0.f ? -INFINITY : kLn2 * (big + log2f(l));
+    for (int u = 0; u < kJoinAhead; ++u) {
+      const float f = big == -INFINITY ? 1.f : ex2(ml[u].x - big);
+      l += ml[u].y * f;
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) sum[e] += o[u][e] * f;
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < kPer; ++e) sums[warp][lane * kPer + e] = sum[e];
+  if (lane == 0) sums[warp][D] = l;
+  __syncthreads();
+  const int v = threadIdx.x * 2;
+  if (v < D) {
+    float2 r = make_float2(0.f, 0.f);
+    l = 0.f;
+#pragma unroll
+    for (int w = 0; w < kJoinWarps; ++w) {
+      r.x += sums[w][v];
+      r.y += sums[w][v + 1];
+      l += sums[w][D];
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;   // a NaN stays
+    *reinterpret_cast<uint32_t *>(a.out + s * a.out_seq + (int64_t)head * a.out_head + v * 2) = Pair<T>::pack(r.x * inv, r.y * inv);
+    if (a.lse != nullptr && threadIdx.x == 0) a.lse[(int64_t)s * q_heads + head] = l == 0.f ? -INFINITY : kLn2 * (big + log2f(l));
+  }
 }
 
 }  // namespace hfk
