@@ -244,8 +244,10 @@ static int plan_attention(const hfk_prefix_attention_desc *d, int ctas, AttnPlan
   // at most HFK_MAX_SEQS at a time, and so few that the line's tiles are counted in 32 bits
   int seqs = (int)std::min<int64_t>(d->num_seqs, HFK_MAX_SEQS);
   const int64_t cap = d->max_blocks_per_seq * d->block_size;
-  while (seqs > 1 && AttnLine(seqs, d->kv_heads, d->group, (int)d->prefix_len).most_tiles(seqs, cap) > INT32_MAX / 2) seqs = (seqs + 1) / 2;
-  if (AttnLine(seqs, d->kv_heads, d->group, (int)d->prefix_len).most_tiles(seqs, cap) > INT32_MAX / 2)
+  // (the smaller tile of a 16-bit cache, so that the workspace does not depend on the format)
+  const int tile = tile_keys(HFK_KV_RAW);
+  while (seqs > 1 && AttnLine(seqs, d->kv_heads, d->group, (int)d->prefix_len, tile).most_tiles(seqs, cap) > INT32_MAX / 2) seqs = (seqs + 1) / 2;
+  if (AttnLine(seqs, d->kv_heads, d->group, (int)d->prefix_len, tile).most_tiles(seqs, cap) > INT32_MAX / 2)
     return fail(HFK_ERR_TOO_LARGE, "%s: K/V heads times keys of one sequence exceed 2^34", op);
   p->seqs = seqs;
   const int64_t rows = (int64_t)seqs * d->group;
@@ -266,11 +268,9 @@ static int plan_attention(const hfk_prefix_attention_desc *d, int ctas, AttnPlan
     }
   }
   p->ctas = d->max_blocks_per_seq == 0 && p->tensor ? 0 : ctas > 0 ? std::min(ctas, 65535) : sms * kAttnCtasPerSm;
-  const AttnLine line(seqs, d->kv_heads, d->group, p->tensor ? 0 : (int)d->prefix_len);
-  p->warps = p->ctas * (d->kv_format == HFK_KV_RAW ? LineWarps<kFmtRaw>::kCount : LineWarps<kFmtE4m3>::kCount);
-  // the size does not depend on the format: one workspace serves caches of either
-  const size_t most_warps = (size_t)p->ctas * std::max(LineWarps<kFmtRaw>::kCount, LineWarps<kFmtE4m3>::kCount);
-  const size_t parts = p->ctas > 0 ? most_warps + (size_t)line.items(seqs) : 0;
+  const AttnLine line(seqs, d->kv_heads, d->group, p->tensor ? 0 : (int)d->prefix_len, tile);
+  p->warps = p->ctas * kLineWarps;
+  const size_t parts = p->ctas > 0 ? (size_t)p->warps + (size_t)line.items(seqs) : 0;
   const auto round = [](size_t n) { return (n + 255) & ~(size_t)255; };
   p->cu_bytes = round((size_t)(seqs + 1) * sizeof(int));
   p->ml_bytes = round(parts * 16 * sizeof(float2));
@@ -328,7 +328,6 @@ static cudaError_t launch_attention(const AttnArgs &a, const AttnPlan &p, unsign
     join.prefix_o = t.part_o;
   }
   if (p.ctas > 0) {
-    constexpr int kLineWarps = LineWarps<kFmt>::kCount;
     const size_t smem = kLineWarps * sizeof(LineRing<kFmt, D>) + (size_t)(a.seqs + 1 + kLineWarps) * sizeof(int);
     auto k = shared_prefix_attention_kernel<T, kFmt, D>;
     if ((e = allow_smem(k, smem)) != cudaSuccess) return e;
@@ -386,6 +385,7 @@ static int attention_impl(const hfk_prefix_attention_desc *d, int ctas, cudaStre
   a.group = d->group;
   a.block = FastDiv::make((uint32_t)d->block_size);
   a.per_group = FastDiv::make((uint32_t)d->group);
+  a.tile = tile_keys(d->kv_format);
   a.scale_log2 = d->scale * kLog2e;
   unsigned char *w = static_cast<unsigned char *>(d->workspace);
   const int64_t id = d->ids_are_int64 ? 8 : 4;

@@ -51,6 +51,8 @@ struct PrefixSmem {
   uint64_t full[kPtStages], empty[kPtStages], meta[kPtMeta], s_full[2], p_full[2], o_full, q_full;
   uint32_t tmem;
   int failed;
+  uint32_t q_top;                                // bits of the largest finite |query|
+  float q_back;                                  // what undoes the queries' scaling
 };
 static_assert(256 * (128 * 4 + 16) <= 2 * PrefixSmem<128>::kTile + kPtStages * PrefixSmem<128>::kTile, "o fits");
 static_assert(256 * (64 * 4 + 16) <= 2 * PrefixSmem<64>::kTile + kPtStages * PrefixSmem<64>::kTile, "o fits");
@@ -79,9 +81,9 @@ __device__ __forceinline__ uint64_t tc_operand(uint32_t addr, uint32_t block_byt
   return (uint64_t)((addr >> 4) & 0x3fff) | ((uint64_t)(block_bytes >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
 }
 // fp32 accumulators, M = 128; b_across: B is read across its rows.
-template <typename T>
+template <typename M>
 __device__ __forceinline__ constexpr uint32_t tc_instruction(int n, bool b_across) {
-  const uint32_t type = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+  const uint32_t type = std::is_same<M, __nv_bfloat16>::value ? 1u : 0u;
   return (1u << 4) | (type << 7) | (type << 10) | ((b_across ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((128u >> 4) << 24);
 }
 __device__ __forceinline__ void tc_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t instr, bool add, uint32_t leader) {
@@ -180,7 +182,7 @@ __device__ __forceinline__ void rescale(uint32_t o_at, float factor) {
 }
 
 // Largest score of the tile (in units of log2 e), -inf without a key.
-template <typename T, int kFmt, bool kMask>
+template <int kFmt, bool kMask>
 __device__ __forceinline__ float tile_max(uint32_t s_at, const float *sk, float scale, const uint32_t (&valid)[4]) {
   float top = -INFINITY;
 #pragma unroll 1
@@ -197,7 +199,7 @@ __device__ __forceinline__ float tile_max(uint32_t s_at, const float *sk, float 
 
 // Weights 2^(score - m) of the tile's 128 keys, packed in pairs, times the values' scales; their sum before that;
 // returns the largest score - m.
-template <typename T, int kFmt, bool kUnits, bool kMask>
+template <typename M, int kFmt, bool kMask>
 __device__ __forceinline__ float tile_weights(uint32_t s_at, const float *sk, const float *sv, float scale, float m, float unit,
                                               const uint32_t (&valid)[4], uint32_t (&w)[64], float &sum) {
   const float safe = m == -INFINITY ? 0.f : m;
@@ -231,12 +233,11 @@ __device__ __forceinline__ float tile_weights(uint32_t s_at, const float *sk, co
         uint64_t p = pair_of(ex2(x.x), ex2(x.y));
         total[k] = add2(total[k], p);
         if (kFmt != kFmtRaw) {
-          uint64_t by_v = k == 0 ? pair_of(g.x, g.y) : pair_of(g.z, g.w);
-          if (kUnits) by_v = mul2(by_v, units);
-          p = mul2(p, by_v);
+          const uint64_t by_v = k == 0 ? pair_of(g.x, g.y) : pair_of(g.z, g.w);
+          p = mul2(p, mul2(by_v, units));
         }
         const float2 y = of_pair(p);
-        w[c * 16 + e / 2 + k] = Pair<T>::pack(y.x, y.y);
+        w[c * 16 + e / 2 + k] = Pair<M>::pack(y.x, y.y);
       }
     }
   }
@@ -253,7 +254,8 @@ __global__ void __launch_bounds__(kPtThreads, 1) prefix_tensor_kernel(const __gr
   Smem &sm = *reinterpret_cast<Smem *>(smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023));
   const AttnArgs &a = args.a;
   constexpr bool kWide = kFmt != kFmtRaw;
-  constexpr bool kUnits = kWide && std::is_same<T, __half>::value;  // see shared_prefix_attention_kernel
+  using M = Operand<T, kFmt>;
+  constexpr bool kScaleQ = kWide && !std::is_same<T, M>::value;  // bf16 queries become fp16
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;  // uniform for the compiler
 
   launch_next();
@@ -280,6 +282,8 @@ __global__ void __launch_bounds__(kPtThreads, 1) prefix_tensor_kernel(const __gr
     mbar_init(&sm.o_full, 1);
     mbar_init(&sm.q_full, tiles * 128);
     sm.failed = 0;
+    sm.q_top = 0;
+    sm.q_back = 1.f;
     mbar_fence_init();
   }
   if (warp == 12) {
@@ -329,12 +333,13 @@ __global__ void __launch_bounds__(kPtThreads, 1) prefix_tensor_kernel(const __gr
       }
       return k;
     };
+    float factor = a.scale_log2;                 // of the scores
     // The rows' places go out first, so that the copies can start; the scales and which keys count follow.
     auto write_places = [&](int i, const Key &k) { sm.off[i % kPtMeta][p] = k.off; };
     auto write_scales = [&](int i, const Key &k) {
       const int m = i % kPtMeta;
       if (kWide) {
-        sm.sk[m][p] = k.sk * a.scale_log2;
+        sm.sk[m][p] = k.sk * factor;
         sm.sv[m][p] = k.sv;
       }
       const uint32_t word = __ballot_sync(0xffffffffu, k.ok);
@@ -417,7 +422,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) prefix_tensor_kernel(const __gr
           const uint32_t w[4] = {codes[v][r].x, codes[v][r].y, codes[v][r].z, codes[v][r].w};
           uint32_t x[8];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) codes_to_pairs<T, kFmt>(w[k], x[2 * k], x[2 * k + 1]);
+          for (int k = 0; k < 4; ++k) codes_to_pairs<kFmt>(w[k], x[2 * k], x[2 * k + 1]);
           const int row = r * kRowsPass + row_in;
           // head_dim 128: lanes of the first half of a row write their even chunk while the others write their odd one, so
           // that the eight lanes of a row hit eight bank groups
@@ -439,6 +444,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) prefix_tensor_kernel(const __gr
         fetches();
         key = key_of(i + 1, next);
         next = page_of(i + 2);
+        if (kScaleQ && i == 0 && wait(&sm.q_full, 0)) factor *= *reinterpret_cast<volatile float *>(&sm.q_back);
         write_scales(i, now);
       };
       announce_tile(0, [&]() {
@@ -457,7 +463,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) prefix_tensor_kernel(const __gr
     // ------------------------------------------------------------- products ---
     if (warp == 12 && n > 0) {
       const uint32_t leader = elect_leader();
-      constexpr uint32_t kScores = tc_instruction<T>(kPtKeys, false), kValues = tc_instruction<T>(D, true);
+      constexpr uint32_t kScores = tc_instruction<M>(kPtKeys, false), kValues = tc_instruction<M>(D, true);
       bool ok = wait_warp(&sm.q_full, 0);
       auto values = [&](int j, int i) {          // o_j += weights_j . V_i
         const uint64_t v = tc_operand(smem_addr(sm.ring[(i & 1) * 2 + 1]), kPtKeys * 128);
@@ -512,21 +518,34 @@ __global__ void __launch_bounds__(kPtThreads, 1) prefix_tensor_kernel(const __gr
       constexpr int kChunks = D / 8, kRowsPass = 32 / kChunks;
       const uint32_t flip = args.negate ? 0x80008000u : 0u;
       const int chunk = lane % kChunks;
+      constexpr int kPasses = 32 / kRowsPass;
+      uint4 w[kPasses];
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        uint4 w[16 / kRowsPass];
+      for (int k = 0; k < kPasses; ++k) {
+        const int row = warp * 32 + k * kRowsPass + lane / kChunks, r = row0 + row;
+        const int sq = (int)a.per_group.div((uint32_t)r);
+        w[k] = make_uint4(0, 0, 0, 0);
+        if (row < rows) w[k] = *reinterpret_cast<const uint4 *>(a.q + sq * a.q_seq + (int64_t)(h * a.group + r - sq * a.group) * a.q_head + chunk * 16);
+      }
+      if constexpr (kScaleQ) {                   // one power of two for all rows of the CTA
+        float top = 0.f;
 #pragma unroll
-        for (int k = 0; k < 16 / kRowsPass; ++k) {
-          const int row = warp * 32 + half * 16 + k * kRowsPass + lane / kChunks, r = row0 + row;
-          const int sq = (int)a.per_group.div((uint32_t)r);
-          w[k] = make_uint4(0, 0, 0, 0);
-          if (row < rows) w[k] = *reinterpret_cast<const uint4 *>(a.q + sq * a.q_seq + (int64_t)(h * a.group + r - sq * a.group) * a.q_head + chunk * 16);
-        }
+        for (int k = 0; k < kPasses; ++k)
+          top = fmaxf(fmaxf(top, fmaxf(largest_of_pair(w[k].x), largest_of_pair(w[k].y))), fmaxf(largest_of_pair(w[k].z), largest_of_pair(w[k].w)));
+        const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
+        if (lane == 0) atomicMax(&sm.q_top, bits);
+        asm volatile("bar.sync 2, %0;" ::"r"(tiles * 128) : "memory");
+        const int e = shift_to_half(__uint_as_float(*reinterpret_cast<volatile uint32_t *>(&sm.q_top)));
+        const float f = power_of_two(e);
+        if (threadIdx.x == 0) sm.q_back = power_of_two(-e);
 #pragma unroll
-        for (int k = 0; k < 16 / kRowsPass; ++k) {
-          const int at = (warp % 4) * 32 + half * 16 + k * kRowsPass + lane / kChunks;
-          *reinterpret_cast<uint4 *>(&sm.q[j][tile_at(at, chunk)]) = make_uint4(w[k].x ^ flip, w[k].y ^ flip, w[k].z ^ flip, w[k].w ^ flip);
-        }
+        for (int k = 0; k < kPasses; ++k)
+          w[k] = make_uint4(pair_to_half(w[k].x, f), pair_to_half(w[k].y, f), pair_to_half(w[k].z, f), pair_to_half(w[k].w, f));
+      }
+#pragma unroll
+      for (int k = 0; k < kPasses; ++k) {
+        const int at = (warp % 4) * 32 + k * kRowsPass + lane / kChunks;
+        *reinterpret_cast<uint4 *>(&sm.q[j][tile_at(at, chunk)]) = make_uint4(w[k].x ^ flip, w[k].y ^ flip, w[k].z ^ flip, w[k].w ^ flip);
       }
       fence_async_proxy();
       mbar_arrive(&sm.q_full);
@@ -542,12 +561,12 @@ __global__ void __launch_bounds__(kPtThreads, 1) prefix_tensor_kernel(const __gr
       const bool all = (valid[0] & valid[1] & valid[2] & valid[3]) == 0xffffffffu;
       if (__any_sync(0xffffffffu, m == -INFINITY)) {
         // rows without a maximum yet (the first tile; tiles whose pages are bad)
-        const float top = all ? tile_max<T, kFmt, false>(s_at, sm.sk[mt], a.scale_log2, valid) : tile_max<T, kFmt, true>(s_at, sm.sk[mt], a.scale_log2, valid);
+        const float top = all ? tile_max<kFmt, false>(s_at, sm.sk[mt], a.scale_log2, valid) : tile_max<kFmt, true>(s_at, sm.sk[mt], a.scale_log2, valid);
         if (m == -INFINITY) m = top;
         __syncwarp();
       }
       float unit = 1.f;
-      if (kUnits) {
+      if (kWide) {
         float big = max_nan(max_nan(sm.sv[mt][lane], sm.sv[mt][lane + 32]), max_nan(sm.sv[mt][lane + 64], sm.sv[mt][lane + 96]));
 #pragma unroll
         for (int d = 16; d > 0; d >>= 1) big = max_nan(big, __shfl_xor_sync(0xffffffffu, big, d));
@@ -560,8 +579,8 @@ __global__ void __launch_bounds__(kPtThreads, 1) prefix_tensor_kernel(const __gr
       }
       uint32_t w[64];
       float sum;
-      float top = all ? tile_weights<T, kFmt, kUnits, false>(s_at, sm.sk[mt], sm.sv[mt], a.scale_log2, m, unit, valid, w, sum)
-                      : tile_weights<T, kFmt, kUnits, true>(s_at, sm.sk[mt], sm.sv[mt], a.scale_log2, m, unit, valid, w, sum);
+      float top = all ? tile_weights<M, kFmt, false>(s_at, sm.sk[mt], sm.sv[mt], a.scale_log2, m, unit, valid, w, sum)
+                      : tile_weights<M, kFmt, true>(s_at, sm.sk[mt], sm.sv[mt], a.scale_log2, m, unit, valid, w, sum);
       if (__any_sync(0xffffffffu, top > 8.f)) {
         // a maximum rose too far: o and l follow, and the weights are taken again (the scores are still there)
         const float rise = top > 8.f ? top : 0.f, factor = ex2(-rise);
@@ -569,9 +588,9 @@ __global__ void __launch_bounds__(kPtThreads, 1) prefix_tensor_kernel(const __gr
         l *= factor;
         if (i > 0) rescale<D>(o_at, factor);
         if (all)
-          tile_weights<T, kFmt, kUnits, false>(s_at, sm.sk[mt], sm.sv[mt], a.scale_log2, m, unit, valid, w, sum);
+          tile_weights<M, kFmt, false>(s_at, sm.sk[mt], sm.sv[mt], a.scale_log2, m, unit, valid, w, sum);
         else
-          tile_weights<T, kFmt, kUnits, true>(s_at, sm.sk[mt], sm.sv[mt], a.scale_log2, m, unit, valid, w, sum);
+          tile_weights<M, kFmt, true>(s_at, sm.sk[mt], sm.sv[mt], a.scale_log2, m, unit, valid, w, sum);
       }
       l += sum;
       tc_store32(s_at, *reinterpret_cast<uint32_t (*)[32]>(&w[0]));      // the weights take the scores' place
@@ -591,7 +610,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) prefix_tensor_kernel(const __gr
       unsigned char *mine = sm.q[0] + at * (D * 4 + 16);
       const int64_t part = (int64_t)split * a.kv_heads * args.rows + (int64_t)h * args.rows + row0 + row;
       if (row < rows) args.part_ml[part] = make_float2(m, l);
-      const float unit = kUnits ? ref : 1.f;
+      const float unit = kWide ? ref : 1.f;
       uint32_t buf[2][32];
       tc_load32(o_at, buf[0]);
 #pragma unroll

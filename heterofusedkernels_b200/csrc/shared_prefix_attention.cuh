@@ -10,8 +10,11 @@
 // K/V head, seqs * G of them, and only what follows the prefix is read for each sequence alone.
 // A row without any key (no prefix, length 0) is 0 with lse = -inf.
 //
-// 8-bit cache: codes are exact in both 16-bit types, so the products run on codes; the scale of a key multiplies
-// its score, the scale of a value its weight.
+// 8-bit cache: codes are exact in fp16, so the products run on codes in fp16; the scale of a key multiplies its score,
+// the scale of a value its weight.  bf16 queries become fp16 numbers times a power of two that brings the largest to
+// 2^14: they have fewer bits than fp16, so only what is 2^29 times smaller than the largest loses any, 2^-40 of it.
+// Weights are fp16 then, four times as exact as bf16 ones.  (The conversion of e4m3 to fp16 is one instruction for two
+// codes; to bf16 it is five, which made up a third of the work of a tile.)
 #pragma once
 
 #include <type_traits>
@@ -38,6 +41,7 @@ struct AttnArgs {
   int64_t own_cap;                // max_blocks * block_size: longest length the tables can name
   int seqs, kv_heads, group;
   FastDiv block, per_group;       // block size; group
+  int tile;                       // keys of a tile of the line
   float scale_log2;               // scale * log2 e
   // partial results (workspace)
   int *cu;                        // [seqs + 1] first tile of each sequence, per (K/V head, row tile)
@@ -56,72 +60,79 @@ template <typename T>
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
 template <>
 __device__ __forceinline__ void mma16816<__nv_bfloat16>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 template <>
 __device__ __forceinline__ void mma16816<__half>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// ---- codes to a 16-bit type: the four codes of a word as two pairs, exact ----------------------------------
-// e4m3 to bf16: sign, exponent and mantissa moved to their places are the number times 2^-120 (the biases
-// differ by 120; subnormal codes become subnormal numbers), and one multiplication by 2^120 follows.
-// int8 to bf16: with u = the low seven bits, 128 + u and 128 (or 256 where the sign bit is set) differ by the
-// code; both are bf16 numbers whose mantissa is the code's bits.  int8 to fp16: 1024 + (code + 128) - 1152.
-template <typename T, int kFmt>
+// ---- codes to fp16: the four codes of a word as two pairs, exact ------------------------------------------
+// int8: code ^ 0x80 is code + 128; 1024 + (code + 128) is an fp16 number with the code's bits in its mantissa.
+template <int kFmt>
 __device__ __forceinline__ void codes_to_pairs(uint32_t w, uint32_t &lo, uint32_t &hi) {
   if constexpr (kFmt == kFmtE4m3) {
-    if constexpr (std::is_same<T, __half>::value) {
-      const __half2_raw a = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w & 0xffffu), __NV_E4M3);
-      const __half2_raw b = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w >> 16), __NV_E4M3);
-      lo = a.x | ((uint32_t)a.y << 16);
-      hi = b.x | ((uint32_t)b.y << 16);
-    } else {
-      const uint32_t l = __byte_perm(w, 0, 0x1404), h = __byte_perm(w, 0, 0x3424);
-      const uint32_t lb = (l & 0x80008000u) | ((l >> 4) & 0x07f007f0u), hb = (h & 0x80008000u) | ((h >> 4) & 0x07f007f0u);
-      asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(lo) : "r"(lb), "r"(0x7b807b80u));
-      asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(hi) : "r"(hb), "r"(0x7b807b80u));
-    }
-  } else if constexpr (std::is_same<T, __half>::value) {
+    const __half2_raw a = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w & 0xffffu), __NV_E4M3);
+    const __half2_raw b = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w >> 16), __NV_E4M3);
+    lo = a.x | ((uint32_t)a.y << 16);
+    hi = b.x | ((uint32_t)b.y << 16);
+  } else {
     const uint32_t u = w ^ 0x80808080u;
     const uint32_t l = __byte_perm(u, 0x64646464u, 0x4140), h = __byte_perm(u, 0x64646464u, 0x4342);
     asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(lo) : "r"(l), "r"(0x64806480u));
     asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(hi) : "r"(h), "r"(0x64806480u));
-  } else {
-    const uint32_t l = __byte_perm(w, 0x43434343u, 0x4140), h = __byte_perm(w, 0x43434343u, 0x4342);
-    asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(lo) : "r"(l & 0xff7fff7fu), "r"(l & 0xff80ff80u));
-    asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(hi) : "r"(h & 0xff7fff7fu), "r"(h & 0xff80ff80u));
   }
+}
+
+// Type of the products' operands.
+template <typename T, int kFmt>
+using Operand = typename std::conditional<kFmt == kFmtRaw, T, __half>::type;
+
+// bf16 queries as fp16: largest magnitude of a pair (infinities and NaN left out), the power of two that takes the
+// largest of all into [2^14, 2^15), and the pair times it.
+__device__ __forceinline__ float largest_of_pair(uint32_t w) {
+  const uint32_t lo = (w << 16) & 0x7fffffffu, hi = w & 0x7fff0000u;
+  return fmaxf(lo < 0x7f800000u ? __uint_as_float(lo) : 0.f, hi < 0x7f800000u ? __uint_as_float(hi) : 0.f);
+}
+__device__ __forceinline__ int shift_to_half(float largest) {
+  const int e = (int)(__float_as_uint(largest) >> 23);   // biased exponent
+  return largest == 0.f ? 0 : max(-126, min(126, 127 + 14 - e));
+}
+__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
+__device__ __forceinline__ uint32_t pair_to_half(uint32_t w, float factor) {
+  const float2 f = Pair<__nv_bfloat16>::unpack(w);
+  return Pair<__half>::pack(f.x * factor, f.y * factor);
 }
 
 // ---- how the work is laid out -------------------------------------------------------------------------------
 // An ITEM is 16 rows of queries against one range of keys: for the prefix a (K/V head, 16 of the seqs * group
-// rows), for a sequence's own keys a (sequence, K/V head, 16 of the group's rows).  Keys go by tiles of 16.
+// rows), for a sequence's own keys a (sequence, K/V head, 16 of the group's rows).  Keys go by tiles of 16, of an 8-bit cache by tiles of 32: 8 KB at head_dim 128.
 // All tiles of all items form one line, items of the prefix first, that is cut into equal pieces, one to a
 // WARP: none has more than one tile more than another, whatever the lengths are (they are known on the
 // device only).  A piece may end one item and begin the next.  The part of warp w of item i has the number
 // w + i: along the line either grows, so no two parts share a number and there are at most warps + items.
-constexpr int kTileKeys = 16;
+__host__ __device__ constexpr int tile_keys(int fmt) { return fmt == HFK_KV_RAW ? 16 : 32; }
 
 struct AttnLine {
   int row_tiles, own_tiles;       // tiles of 16 rows: of the prefix's rows, of a group
-  int prefix_items, prefix_tiles; // tiles of 16 keys of an item
+  int prefix_items, prefix_tiles; // tiles of keys of an item
   int per_seq;                    // items of a sequence
-  __host__ __device__ AttnLine(int seqs, int kv_heads, int group, int prefix_len) {
+  int tile;                       // keys of a tile
+  __host__ __device__ AttnLine(int seqs, int kv_heads, int group, int prefix_len, int tile) : tile(tile) {
     row_tiles = (seqs * group + 15) / 16;
     own_tiles = (group + 15) / 16;
-    prefix_tiles = (prefix_len + kTileKeys - 1) / kTileKeys;
+    prefix_tiles = (prefix_len + tile - 1) / tile;
     prefix_items = prefix_tiles > 0 ? row_tiles * kv_heads : 0;
     per_seq = kv_heads * own_tiles;
   }
   __host__ __device__ int64_t items(int seqs) const { return prefix_items + (int64_t)seqs * per_seq; }
   // Most tiles the line can have; the host takes so few sequences at a time that they number less than 2^31.
   __host__ __device__ int64_t most_tiles(int seqs, int64_t own_cap) const {
-    return (int64_t)prefix_items * prefix_tiles + (int64_t)seqs * per_seq * ((own_cap + kTileKeys - 1) / kTileKeys);
+    return (int64_t)prefix_items * prefix_tiles + (int64_t)seqs * per_seq * ((own_cap + tile - 1) / tile);
   }
 };
 
@@ -154,7 +165,7 @@ __device__ __forceinline__ void scan_tiles(const AttnArgs &a, int *cu, int *warp
   int n[kMost], sum = 0;
 #pragma unroll
   for (int k = 0; k < kMost; ++k) {
-    n[k] = k < per && s0 + k < a.seqs ? (int)((own_length(a, s0 + k, blockIdx.x == 0) + kTileKeys - 1) / kTileKeys) : 0;
+    n[k] = k < per && s0 + k < a.seqs ? (int)((own_length(a, s0 + k, blockIdx.x == 0) + a.tile - 1) / a.tile) : 0;
     sum += n[k];
   }
   int inc = sum;
@@ -236,21 +247,18 @@ __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_gr
 __device__ __forceinline__ void launch_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void launch_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
-// Warps of a CTA.  A 16-bit cache of long sequences is bound by HBM with 8 (two tiles of 8 KB in flight each, 355 us for
-// 2.4 GB); an 8-bit cache has half the bytes and more arithmetic to a tile, and 12 hide its latencies better.
-template <int kFmt>
-struct LineWarps {
-  static constexpr int kCount = kFmt == kFmtRaw ? 8 : 12;
-};
+constexpr int kLineWarps = 8;     // of a CTA; one CTA an SM
 
-// Ring of a warp: kStages tiles of 16 keys, K rows, V rows, and for an 8-bit cache their scales.
+// Ring of a warp: kStages tiles, K rows, V rows, and for an 8-bit cache the scales of the keys, then of the values.
 template <int kFmt, int D>
 struct alignas(128) LineRing {
+  static constexpr int kKeys = tile_keys(kFmt);
   static constexpr int kRow = D * (kFmt == kFmtRaw ? 2 : 1);
-  static constexpr int kStages = kRow >= 256 ? 3 : kRow >= 128 ? 4 : 8;
-  unsigned char k[kStages][16 * kRow], v[kStages][16 * kRow];
-  float scales[kStages][32];      // of 16 keys, of 16 values
-  uint32_t valid[kStages + (kStages & 1)];
+  static constexpr int kStages = D == 128 ? 3 : 5;
+  unsigned char k[kStages][kKeys * kRow], v[kStages][kKeys * kRow];
+  float scales[kStages][2 * kKeys];
+  uint32_t valid[kStages];
+  LineItem items[kStages + 1];    // items whose tiles are in the ring or next to come, by the number of changes so far
 };
 
 // ---- the kernel ------------------------------------------------------------------------------------------------
@@ -264,18 +272,19 @@ struct alignas(128) LineRing {
 //
 // Bound by HBM for long sequences; for short ones by the chain from a sequence's length over its page ids to its rows.
 template <typename T, int kFmt, int D>
-__global__ void __launch_bounds__(LineWarps<kFmt>::kCount * 32, 1) shared_prefix_attention_kernel(const __grid_constant__ AttnArgs a) {
+__global__ void __launch_bounds__(kLineWarps * 32, 1) shared_prefix_attention_kernel(const __grid_constant__ AttnArgs a) {
   using Ring = LineRing<kFmt, D>;
+  using M = Operand<T, kFmt>;
   constexpr int kElt = kFmt == kFmtRaw ? 2 : 1;
-  constexpr int kRow = Ring::kRow, kStages = Ring::kStages;
+  constexpr int kKeys = Ring::kKeys, kRow = Ring::kRow, kStages = Ring::kStages;
   constexpr int kKc = kRow / 64;                          // 16-byte chunks of a K row per lane
   constexpr int kVb = kRow / 8 < 16 ? kRow / 8 : 16;      // bytes of a V chunk
   constexpr int kVc = kRow / 8 / kVb;                     // V chunks of a row per lane
   constexpr int kVe = kVb / kElt;                         // values of a V chunk
   constexpr int kE = 16 / kElt;                           // values of a K chunk
   constexpr int kCpr = kRow / 16, kRowsPass = 32 / kCpr;  // copies: chunks of a row, rows of a warp's pass
-  constexpr bool kUnits = kFmt != kFmtRaw && std::is_same<T, __half>::value;
-  constexpr int kLineWarps = LineWarps<kFmt>::kCount;
+  constexpr int kN = kKeys / 8;                           // blocks of 8 keys
+  constexpr bool kCodes = kFmt != kFmtRaw;
   extern __shared__ __align__(128) unsigned char smem_raw[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   Ring &ring = reinterpret_cast<Ring *>(smem_raw)[warp];
@@ -286,96 +295,112 @@ __global__ void __launch_bounds__(LineWarps<kFmt>::kCount * 32, 1) shared_prefix
   scan_tiles<kLineWarps * 32>(a, cu, warp_sums);
   if (blockIdx.x == 0)
     for (int s = threadIdx.x; s <= a.seqs; s += kLineWarps * 32) a.cu[s] = cu[s];
-  const AttnLine line(a.seqs, a.kv_heads, a.group, a.prefix_len);
+  const AttnLine line(a.seqs, a.kv_heads, a.group, a.prefix_len, kKeys);
   const int total = line.prefix_items * line.prefix_tiles + cu[a.seqs] * line.per_seq;
   const int warps = line_warps((int)gridDim.x * kLineWarps, total);
   // neighbouring pieces go to different SMs: a batch of few tiles is spread over all of them
   const int me = warp * (int)gridDim.x + (int)blockIdx.x;
   const int begin = me < warps ? first_tile(me, warps, total) : total, end = me < warps ? first_tile(me + 1, warps, total) : total;
 
-  // ---- loads: tile `load_at` of the line is the next to be brought in
+  // ---- loads: tile `load_at` of the line is the next to be brought in, in groups of 16 keys
+  // (This and line_item have one place each in the code: with the loads ahead of the loop and the items of loads and
+  // products found separately, warps waited for instructions more than for anything else.)
   LineItem in = {};
-  int load_at = begin;
-  // Pages of a multiple of 16 tokens: a tile lies in one page, and lane j holds the id of the page of tile ids_from + j of
-  // the item.  Other pages: lane j holds the id of the page of key j & 15 of the tile.
-  const bool whole = a.block.d % kTileKeys == 0;
+  in.tile = -1;               // no item yet
+  int load_at = begin, loads = 0;
+  // Pages of a multiple of 16 tokens: a group lies in one page, and lane j holds the id of the page of group ids_from + j
+  // of the item.  Other pages: lane j holds the id of the page of key j & 15 of the group.
+  const bool whole = a.block.d % 16 == 0;
   int64_t id = -1;
   int ids_from = 0;
-  auto fetch_ids = [&]() {
-    const int key = whole ? (in.tile + lane) * kTileKeys : in.tile * kTileKeys + (lane & 15);
+  auto fetch_ids = [&](int group) {
+    const int64_t key = whole ? ((int64_t)group + lane) * 16 : (int64_t)group * 16 + (lane & 15);
     id = key < in.len ? load_id(in.table, a.ids_are_int64, in.table_at + a.block.div((uint32_t)key)) : -1;
-    ids_from = in.tile;
+    ids_from = group;
   };
-  int load_stage = 0;
+  int load_stage = 0, changes = 0;
   const int chunk = lane % kCpr, sub = lane / kCpr;
+  auto load_group = [&](int group, int part) -> uint32_t {     // group `part` of the tile; returns which keys count
+    const int key0 = group * 16;
+    const uint32_t kb = smem_addr(ring.k[load_stage]) + part * 16 * kRow, vb = smem_addr(ring.v[load_stage]) + part * 16 * kRow;
+    // lanes 0-15 the scales of the keys, 16-31 those of the values
+    const uint32_t sb = smem_addr(&ring.scales[load_stage][(lane < 16 ? 0 : kKeys) + part * 16 + (lane & 15)]);
+    if (whole) {
+      const int64_t page_id = __shfl_sync(0xffffffffu, id, group - ids_from);
+      const bool ok = page_id >= 0 && page_id < a.num_blocks;
+      if (!ok && lane == 0 && key0 < in.len) raise_status(HFK_DEV_BAD_DEVICE_BLOCK_ID);
+      const int64_t page = ok ? page_id * a.block_stride : 0;
+      const int left = ok ? in.len - key0 : 0;              // rows behind the last key are zero
+      // row of the page of the group's first key
+      const uint32_t b = a.block.div((uint32_t)key0);
+      const uint32_t row = ((uint32_t)key0 - b * a.block.d) * a.kv_heads + in.h;
+      const int64_t from = page + (int64_t)(row + sub * a.kv_heads) * kRow + chunk * 16;
+      const int step = kRowsPass * a.kv_heads * kRow;       // bytes from pass to pass, less than a page
+      const unsigned char *kp = a.k_cache + from, *vp = a.v_cache + from;
+      if (kCodes) {
+        const bool mine = (lane & 15) < left;
+        cp_async4(sb, (lane < 16 ? a.k_cache : a.v_cache) + page + a.scales_at + (mine ? (int64_t)(row + (lane & 15) * a.kv_heads) * 4 : 0), mine);
+      }
+#pragma unroll
+      for (int r = 0; r < 16; r += kRowsPass) {
+        const int at = r + sub;
+        const bool mine = at < left;
+        const int kc = kCpr >= 8 ? chunk ^ ((at & 1) << 2) : chunk;
+        const int vc = kCpr >= 8 ? chunk ^ (((at >> 1) & 3) << 1) : chunk ^ ((at >> 1) & 3);
+        cp_async16(kb + at * kRow + kc * 16, mine ? kp : a.k_cache, mine);
+        cp_async16(vb + at * kRow + vc * 16, mine ? vp : a.v_cache, mine);
+        kp += step;
+        vp += step;
+      }
+      return left >= 16 ? 0xffffu : (1u << max(left, 0)) - 1u;
+    }
+    const int key = key0 + (lane & 15);
+    const bool inside = key < in.len;
+    const bool ok = inside && id >= 0 && id < a.num_blocks;
+    if (inside && !ok) raise_status(HFK_DEV_BAD_DEVICE_BLOCK_ID);
+    const uint32_t row = ((uint32_t)key - a.block.div((uint32_t)key) * a.block.d) * a.kv_heads + in.h;
+    const int64_t page = ok ? id * a.block_stride : 0;
+    const int64_t off = ok ? page + (int64_t)row * kRow : -1;
+    if (kCodes) cp_async4(sb, (lane < 16 ? a.k_cache : a.v_cache) + page + a.scales_at + (ok ? (int64_t)row * 4 : 0), ok);
+#pragma unroll
+    for (int r = 0; r < 16; r += kRowsPass) {
+      const int at = r + sub;
+      const int64_t o = __shfl_sync(0xffffffffu, off, at);
+      const int64_t from = (o < 0 ? 0 : o) + chunk * 16;
+      const int kc = kCpr >= 8 ? chunk ^ ((at & 1) << 2) : chunk;
+      const int vc = kCpr >= 8 ? chunk ^ (((at >> 1) & 3) << 1) : chunk ^ ((at >> 1) & 3);
+      cp_async16(kb + at * kRow + kc * 16, a.k_cache + from, o >= 0);
+      cp_async16(vb + at * kRow + vc * 16, a.v_cache + from, o >= 0);
+    }
+    return __ballot_sync(0xffffffffu, ok) & 0xffffu;
+  };
   auto load_tile = [&]() {
     if (load_at < end) {
-      const int key0 = in.tile * kTileKeys;
-      const uint32_t kb = smem_addr(ring.k[load_stage]), vb = smem_addr(ring.v[load_stage]);
-      const uint32_t sb = smem_addr(&ring.scales[load_stage][lane]);
-      uint32_t mask;
-      if (whole) {
-        const int64_t page_id = __shfl_sync(0xffffffffu, id, in.tile - ids_from);
-        const bool ok = page_id >= 0 && page_id < a.num_blocks;
-        if (!ok && lane == 0) raise_status(HFK_DEV_BAD_DEVICE_BLOCK_ID);
-        const int64_t page = ok ? page_id * a.block_stride : 0;
-        const int left = ok ? in.len - key0 : 0;            // rows behind the last key are zero
-        mask = left >= 16 ? 0xffffu : (1u << max(left, 0)) - 1u;
-        // row of the page of the tile's first key
-        const uint32_t b = a.block.div((uint32_t)key0);
-        const uint32_t row = ((uint32_t)key0 - b * a.block.d) * a.kv_heads + in.h;
-        const int64_t from = page + (int64_t)(row + sub * a.kv_heads) * kRow + chunk * 16;
-        const int step = kRowsPass * a.kv_heads * kRow;     // bytes from pass to pass, less than a page
-        const unsigned char *kp = a.k_cache + from, *vp = a.v_cache + from;
-        if (kFmt != kFmtRaw) {  // lanes 0-15 the scales of the keys, 16-31 those of the values
-          const bool mine = (lane & 15) < left;
-          cp_async4(sb, (lane < 16 ? a.k_cache : a.v_cache) + page + a.scales_at + (mine ? (int64_t)(row + (lane & 15) * a.kv_heads) * 4 : 0), mine);
+      if (loads > 0) {
+        uint32_t mask = 0;
+        const int group = in.tile * (kKeys / 16);
+#pragma unroll 1
+        for (int part = 0; part < kKeys / 16; ++part) {
+          if (part > 0 && !whole) fetch_ids(group + part);
+          mask |= load_group(group + part, part) << (16 * part);
         }
-#pragma unroll
-        for (int r = 0; r < 16; r += kRowsPass) {
-          const int at = r + sub;
-          const bool mine = at < left;
-          const int kc = kCpr >= 8 ? chunk ^ ((at & 1) << 2) : chunk;
-          const int vc = kCpr >= 8 ? chunk ^ (((at >> 1) & 3) << 1) : chunk ^ ((at >> 1) & 3);
-          const int64_t on = (int64_t)(r / kRowsPass) * step;
-          cp_async16(kb + at * kRow + kc * 16, mine ? kp + on : a.k_cache, mine);
-          cp_async16(vb + at * kRow + vc * 16, mine ? vp + on : a.v_cache, mine);
-        }
-      } else {
-        const int key = key0 + (lane & 15);
-        const bool inside = key < in.len;
-        const bool ok = inside && id >= 0 && id < a.num_blocks;
-        if (inside && !ok) raise_status(HFK_DEV_BAD_DEVICE_BLOCK_ID);
-        const uint32_t row = ((uint32_t)key - a.block.div((uint32_t)key) * a.block.d) * a.kv_heads + in.h;
-        const int64_t page = ok ? id * a.block_stride : 0;
-        const int64_t off = ok ? page + (int64_t)row * kRow : -1;
-        if (kFmt != kFmtRaw)
-          cp_async4(sb, (lane < 16 ? a.k_cache : a.v_cache) + page + a.scales_at + (ok ? (int64_t)row * 4 : 0), ok);
-        mask = __ballot_sync(0xffffffffu, ok) & 0xffffu;
-#pragma unroll
-        for (int r = 0; r < 16; r += kRowsPass) {
-          const int at = r + sub;
-          const int64_t o = __shfl_sync(0xffffffffu, off, at);
-          const int64_t from = (o < 0 ? 0 : o) + chunk * 16;
-          const int kc = kCpr >= 8 ? chunk ^ ((at & 1) << 2) : chunk;
-          const int vc = kCpr >= 8 ? chunk ^ (((at >> 1) & 3) << 1) : chunk ^ ((at >> 1) & 3);
-          cp_async16(kb + at * kRow + kc * 16, a.k_cache + from, o >= 0);
-          cp_async16(vb + at * kRow + vc * 16, a.v_cache + from, o >= 0);
-        }
+        if (lane == 0) ring.valid[load_stage] = mask;
+        load_stage = load_stage + 1 == kStages ? 0 : load_stage + 1;
+        ++load_at;
       }
-      if (lane == 0) ring.valid[load_stage] = mask;
-      ++load_at;
-      if (load_at < end) {
-        if (++in.tile == in.tiles) {
+      if (load_at < end) {    // the next tile's page ids, a tile ahead of their use
+        const bool next_item = ++in.tile == in.tiles;
+        if (next_item) {
           in = line_item(a, line, cu, load_at);
-          fetch_ids();
-        } else if (!whole || in.tile - ids_from == 32) {
-          fetch_ids();
+          if (lane == 0) ring.items[changes % (kStages + 1)] = in;
+          ++changes;
         }
+        const int next = in.tile * (kKeys / 16);
+        if (next_item || !whole || next - ids_from >= 32) fetch_ids(next);
       }
-      load_stage = load_stage + 1 == kStages ? 0 : load_stage + 1;
     }
-    cp_async_commit();        // one group a tile, empty behind the last one
+    ++loads;
+    cp_async_commit();        // one group a tile, empty before the first and behind the last one
   };
   // queries: rows g and g + 8, the chunks this lane also takes of K
   uint32_t qf[D / 16][4];
@@ -400,122 +425,139 @@ __global__ void __launch_bounds__(LineWarps<kFmt>::kCount * 32, 1) shared_prefix
         }
     }
   };
-  if (begin < end) {
-    in = line_item(a, line, cu, begin);
-    fetch_ids();
-    load_queries(in);         // under way while the first tiles are asked for
-  }
-  LineItem x = in;
-#pragma unroll
-  for (int i = 0; i < kStages - 1; ++i) load_tile();
-
-  int stage = 0;
-  for (int at = begin; at < end;) {
-    if (at != begin) {
-      x = line_item(a, line, cu, at);
+  int stage = 0, items = 0;
+  LineItem x;
+  float by[2], m[2], l[2], ref, unit;
+  float o[D / 8][4];
+#pragma unroll 1
+  for (int at = begin - kStages; at < end; ++at) {
+    __syncwarp();             // the stage that is loaded now has been read by every lane
+    load_tile();
+    if (at < begin) continue;
+    const bool first = at == begin || x.tile == x.tiles;
+    if (first) {              // an item begins
+      x = ring.items[items % (kStages + 1)];
+      ++items;
       load_queries(x);
     }
-    const int stop = min(end, at + (x.tiles - x.tile));
-
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, ref = 0.f;
-    float o[D / 8][4];
+    cp_async_wait<kStages - 1>();
+    __syncwarp();             // every lane's copies of this tile have arrived
+    if (first) {
+by[0] = by[1] = a.scale_log2;              // what a row's products are multiplied by
+      if constexpr (kCodes && !std::is_same<T, __half>::value) {
 #pragma unroll
-    for (int j = 0; j < D / 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
-
-    for (; at < stop; ++at) {
-      cp_async_wait<kStages - 2>();
-      __syncwarp();           // every lane's copies of this tile have arrived, and the stage before it has been read
-      load_tile();
-      const unsigned char *ks = ring.k[stage], *vs = ring.v[stage];
-      const uint32_t valid = ring.valid[stage];
-      const bool live[4] = {(valid >> (2 * t) & 1) != 0, (valid >> (2 * t + 1) & 1) != 0, (valid >> (2 * t + 8) & 1) != 0,
-                            (valid >> (2 * t + 9) & 1) != 0};
-      float sk[4] = {0.f, 0.f, 0.f, 0.f}, sv[4] = {0.f, 0.f, 0.f, 0.f};
-      if (kFmt != kFmtRaw) {
-        const float *sc = ring.scales[stage];
+        for (int half = 0; half < 2; ++half) {
+          float top = 0.f;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const float2 f = *reinterpret_cast<const float2 *>(sc + 8 * i + 2 * t), h2 = *reinterpret_cast<const float2 *>(sc + 16 + 8 * i + 2 * t);
-          sk[2 * i] = f.x;
-          sk[2 * i + 1] = f.y;
-          sv[2 * i] = h2.x;
-          sv[2 * i + 1] = h2.y;
+          for (int k = 0; k < D / 16; ++k) top = fmaxf(top, fmaxf(largest_of_pair(qf[k][half]), largest_of_pair(qf[k][half + 2])));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+          const int e = shift_to_half(top);
+          const float f = power_of_two(e);
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k) {
+            qf[k][half] = pair_to_half(qf[k][half], f);
+            qf[k][half + 2] = pair_to_half(qf[k][half + 2], f);
+          }
+          by[half] *= power_of_two(-e);
         }
       }
+      m[0] = m[1] = -INFINITY;
+      l[0] = l[1] = ref = unit = 0.f;
+#pragma unroll
+      for (int j = 0; j < D / 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
+    }
+    {
+      const unsigned char *ks = ring.k[stage], *vs = ring.v[stage];
+      const uint32_t valid = ring.valid[stage];
 
-      // scores of 16 rows and 16 keys: s[n][0..1] row g, s[n][2..3] row g + 8, keys 8n + 2t, 8n + 2t + 1
-      float s[2][4];
+      // scores of 16 rows and kKeys keys: s[n][0..1] row g, s[n][2..3] row g + 8, keys 8n + 2t, 8n + 2t + 1
+      float s[kN][4];
 #pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
-        const int kr = g + 8 * n;
+      for (int n = 0; n < kN; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
 #pragma unroll
-        for (int c = 0; c < kKc; ++c) {
-          const int chunk = kCpr >= 8 ? (c * 4 + t) ^ ((kr & 1) << 2) : c * 4 + t;
-          const uint4 kw = *reinterpret_cast<const uint4 *>(ks + kr * kRow + chunk * 16);
+      for (int c = 0; c < kKc; ++c)
+#pragma unroll
+        for (int n = 0; n < kN; ++n) {
+          const int kr = g + 8 * n;
+          const int at16 = kCpr >= 8 ? (c * 4 + t) ^ ((kr & 1) << 2) : c * 4 + t;
+          const uint4 kw = *reinterpret_cast<const uint4 *>(ks + kr * kRow + at16 * 16);
           const uint32_t w[4] = {kw.x, kw.y, kw.z, kw.w};
-          if constexpr (kFmt == kFmtRaw) {
-            mma16816<T>(s[n], qf[2 * c], w[0], w[1]);
-            mma16816<T>(s[n], qf[2 * c + 1], w[2], w[3]);
+          if constexpr (!kCodes) {
+            mma16816<M>(s[n], qf[2 * c], w[0], w[1]);
+            mma16816<M>(s[n], qf[2 * c + 1], w[2], w[3]);
           } else {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               uint32_t b0, b1;
-              codes_to_pairs<T, kFmt>(w[i], b0, b1);
-              mma16816<T>(s[n], qf[4 * c + i], b0, b1);
+              codes_to_pairs<kFmt>(w[i], b0, b1);
+              mma16816<M>(s[n], qf[4 * c + i], b0, b1);
             }
           }
         }
-      }
+      float sv[kN][2];        // scales of the values
       float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int i = 2 * n + e;
-          const float f = kFmt == kFmtRaw ? a.scale_log2 : a.scale_log2 * sk[i];
-          s[n][e] = live[i] ? s[n][e] * f : -INFINITY;
-          s[n][2 + e] = live[i] ? s[n][2 + e] * f : -INFINITY;
-          top[0] = fmaxf(top[0], s[n][e]);
-          top[1] = fmaxf(top[1], s[n][2 + e]);
+      for (int n = 0; n < kN; ++n) {
+        float2 sk = make_float2(1.f, 1.f);
+        if (kCodes) {
+          sk = *reinterpret_cast<const float2 *>(&ring.scales[stage][8 * n + 2 * t]);
+          const float2 f = *reinterpret_cast<const float2 *>(&ring.scales[stage][kKeys + 8 * n + 2 * t]);
+          sv[n][0] = f.x;
+          sv[n][1] = f.y;
         }
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          s[n][2 * r] *= kCodes ? by[r] * sk.x : by[r];
+          s[n][2 * r + 1] *= kCodes ? by[r] * sk.y : by[r];
+        }
+      }
+      constexpr uint32_t kAll = kKeys == 32 ? 0xffffffffu : 0xffffu;
+      if (valid != kAll) {
+#pragma unroll
+        for (int n = 0; n < kN; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            if (!(valid >> (8 * n + 2 * t + e) & 1)) s[n][e] = s[n][2 + e] = -INFINITY;
+      }
+#pragma unroll
+      for (int n = 0; n < kN; ++n)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) top[r] = fmaxf(top[r], fmaxf(s[n][2 * r], s[n][2 * r + 1]));
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
         top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
         top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
       }
-      // fp16 weights of an 8-bit cache: weight * scale may leave fp16's range, so o is kept in units of the
-      // largest scale of a value so far
-      float grow = 1.f, unit = 1.f;
-      if (kUnits) {
-        float big = max_nan(max_nan(sv[0], sv[1]), max_nan(sv[2], sv[3]));
-        big = max_nan(big, __shfl_xor_sync(0xffffffffu, big, 1));
-        big = max_nan(big, __shfl_xor_sync(0xffffffffu, big, 2));
-        const float next = max_nan(ref, big);
-        grow = next == ref || next == 0.f ? 1.f : ref / next;
-        unit = next == 0.f ? 0.f : 1.f / next;
-        ref = next;
+      // m follows a row's maximum only where it is 2^8 behind: weights up to 2^8 are as exact as weights up to 1
+      bool move = top[0] > m[0] + 8.f || top[1] > m[1] + 8.f;
+      // fp16 weights of an 8-bit cache: weight * scale may leave fp16's range, so o is kept in units of (a quarter or
+      // more of) the largest scale of a value so far
+      float big = 0.f;
+      if (kCodes) {
+#pragma unroll
+        for (int n = 0; n < kN; ++n) big = max_nan(big, max_nan(sv[n][0], sv[n][1]));
+        move = move || !(big <= 4.f * ref);       // also a NaN
       }
-      float alpha[2];
+      if (__any_sync(0xffffffffu, move)) {
+        float alpha[2];
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const float next = fmaxf(m[r], top[r]);
-        const float safe = next == -INFINITY ? 0.f : next;
-        alpha[r] = ex2(m[r] - safe);
-        m[r] = next;
-        float sum = 0.f;
-#pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const float p = ex2(s[n][2 * r + e] - safe);
-            sum += p;
-            s[n][2 * r + e] = kFmt == kFmtRaw ? p : p * (sv[2 * n + e] * unit);
+        for (int r = 0; r < 2; ++r) {
+          const float next = top[r] > m[r] + 8.f ? top[r] : m[r];
+          alpha[r] = next == m[r] ? 1.f : ex2(m[r] - next);
+          m[r] = next;
+          l[r] *= alpha[r];
+        }
+        if (kCodes) {
+          big = max_nan(big, __shfl_xor_sync(0xffffffffu, big, 1));
+          big = max_nan(big, __shfl_xor_sync(0xffffffffu, big, 2));
+          if (!(big <= 4.f * ref)) {              // the same in every lane
+            alpha[0] *= ref / big;
+            alpha[1] *= ref / big;
+            ref = big;
+            unit = 1.f / big;
           }
-        l[r] = l[r] * alpha[r] + sum;
-        alpha[r] *= grow;
-      }
-      if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
+        }
 #pragma unroll
         for (int j = 0; j < D / 8; ++j) {
           o[j][0] *= alpha[0];
@@ -524,47 +566,66 @@ __global__ void __launch_bounds__(LineWarps<kFmt>::kCount * 32, 1) shared_prefix
           o[j][3] *= alpha[1];
         }
       }
-      const uint32_t pf[4] = {Pair<T>::pack(s[0][0], s[0][1]), Pair<T>::pack(s[0][2], s[0][3]),
-                              Pair<T>::pack(s[1][0], s[1][1]), Pair<T>::pack(s[1][2], s[1][3])};
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const float safe = m[r] == -INFINITY ? 0.f : m[r];
+        float sum = 0.f;
+#pragma unroll
+        for (int n = 0; n < kN; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float p = ex2(s[n][2 * r + e] - safe);
+            sum += p;
+            s[n][2 * r + e] = kCodes ? p * (sv[n][e] * unit) : p;
+          }
+        l[r] += sum;
+      }
       // o column q (0..7) of block j = c * kVe + e holds value (c * 8 + q) * kVe + e of the head
 #pragma unroll
-      for (int c = 0; c < kVc; ++c) {
-        uint32_t w[4][4];
+      for (int step = 0; step < kKeys / 16; ++step) {
+        const uint32_t pf[4] = {Pair<M>::pack(s[2 * step][0], s[2 * step][1]), Pair<M>::pack(s[2 * step][2], s[2 * step][3]),
+                                Pair<M>::pack(s[2 * step + 1][0], s[2 * step + 1][1]), Pair<M>::pack(s[2 * step + 1][2], s[2 * step + 1][3])};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int vr = 2 * t + (i & 1) + 8 * (i >> 1);
-          if constexpr (kVb == 16) {
-            const uint4 x4 = *reinterpret_cast<const uint4 *>(vs + vr * kRow + (((c * 8 + g) ^ (((vr >> 1) & 3) << 1)) * 16));
-            w[i][0] = x4.x;
-            w[i][1] = x4.y;
-            w[i][2] = x4.z;
-            w[i][3] = x4.w;
-          } else {
-            const uint2 x2 = *reinterpret_cast<const uint2 *>(vs + vr * kRow + (((g >> 1) ^ ((vr >> 1) & 3)) * 16) + (g & 1) * 8);
-            w[i][0] = x2.x;
-            w[i][1] = x2.y;
+        for (int c = 0; c < kVc; ++c) {
+          uint32_t w[4][4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int vr = 16 * step + 2 * t + (i & 1) + 8 * (i >> 1);
+            if constexpr (kVb == 16) {
+              const uint4 x4 = *reinterpret_cast<const uint4 *>(vs + vr * kRow + (((c * 8 + g) ^ (((vr >> 1) & 3) << 1)) * 16));
+              w[i][0] = x4.x;
+              w[i][1] = x4.y;
+              w[i][2] = x4.z;
+              w[i][3] = x4.w;
+            } else {
+              const uint2 x2 = *reinterpret_cast<const uint2 *>(vs + vr * kRow + (((g >> 1) ^ ((vr >> 1) & 3)) * 16) + (g & 1) * 8);
+              w[i][0] = x2.x;
+              w[i][1] = x2.y;
+            }
           }
-        }
 #pragma unroll
-        for (int i = 0; i < kVb / 4; ++i) {
-          if constexpr (kFmt == kFmtRaw) {
-            mma16816<T>(o[c * kVe + 2 * i], pf, __byte_perm(w[0][i], w[1][i], 0x5410), __byte_perm(w[2][i], w[3][i], 0x5410));
-            mma16816<T>(o[c * kVe + 2 * i + 1], pf, __byte_perm(w[0][i], w[1][i], 0x7632), __byte_perm(w[2][i], w[3][i], 0x7632));
-          } else {
-            uint32_t x0, x1, x2, x3, y0, y1, y2, y3;
-            codes_to_pairs<T, kFmt>(__byte_perm(w[0][i], w[1][i], 0x5140), x0, x1);
-            codes_to_pairs<T, kFmt>(__byte_perm(w[0][i], w[1][i], 0x7362), x2, x3);
-            codes_to_pairs<T, kFmt>(__byte_perm(w[2][i], w[3][i], 0x5140), y0, y1);
-            codes_to_pairs<T, kFmt>(__byte_perm(w[2][i], w[3][i], 0x7362), y2, y3);
-            mma16816<T>(o[c * kVe + 4 * i], pf, x0, y0);
-            mma16816<T>(o[c * kVe + 4 * i + 1], pf, x1, y1);
-            mma16816<T>(o[c * kVe + 4 * i + 2], pf, x2, y2);
-            mma16816<T>(o[c * kVe + 4 * i + 3], pf, x3, y3);
+          for (int i = 0; i < kVb / 4; ++i) {
+            if constexpr (!kCodes) {
+              mma16816<M>(o[c * kVe + 2 * i], pf, __byte_perm(w[0][i], w[1][i], 0x5410), __byte_perm(w[2][i], w[3][i], 0x5410));
+              mma16816<M>(o[c * kVe + 2 * i + 1], pf, __byte_perm(w[0][i], w[1][i], 0x7632), __byte_perm(w[2][i], w[3][i], 0x7632));
+            } else {
+              uint32_t x0, x1, x2, x3, y0, y1, y2, y3;
+              codes_to_pairs<kFmt>(__byte_perm(w[0][i], w[1][i], 0x5140), x0, x1);
+              codes_to_pairs<kFmt>(__byte_perm(w[0][i], w[1][i], 0x7362), x2, x3);
+              codes_to_pairs<kFmt>(__byte_perm(w[2][i], w[3][i], 0x5140), y0, y1);
+              codes_to_pairs<kFmt>(__byte_perm(w[2][i], w[3][i], 0x7362), y2, y3);
+              mma16816<M>(o[c * kVe + 4 * i], pf, x0, y0);
+              mma16816<M>(o[c * kVe + 4 * i + 1], pf, x1, y1);
+              mma16816<M>(o[c * kVe + 4 * i + 2], pf, x2, y2);
+              mma16816<M>(o[c * kVe + 4 * i + 3], pf, x3, y3);
+            }
           }
         }
       }
       stage = stage + 1 == kStages ? 0 : stage + 1;
     }
+    ++x.tile;
+    if (x.tile != x.tiles && at + 1 != end) continue;
 
     // this warp's part of the item: lane (g, t) has columns 2t and 2t + 1 of every block, which is, for a chunk c, kVe
     // values in a row of the head each
@@ -576,7 +637,7 @@ __global__ void __launch_bounds__(LineWarps<kFmt>::kCount * 32, 1) shared_prefix
       const int row = g + 8 * r;
       if (row < x.rows) {
         if (t == 0) a.part_ml[part * 16 + row] = make_float2(m[r], l[r]);
-        const float unit = kUnits ? ref : 1.f;
+        const float back = kCodes ? ref : 1.f;
         float *dst = a.part_o + (part * 16 + row) * D;
 #pragma unroll
         for (int c = 0; c < kVc; ++c)
@@ -585,8 +646,8 @@ __global__ void __launch_bounds__(LineWarps<kFmt>::kCount * 32, 1) shared_prefix
 #pragma unroll
             for (int e = 0; e < kVe; e += 4)
               *reinterpret_cast<float4 *>(dst + (c * 8 + 2 * t + y) * kVe + e) =
-                  make_float4(o[c * kVe + e][2 * r + y] * unit, o[c * kVe + e + 1][2 * r + y] * unit, o[c * kVe + e + 2][2 * r + y] * unit,
-                              o[c * kVe + e + 3][2 * r + y] * unit);
+                  make_float4(o[c * kVe + e][2 * r + y] * back, o[c * kVe + e + 1][2 * r + y] * back, o[c * kVe + e + 2][2 * r + y] * back,
+                              o[c * kVe + e + 3][2 * r + y] * back);
       }
     }
   }
@@ -619,7 +680,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) shared_prefix_join_kernel(con
   int count[3] = {0, 0, 0};
   int64_t first[3] = {0, 0, 0};
   if (args.warps > 0) {
-    const AttnLine line(a.seqs, a.kv_heads, a.group, a.prefix_len);
+    const AttnLine line(a.seqs, a.kv_heads, a.group, a.prefix_len, a.tile);
     const int in_prefix = line.prefix_items * line.prefix_tiles;
     const int before = a.cu[s], behind = a.cu[s + 1];
     const int total = in_prefix + a.cu[a.seqs] * line.per_seq;
