@@ -6,9 +6,8 @@
 //   0-3, 4-7  softmax of tile 0 and of tile 1: one thread a row, so neither the maximum nor the sum needs a shuffle
 //   8-11      bring K and V tiles into shared memory (asynchronous copies; 8-bit codes are widened on the way)
 //   12        issues the matrix products (13-15 only bring their registers)
-// A thread starts with 128 registers; the softmax keeps the 64 words of its row's weights at once and would spill (what it
-// spilled went to L2, shared memory leaves no L1: 64 us instead of 59 for 2048 rows x 32768 keys), so the groups split
-// the registers 168 + 168 + 120 + 56 = 4 x 128.
+// A thread starts with 128 registers; the warps that widen codes hold two tiles of them and would spill (to L2: shared
+// memory leaves no L1), so the groups split the registers 144 + 144 + 176 + 48 = 4 x 128.
 // TMEM: scores of the two tiles (128 columns each), o of the two tiles (head_dim columns each).  The 16-bit weights
 // take the place of the scores they came from, and the second product reads them from there.  While one tile is
 // in its softmax, the tensor cores work on the other: per 128 keys and tile, at head_dim 128, both products take about
@@ -45,7 +44,7 @@ struct PrefixSmem {
   unsigned char q[2][kTile];
   unsigned char ring[kPtStages][kTile];          // K of tile i in stage 2 (i % 2), V in the next
   int64_t off[kPtMeta][kPtKeys];                 // byte offset of a key's row, -1: leave out
-  alignas(16) float sk[kPtMeta][kPtKeys];         // scales of keys (times scale * log2 e) and of values, 0: leave out
+  alignas(16) float sk[kPtMeta][kPtKeys];         // scales of keys (times scale * log2 e) and of values
   alignas(16) float sv[kPtMeta][kPtKeys];
   uint32_t valid[kPtMeta][4];
   uint64_t full[kPtStages], empty[kPtStages], meta[kPtMeta], s_full[2], p_full[2], o_full, q_full;
@@ -181,38 +180,63 @@ __device__ __forceinline__ void rescale(uint32_t o_at, float factor) {
   }
 }
 
-// Largest score of the tile (in units of log2 e), -inf without a key.
-template <int kFmt, bool kMask>
-__device__ __forceinline__ float tile_max(uint32_t s_at, const float *sk, float scale, const uint32_t (&valid)[4]) {
-  float top = -INFINITY;
+// Scores of keys that do not count become -inf (the last tile of the prefix, pages that are not there), so that
+// what follows needs one form only: every copy of the code below costs instruction cache, and the kernel waited for
+// instructions when it had four.
+__device__ __forceinline__ void mask_scores(uint32_t s_at, const uint32_t *valid) {
 #pragma unroll 1
   for (int c = 0; c < 4; ++c) {
     uint32_t s[32];
     tc_load32(s_at + c * 32, s);
     tc_wait_load();
+    const uint32_t bits = valid[c];
 #pragma unroll
     for (int e = 0; e < 32; ++e)
-      if (!kMask || (valid[c] >> e & 1)) top = fmaxf(top, __uint_as_float(s[e]) * (kFmt == kFmtRaw ? scale : sk[c * 32 + e]));
+      if (!(bits >> e & 1)) s[e] = 0xff800000u;
+    tc_store32(s_at + c * 32, s);
   }
-  return top;
+  tc_wait_store();
 }
 
-// Weights 2^(score - m) of the tile's 128 keys, packed in pairs, times the values' scales; their sum before that;
-// returns the largest score - m.
-template <typename M, int kFmt, bool kMask>
-__device__ __forceinline__ float tile_weights(uint32_t s_at, const float *sk, const float *sv, float scale, float m, float unit,
-                                              const uint32_t (&valid)[4], uint32_t (&w)[64], float &sum) {
-  const float safe = m == -INFINITY ? 0.f : m;
-  const uint64_t minus = pair_of(-safe, -safe), factor = pair_of(scale, scale), units = pair_of(unit, unit);
-  uint64_t total[2] = {0, 0};
+// Largest score of the tile (in units of log2 e), -inf without a key.  (scale is not 0: the -inf of a masked key.)
+template <int kFmt>
+__device__ __forceinline__ float tile_max(uint32_t s_at, const float *sk, float scale) {
   float top[2] = {-INFINITY, -INFINITY};
-  uint32_t buf[2][32];                           // the next 32 columns are on their way while these are worked on
-  tc_load32(s_at, buf[0]);
-#pragma unroll
+#pragma unroll 1
   for (int c = 0; c < 4; ++c) {
-    uint32_t (&s)[32] = buf[c & 1];
+    uint32_t s[32];
+    tc_load32(s_at + c * 32, s);
     tc_wait_load(s);
-    if (c < 3) tc_load32(s_at + (c + 1) * 32, buf[(c + 1) & 1]);
+#pragma unroll
+    for (int e = 0; e < 32; e += 4) {
+      float x[4] = {__uint_as_float(s[e]), __uint_as_float(s[e + 1]), __uint_as_float(s[e + 2]), __uint_as_float(s[e + 3])};
+      if (kFmt != kFmtRaw) {
+        const float4 f = *reinterpret_cast<const float4 *>(sk + c * 32 + e);
+        const float2 lo = of_pair(mul2(pair_of(x[0], x[1]), pair_of(f.x, f.y))), hi = of_pair(mul2(pair_of(x[2], x[3]), pair_of(f.z, f.w)));
+        x[0] = lo.x;
+        x[1] = lo.y;
+        x[2] = hi.x;
+        x[3] = hi.y;
+      }
+      top[0] = max3(top[0], x[0], x[1]);
+      top[1] = max3(top[1], x[2], x[3]);
+    }
+  }
+  const float t = fmaxf(top[0], top[1]);
+  return kFmt == kFmtRaw ? t * scale : t;
+}
+
+// Weights 2^(score - origin) of the tile's 128 keys, times the values' scales, take the place of the scores (behind what
+// has been read); returns their sum before the scales.
+template <typename M, int kFmt>
+__device__ __forceinline__ float tile_weights(uint32_t s_at, const float *sk, const float *sv, float scale, float origin) {
+  const uint64_t minus = pair_of(-origin, -origin), factor = pair_of(scale, scale);
+  uint64_t total[2] = {0, 0};
+#pragma unroll 1
+  for (int c = 0; c < 4; ++c) {
+    uint32_t s[32], w[16];
+    tc_load32(s_at + c * 32, s);
+    tc_wait_load(s);
 #pragma unroll
     for (int e = 0; e < 32; e += 4) {
       float4 f, g;
@@ -223,27 +247,18 @@ __device__ __forceinline__ float tile_weights(uint32_t s_at, const float *sk, co
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         const uint64_t score = pair_of(__uint_as_float(s[e + 2 * k]), __uint_as_float(s[e + 2 * k + 1]));
-        const uint64_t by = kFmt == kFmtRaw ? factor : k == 0 ? pair_of(f.x, f.y) : pair_of(f.z, f.w);
-        float2 x = of_pair(fma2(score, by, minus));
-        if (kMask) {
-          if (!(valid[c] >> (e + 2 * k) & 1)) x.x = -INFINITY;
-          if (!(valid[c] >> (e + 2 * k + 1) & 1)) x.y = -INFINITY;
-        }
-        top[k] = max3(top[k], x.x, x.y);
+        const float2 x = of_pair(fma2(score, kFmt == kFmtRaw ? factor : k == 0 ? pair_of(f.x, f.y) : pair_of(f.z, f.w), minus));
         uint64_t p = pair_of(ex2(x.x), ex2(x.y));
         total[k] = add2(total[k], p);
-        if (kFmt != kFmtRaw) {
-          const uint64_t by_v = k == 0 ? pair_of(g.x, g.y) : pair_of(g.z, g.w);
-          p = mul2(p, mul2(by_v, units));
-        }
+        if (kFmt != kFmtRaw) p = mul2(p, k == 0 ? pair_of(g.x, g.y) : pair_of(g.z, g.w));
         const float2 y = of_pair(p);
-        w[c * 16 + e / 2 + k] = Pair<M>::pack(y.x, y.y);
+        w[e / 2 + k] = Pair<M>::pack(y.x, y.y);
       }
     }
+    tc_store16(s_at + c * 16, w);
   }
   const float2 t = of_pair(add2(total[0], total[1]));
-  sum = t.x + t.y;
-  return fmaxf(top[0], top[1]);
+  return t.x + t.y;
 }
 
 template <typename T, int kFmt, int D>
@@ -295,16 +310,23 @@ __global__ void __launch_bounds__(kPtThreads, 1) prefix_tensor_kernel(const __gr
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, *reinterpret_cast<volatile uint32_t *>(&sm.tmem), 0);
   auto wait = [&](uint64_t *bar, uint32_t parity) -> bool {
-    if (mbar_wait_bounded(bar, parity)) return true;
-    raise_status(HFK_DEV_WAIT_TIMEOUT);
-    *reinterpret_cast<volatile int *>(&sm.failed) = 1;
-    return false;
+    if (mbar_try_wait(bar, parity)) return true;
+    const uint64_t t0 = global_timer_ns();
+    while (!mbar_try_wait(bar, parity)) {
+      if (*reinterpret_cast<volatile int *>(&sm.failed)) return false;   // another one gave up: all do
+      if (global_timer_ns() - t0 > kWaitLimitNs) {
+        raise_status(HFK_DEV_WAIT_TIMEOUT);
+        *reinterpret_cast<volatile int *>(&sm.failed) = 1;
+        return false;
+      }
+    }
+    return true;
   };
 
   auto wait_warp = [&](uint64_t *bar, uint32_t parity) -> bool { return __all_sync(0xffffffffu, wait(bar, parity)); };
 
   if (warp >= 8 && warp < 12) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 120;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
     // ---------------------------------------------------------------- loads ---
     const int p = threadIdx.x - 256;
     // key p of a tile: where its row is
@@ -339,14 +361,17 @@ __global__ void __launch_bounds__(kPtThreads, 1) prefix_tensor_kernel(const __gr
     auto write_scales = [&](int i, const Key &k) {
       const int m = i % kPtMeta;
       if (kWide) {
-        sm.sk[m][p] = k.sk * factor;
+        sm.sk[m][p] = k.ok ? k.sk * factor : 1.f;   // its score is -inf, and -inf * 0 would be NaN
         sm.sv[m][p] = k.sv;
       }
       const uint32_t word = __ballot_sync(0xffffffffu, k.ok);
       if (lane == 0) sm.valid[m][p >> 5] = word;
       mbar_arrive(&sm.meta[m]);
     };
-    auto producers = [&]() { asm volatile("bar.sync 1, 128;" ::: "memory"); };
+    auto producers = [&]() {
+      __syncwarp();
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+    };
     Key key = key_of(0, page_of(0));
     int64_t next = page_of(1);
     if constexpr (!kWide) {
@@ -358,13 +383,15 @@ __global__ void __launch_bounds__(kPtThreads, 1) prefix_tensor_kernel(const __gr
         fence_async_proxy();
         mbar_arrive(&sm.full[pending]);
       };
+      bool ok = true;                            // after a wait that ran out the warps still meet at the barriers
+#pragma unroll 1
       for (int i = 0; i < n; ++i) {
         write_places(i, key);
         write_scales(i, key);
         key = key_of(i + 1, next);
         next = page_of(i + 2);
         producers();
-        bool ok = true;
+#pragma unroll 1
         for (int v = 0; v < 2 && ok; ++v) {
           const int stage = (i & 1) * 2 + v;
           const uint32_t parity = ((i >> 1) & 1) ^ 1;
@@ -391,16 +418,17 @@ __global__ void __launch_bounds__(kPtThreads, 1) prefix_tensor_kernel(const __gr
           }
           pending = stage;
         }
-        if (!ok) break;
       }
       cp_async_wait<0>();
       if (pending >= 0) announce();
     } else {
+      // A thread holds the codes of its next K and V tiles while it widens the ones before: each has a whole tile's time to
+      // arrive.  Eight lanes take four chunks of two neighbouring rows, so that what they write hits eight bank groups.
       constexpr int kChunks = D / 16;            // 16-byte chunks of codes of a row
       constexpr int kRowsPass = 128 / kChunks;
       constexpr int kPasses = kPtKeys / kRowsPass;
-      const int chunk = p % kChunks, row_in = p / kChunks;
-      // codes of the next K and the next V tile in registers: each has a whole tile's time to arrive
+      const int chunk = D == 128 ? (lane & 3) + ((lane >> 3) & 1) * 4 : lane & 3;
+      const int row_in = D == 128 ? (warp - 8) * 4 + ((lane >> 2) & 1) + (lane >> 4) * 2 : (warp - 8) * 8 + (lane >> 2);
       uint4 codes[2][kPasses];
       auto fetch = [&](int i, auto which) {
         constexpr int v = decltype(which)::value;
@@ -412,10 +440,12 @@ __global__ void __launch_bounds__(kPtThreads, 1) prefix_tensor_kernel(const __gr
           if (off >= 0) codes[v][r] = *reinterpret_cast<const uint4 *>(cache + off + chunk * 16);
         }
       };
-      auto widen = [&](int i, auto which) -> bool {
+      bool ok = true;                            // after a wait that ran out the warps still meet at the barriers
+      auto widen = [&](int i, auto which) {
         constexpr int v = decltype(which)::value;
         const int stage = (i & 1) * 2 + v;
-        if (!wait(&sm.empty[stage], ((i >> 1) & 1) ^ 1)) return false;
+        if (ok) ok = wait(&sm.empty[stage], ((i >> 1) & 1) ^ 1);
+        if (!ok) return;
         unsigned char *ring = sm.ring[stage];
 #pragma unroll
         for (int r = 0; r < kPasses; ++r) {
@@ -424,42 +454,44 @@ __global__ void __launch_bounds__(kPtThreads, 1) prefix_tensor_kernel(const __gr
 #pragma unroll
           for (int k = 0; k < 4; ++k) codes_to_pairs<kFmt>(w[k], x[2 * k], x[2 * k + 1]);
           const int row = r * kRowsPass + row_in;
-          // head_dim 128: lanes of the first half of a row write their even chunk while the others write their odd one, so
-          // that the eight lanes of a row hit eight bank groups
-          const bool swap = D == 128 && chunk >= 4;
-          const uint4 even = make_uint4(x[0], x[1], x[2], x[3]), odd = make_uint4(x[4], x[5], x[6], x[7]);
-          *reinterpret_cast<uint4 *>(ring + tile_at(row, 2 * chunk + (swap ? 1 : 0))) = swap ? odd : even;
-          *reinterpret_cast<uint4 *>(ring + tile_at(row, 2 * chunk + (swap ? 0 : 1))) = swap ? even : odd;
+          *reinterpret_cast<uint4 *>(ring + tile_at(row, 2 * chunk)) = make_uint4(x[0], x[1], x[2], x[3]);
+          *reinterpret_cast<uint4 *>(ring + tile_at(row, 2 * chunk + 1)) = make_uint4(x[4], x[5], x[6], x[7]);
         }
         fence_async_proxy();
         mbar_arrive(&sm.full[stage]);
-        return true;
       };
       constexpr std::integral_constant<int, 0> kK{};
       constexpr std::integral_constant<int, 1> kV{};
-      auto announce_tile = [&](int i, auto fetches) {
-        const Key now = key;
-        write_places(i, now);
-        producers();
-        fetches();
-        key = key_of(i + 1, next);
-        next = page_of(i + 2);
-        if (kScaleQ && i == 0 && wait(&sm.q_full, 0)) factor *= *reinterpret_cast<volatile float *>(&sm.q_back);
-        write_scales(i, now);
-      };
-      announce_tile(0, [&]() {
-        fetch(0, kK);
-        fetch(0, kV);
-      });
+      // `key` and `next` run ahead: sm.off and the scales of tile i + 2 are written when all warps are done with tile i
+      // (nobody reads those of tile i - 2 any more then).
+      write_places(0, key);
+      producers();
+      fetch(0, kK);
+      fetch(0, kV);
+      const Key then = key_of(1, next);
+      next = page_of(2);
+      if (kScaleQ && wait(&sm.q_full, 0)) factor *= *reinterpret_cast<volatile float *>(&sm.q_back);
+      write_scales(0, key);
+      write_places(1, then);
+      write_scales(1, then);
+      producers();
+      key = key_of(2, next);
+      next = page_of(3);
+#pragma unroll 1
       for (int i = 0; i < n; ++i) {
-        if (!widen(i, kK)) break;
-        if (i + 1 < n) announce_tile(i + 1, [&]() { fetch(i + 1, kK); });
-        if (!widen(i, kV)) break;
+        widen(i, kK);
+        if (i + 1 < n) fetch(i + 1, kK);
+        widen(i, kV);
         if (i + 1 < n) fetch(i + 1, kV);
+        producers();
+        write_places(i + 2, key);
+        write_scales(i + 2, key);
+        key = key_of(i + 3, next);
+        next = page_of(i + 4);
       }
     }
   } else if (warp >= 12) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
     // ------------------------------------------------------------- products ---
     if (warp == 12 && n > 0) {
       const uint32_t leader = elect_leader();
@@ -506,13 +538,17 @@ __global__ void __launch_bounds__(kPtThreads, 1) prefix_tensor_kernel(const __gr
     }
     __syncwarp();
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 144;");
     // -------------------------------------------------------------- softmax ---
     if (warp / 4 < tiles) {
     const int j = warp / 4;
     const uint32_t lanes = (uint32_t)(warp % 4) << 21;   // first TMEM lane of this warp, in bits 16 and up
     const uint32_t s_at = tmem + j * 128 + lanes, o_at = tmem + 256 + j * D + lanes;
-    float m = -INFINITY, l = 0.f, ref = 0.f;
+    // Weights are taken at the origin m + log2(ref), ref a quarter or more of the largest scale of a value so far: the
+    // products with the scales then stay within fp16, whatever the scales are.  (l is at the same origin.)
+    constexpr float kLeastRef = 7.9e-31f;        // 2^-100: its reciprocal times 2^8 and many keys is finite
+    float m = -INFINITY, l = 0.f, ref = kLeastRef, log_ref = kWide ? -100.f : 0.f;
+    const float scale = a.scale_log2 == 0.f ? kLeastScale : a.scale_log2;   // 0 times the -inf of a masked key is NaN
     bool ok = true;
     {                                            // this warp's 32 rows of queries, zero behind the last one
       constexpr int kChunks = D / 8, kRowsPass = 32 / kChunks;
@@ -557,44 +593,28 @@ __global__ void __launch_bounds__(kPtThreads, 1) prefix_tensor_kernel(const __gr
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tc_fence_after();
-      const uint32_t valid[4] = {sm.valid[mt][0], sm.valid[mt][1], sm.valid[mt][2], sm.valid[mt][3]};
-      const bool all = (valid[0] & valid[1] & valid[2] & valid[3]) == 0xffffffffu;
-      if (__any_sync(0xffffffffu, m == -INFINITY)) {
-        // rows without a maximum yet (the first tile; tiles whose pages are bad)
-        const float top = all ? tile_max<kFmt, false>(s_at, sm.sk[mt], a.scale_log2, valid) : tile_max<kFmt, true>(s_at, sm.sk[mt], a.scale_log2, valid);
-        if (m == -INFINITY) m = top;
-        __syncwarp();
+      if ((sm.valid[mt][0] & sm.valid[mt][1] & sm.valid[mt][2] & sm.valid[mt][3]) != 0xffffffffu) mask_scores(s_at, sm.valid[mt]);
+      const float top = tile_max<kFmt>(s_at, sm.sk[mt], scale);
+      // the row's maximum in use, and whether o and l have to follow
+      float factor = 1.f;
+      if (top > m + 8.f) {
+        factor = ex2(m - top);
+        m = top;
       }
-      float unit = 1.f;
       if (kWide) {
         float big = max_nan(max_nan(sm.sv[mt][lane], sm.sv[mt][lane + 32]), max_nan(sm.sv[mt][lane + 64], sm.sv[mt][lane + 96]));
 #pragma unroll
         for (int d = 16; d > 0; d >>= 1) big = max_nan(big, __shfl_xor_sync(0xffffffffu, big, d));
         if (!(big <= 4.f * ref)) {               // also a NaN; the same for every row
-          if (i > 0) rescale<D>(o_at, ref / big);
+          factor *= ref / big;
           ref = big;
+          log_ref = log2f(ref);
         }
         __syncwarp();
-        unit = ref == 0.f ? 0.f : 1.f / ref;
       }
-      uint32_t w[64];
-      float sum;
-      float top = all ? tile_weights<M, kFmt, false>(s_at, sm.sk[mt], sm.sv[mt], a.scale_log2, m, unit, valid, w, sum)
-                      : tile_weights<M, kFmt, true>(s_at, sm.sk[mt], sm.sv[mt], a.scale_log2, m, unit, valid, w, sum);
-      if (__any_sync(0xffffffffu, top > 8.f)) {
-        // a maximum rose too far: o and l follow, and the weights are taken again (the scores are still there)
-        const float rise = top > 8.f ? top : 0.f, factor = ex2(-rise);
-        m = m == -INFINITY ? m : m + rise;
-        l *= factor;
-        if (i > 0) rescale<D>(o_at, factor);
-        if (all)
-          tile_weights<M, kFmt, false>(s_at, sm.sk[mt], sm.sv[mt], a.scale_log2, m, unit, valid, w, sum);
-        else
-          tile_weights<M, kFmt, true>(s_at, sm.sk[mt], sm.sv[mt], a.scale_log2, m, unit, valid, w, sum);
-      }
-      l += sum;
-      tc_store32(s_at, *reinterpret_cast<uint32_t (*)[32]>(&w[0]));      // the weights take the scores' place
-      tc_store32(s_at + 32, *reinterpret_cast<uint32_t (*)[32]>(&w[32]));
+      if (i > 0 && __any_sync(0xffffffffu, factor != 1.f)) rescale<D>(o_at, factor);
+      l *= factor;
+      l += tile_weights<M, kFmt>(s_at, sm.sk[mt], sm.sv[mt], scale, (m == -INFINITY ? 0.f : m) + log_ref);
       tc_wait_store();
       tc_fence_before();
       mbar_arrive(&sm.p_full[j]);
@@ -609,8 +629,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) prefix_tensor_kernel(const __gr
       const int at = threadIdx.x, row = at;
       unsigned char *mine = sm.q[0] + at * (D * 4 + 16);
       const int64_t part = (int64_t)split * a.kv_heads * args.rows + (int64_t)h * args.rows + row0 + row;
-      if (row < rows) args.part_ml[part] = make_float2(m, l);
-      const float unit = kWide ? ref : 1.f;
+      if (row < rows) args.part_ml[part] = make_float2(m == -INFINITY ? m : m + log_ref, l);
       uint32_t buf[2][32];
       tc_load32(o_at, buf[0]);
 #pragma unroll
@@ -621,8 +640,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) prefix_tensor_kernel(const __gr
 #pragma unroll
         for (int e = 0; e < 8; ++e)
           *reinterpret_cast<float4 *>(mine + c * 128 + e * 16) =
-              make_float4(__uint_as_float(s[4 * e]) * unit, __uint_as_float(s[4 * e + 1]) * unit, __uint_as_float(s[4 * e + 2]) * unit,
-                          __uint_as_float(s[4 * e + 3]) * unit);
+              make_float4(__uint_as_float(s[4 * e]), __uint_as_float(s[4 * e + 1]), __uint_as_float(s[4 * e + 2]), __uint_as_float(s[4 * e + 3]));
       }
       fence_async_proxy();
       if (row < rows) {

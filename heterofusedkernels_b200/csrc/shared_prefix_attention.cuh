@@ -76,10 +76,7 @@ __device__ __forceinline__ void mma16816<__half>(float (&c)[4], const uint32_t (
 template <int kFmt>
 __device__ __forceinline__ void codes_to_pairs(uint32_t w, uint32_t &lo, uint32_t &hi) {
   if constexpr (kFmt == kFmtE4m3) {
-    const __half2_raw a = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w & 0xffffu), __NV_E4M3);
-    const __half2_raw b = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w >> 16), __NV_E4M3);
-    lo = a.x | ((uint32_t)a.y << 16);
-    hi = b.x | ((uint32_t)b.y << 16);
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}" : "=r"(lo), "=r"(hi) : "r"(w));
   } else {
     const uint32_t u = w ^ 0x80808080u;
     const uint32_t l = __byte_perm(u, 0x64646464u, 0x4140), h = __byte_perm(u, 0x64646464u, 0x4342);
