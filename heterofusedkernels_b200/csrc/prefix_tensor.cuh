@@ -3,7 +3,7 @@
 //
 // A CTA takes up to 256 rows of one K/V head (two tiles of 128, one TMEM lane a row) against a run of key tiles
 // of 128, and leaves a partial result (m, l, o).  Four groups of four warps:
-//   0-3, 4-7  softmax of tile 0 and of tile 1: one thread a row, so neither the maximum nor the sum needs a shuffle
+//   0-3, 4-7  softmax of tile 0 and of tile 1, 32 rows a warp
 //   8-11      bring K and V tiles into shared memory (asynchronous copies; 8-bit codes are widened on the way)
 //   12        issues the matrix products (13-15 only bring their registers)
 // A thread starts with 128 registers; the warps that widen codes hold two tiles of them and would spill (to L2: shared
@@ -116,11 +116,17 @@ __device__ __forceinline__ void tc_store32(uint32_t addr, const uint32_t (&r)[32
       "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]),
       "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(addr));
 }
-__device__ __forceinline__ void tc_store16(uint32_t addr, const uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]),
-      "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
-      "r"(addr));
+// 32 columns of 16 lanes in the layout of a matrix product's result: register 4n + 2r + x of thread 4g + t is column
+// 8n + 2t + x of lane g + 8r; and the store of pairs packed to 16 columns: register 2n + r is column 4n + t of lane g + 8r.
+__device__ __forceinline__ void tc_load_block(uint32_t addr, uint32_t *r) {
+  asm volatile("tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+                 "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+               : "r"(addr));
+}
+__device__ __forceinline__ void tc_store_pairs(uint32_t addr, const uint32_t *r) {
+  asm volatile("tcgen05.st.sync.aligned.16x128b.x4.b32 [%8], {%0,%1,%2,%3,%4,%5,%6,%7};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]),
+               "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(addr));
 }
 __device__ __forceinline__ void tc_wait_load() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 // The same for one tc_load32, whose registers nothing may read earlier; other memory is free to move across.
@@ -164,7 +170,6 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
-__device__ __forceinline__ float max3(float a, float b, float c) { return fmaxf(fmaxf(a, b), c); }
 
 // o of this warp's rows times a factor of each row
 template <int D>
@@ -198,67 +203,103 @@ __device__ __forceinline__ void mask_scores(uint32_t s_at, const uint32_t *valid
   tc_wait_store();
 }
 
-// Largest score of the tile (in units of log2 e), -inf without a key.  (scale is not 0: the -inf of a masked key.)
+// A warp's 32 rows of scores, 32 columns at a time: thread 4g + t has columns 8n + 2t, 8n + 2t + 1 (n < 4) of the four rows
+// g + 8k, s[16 (k / 2) + 4n + 2 (k % 2)] and the next.  So a thread needs a quarter of the scales and uses each for four
+// rows; with a row a thread, their loads from shared memory (512 bytes to the registers each, whatever they read) took
+// longer than the exponentials.
+constexpr uint32_t kUpperLanes = 16u << 16;
+__device__ __forceinline__ void load_scores(uint32_t at, uint32_t (&s)[32]) {
+  tc_load_block(at, s);
+  tc_load_block(at + kUpperLanes, s + 16);
+}
+
+// Largest score of each of the four rows over the tile (in units of log2 e), -inf without a key.  (scale is not 0.)
 template <int kFmt>
-__device__ __forceinline__ float tile_max(uint32_t s_at, const float *sk, float scale) {
-  float top[2] = {-INFINITY, -INFINITY};
-#pragma unroll 1
-  for (int c = 0; c < 4; ++c) {
-    uint32_t s[32];
-    tc_load32(s_at + c * 32, s);
-    tc_wait_load(s);
+__device__ __forceinline__ void tile_max(uint32_t s_at, const float *sk, float scale, float (&top)[4]) {
+  const int t2 = (threadIdx.x & 3) * 2;
+  top[0] = top[1] = top[2] = top[3] = -INFINITY;
+  uint32_t buf[2][32];                           // the next 32 columns are on their way while these are looked at
+  auto look = [&](int c, const uint32_t (&s)[32]) {
 #pragma unroll
-    for (int e = 0; e < 32; e += 4) {
-      float x[4] = {__uint_as_float(s[e]), __uint_as_float(s[e + 1]), __uint_as_float(s[e + 2]), __uint_as_float(s[e + 3])};
-      if (kFmt != kFmtRaw) {
-        const float4 f = *reinterpret_cast<const float4 *>(sk + c * 32 + e);
-        const float2 lo = of_pair(mul2(pair_of(x[0], x[1]), pair_of(f.x, f.y))), hi = of_pair(mul2(pair_of(x[2], x[3]), pair_of(f.z, f.w)));
-        x[0] = lo.x;
-        x[1] = lo.y;
-        x[2] = hi.x;
-        x[3] = hi.y;
+    for (int n = 0; n < 4; ++n) {
+      float2 f = make_float2(1.f, 1.f);
+      if (kFmt != kFmtRaw) f = *reinterpret_cast<const float2 *>(sk + c * 32 + n * 8 + t2);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int i = 16 * (k >> 1) + 4 * n + 2 * (k & 1);
+        float2 x = make_float2(__uint_as_float(s[i]), __uint_as_float(s[i + 1]));
+        if (kFmt != kFmtRaw) x = of_pair(mul2(pair_of(x.x, x.y), pair_of(f.x, f.y)));
+        top[k] = fmaxf(top[k], fmaxf(x.x, x.y));
       }
-      top[0] = max3(top[0], x[0], x[1]);
-      top[1] = max3(top[1], x[2], x[3]);
     }
+  };
+  load_scores(s_at, buf[0]);
+#pragma unroll 1
+  for (int c = 0; c < 4; c += 2) {
+    tc_wait_load(buf[0]);
+    load_scores(s_at + (c + 1) * 32, buf[1]);
+    look(c, buf[0]);
+    tc_wait_load(buf[1]);
+    if (c == 0) load_scores(s_at + 64, buf[0]);
+    look(c + 1, buf[1]);
   }
-  const float t = fmaxf(top[0], top[1]);
-  return kFmt == kFmtRaw ? t * scale : t;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], 1));
+    top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], 2));
+    if (kFmt == kFmtRaw) top[k] *= scale;
+  }
 }
 
 // Weights 2^(score - origin) of the tile's 128 keys, times the values' scales, take the place of the scores (behind what
-// has been read); returns their sum before the scales.
+// has been read); adds this thread's columns of them, before the scales, to l.
 template <typename M, int kFmt>
-__device__ __forceinline__ float tile_weights(uint32_t s_at, const float *sk, const float *sv, float scale, float origin) {
-  const uint64_t minus = pair_of(-origin, -origin), factor = pair_of(scale, scale);
-  uint64_t total[2] = {0, 0};
-#pragma unroll 1
-  for (int c = 0; c < 4; ++c) {
-    uint32_t s[32], w[16];
-    tc_load32(s_at + c * 32, s);
-    tc_wait_load(s);
+__device__ __forceinline__ void tile_weights(uint32_t s_at, const float *sk, const float *sv, float scale, const float (&origin)[4], float (&l)[4]) {
+  const int t2 = (threadIdx.x & 3) * 2;
+  const uint64_t factor = pair_of(scale, scale);
+  uint64_t total[4] = {0, 0, 0, 0}, minus[4];
 #pragma unroll
-    for (int e = 0; e < 32; e += 4) {
-      float4 f, g;
+  for (int k = 0; k < 4; ++k) minus[k] = pair_of(-origin[k], -origin[k]);
+  uint32_t buf[2][32];
+  auto weigh = [&](int c, const uint32_t (&s)[32]) {
+    uint32_t w[16];
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      float2 f, g;
       if (kFmt != kFmtRaw) {
-        f = *reinterpret_cast<const float4 *>(sk + c * 32 + e);
-        g = *reinterpret_cast<const float4 *>(sv + c * 32 + e);
+        f = *reinterpret_cast<const float2 *>(sk + c * 32 + n * 8 + t2);
+        g = *reinterpret_cast<const float2 *>(sv + c * 32 + n * 8 + t2);
       }
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const uint64_t score = pair_of(__uint_as_float(s[e + 2 * k]), __uint_as_float(s[e + 2 * k + 1]));
-        const float2 x = of_pair(fma2(score, kFmt == kFmtRaw ? factor : k == 0 ? pair_of(f.x, f.y) : pair_of(f.z, f.w), minus));
+      for (int k = 0; k < 4; ++k) {
+        const int i = 16 * (k >> 1) + 4 * n + 2 * (k & 1);
+        const uint64_t score = pair_of(__uint_as_float(s[i]), __uint_as_float(s[i + 1]));
+        const float2 x = of_pair(fma2(score, kFmt == kFmtRaw ? factor : pair_of(f.x, f.y), minus[k]));
         uint64_t p = pair_of(ex2(x.x), ex2(x.y));
         total[k] = add2(total[k], p);
-        if (kFmt != kFmtRaw) p = mul2(p, k == 0 ? pair_of(g.x, g.y) : pair_of(g.z, g.w));
+        if (kFmt != kFmtRaw) p = mul2(p, pair_of(g.x, g.y));
         const float2 y = of_pair(p);
-        w[e / 2 + k] = Pair<M>::pack(y.x, y.y);
+        w[8 * (k >> 1) + 2 * n + (k & 1)] = Pair<M>::pack(y.x, y.y);
       }
     }
-    tc_store16(s_at + c * 16, w);
+    tc_store_pairs(s_at + c * 16, w);
+    tc_store_pairs(s_at + kUpperLanes + c * 16, w + 8);
+  };
+  load_scores(s_at, buf[0]);
+#pragma unroll 1
+  for (int c = 0; c < 4; c += 2) {
+    tc_wait_load(buf[0]);
+    load_scores(s_at + (c + 1) * 32, buf[1]);    // columns that the weights of chunk c do not reach
+    weigh(c, buf[0]);
+    tc_wait_load(buf[1]);
+    if (c == 0) load_scores(s_at + 64, buf[0]);
+    weigh(c + 1, buf[1]);
   }
-  const float2 t = of_pair(add2(total[0], total[1]));
-  return t.x + t.y;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const float2 x = of_pair(total[k]);
+    l[k] += x.x + x.y;
+  }
 }
 
 template <typename T, int kFmt, int D>
@@ -547,7 +588,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) prefix_tensor_kernel(const __gr
     // Weights are taken at the origin m + log2(ref), ref a quarter or more of the largest scale of a value so far: the
     // products with the scales then stay within fp16, whatever the scales are.  (l is at the same origin.)
     constexpr float kLeastRef = 7.9e-31f;        // 2^-100: its reciprocal times 2^8 and many keys is finite
-    float m = -INFINITY, l = 0.f, ref = kLeastRef, log_ref = kWide ? -100.f : 0.f;
+    float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, l[4] = {0.f, 0.f, 0.f, 0.f}, ref = kLeastRef, log_ref = kWide ? -100.f : 0.f;
     const float scale = a.scale_log2 == 0.f ? kLeastScale : a.scale_log2;   // 0 times the -inf of a masked key is NaN
     bool ok = true;
     {                                            // this warp's 32 rows of queries, zero behind the last one
@@ -594,27 +635,43 @@ __global__ void __launch_bounds__(kPtThreads, 1) prefix_tensor_kernel(const __gr
       if (!ok) break;
       tc_fence_after();
       if ((sm.valid[mt][0] & sm.valid[mt][1] & sm.valid[mt][2] & sm.valid[mt][3]) != 0xffffffffu) mask_scores(s_at, sm.valid[mt]);
-      const float top = tile_max<kFmt>(s_at, sm.sk[mt], scale);
-      // the row's maximum in use, and whether o and l have to follow
-      float factor = 1.f;
-      if (top > m + 8.f) {
-        factor = ex2(m - top);
-        m = top;
-      }
+      float top[4], factor[4], origin[4];
+      tile_max<kFmt>(s_at, sm.sk[mt], scale, top);
+      float turn = 1.f;                          // of every row
       if (kWide) {
         float big = max_nan(max_nan(sm.sv[mt][lane], sm.sv[mt][lane + 32]), max_nan(sm.sv[mt][lane + 64], sm.sv[mt][lane + 96]));
 #pragma unroll
         for (int d = 16; d > 0; d >>= 1) big = max_nan(big, __shfl_xor_sync(0xffffffffu, big, d));
-        if (!(big <= 4.f * ref)) {               // also a NaN; the same for every row
-          factor *= ref / big;
+        if (!(big <= 4.f * ref)) {               // also a NaN
+          turn = ref / big;
           ref = big;
           log_ref = log2f(ref);
         }
         __syncwarp();
       }
-      if (i > 0 && __any_sync(0xffffffffu, factor != 1.f)) rescale<D>(o_at, factor);
-      l *= factor;
-      l += tile_weights<M, kFmt>(s_at, sm.sk[mt], sm.sv[mt], scale, (m == -INFINITY ? 0.f : m) + log_ref);
+      // the rows' maxima in use, and whether o and l have to follow
+      bool follow = false;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        factor[k] = turn;
+        if (top[k] > m[k] + 8.f) {
+          factor[k] *= ex2(m[k] - top[k]);
+          m[k] = top[k];
+        }
+        follow = follow || factor[k] != 1.f;
+        l[k] *= factor[k];
+        origin[k] = (m[k] == -INFINITY ? 0.f : m[k]) + log_ref;
+      }
+      if (i > 0 && __any_sync(0xffffffffu, follow)) {
+        float mine = 1.f;                        // factor of row `lane`: thread 4 (lane % 8) has it, number lane / 8
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float f = __shfl_sync(0xffffffffu, factor[k], (lane & 7) * 4);
+          if (lane >> 3 == k) mine = f;
+        }
+        rescale<D>(o_at, mine);
+      }
+      tile_weights<M, kFmt>(s_at, sm.sk[mt], sm.sv[mt], scale, origin, l);
       tc_wait_store();
       tc_fence_before();
       mbar_arrive(&sm.p_full[j]);
@@ -629,7 +686,13 @@ __global__ void __launch_bounds__(kPtThreads, 1) prefix_tensor_kernel(const __gr
       const int at = threadIdx.x, row = at;
       unsigned char *mine = sm.q[0] + at * (D * 4 + 16);
       const int64_t part = (int64_t)split * a.kv_heads * args.rows + (int64_t)h * args.rows + row0 + row;
-      if (row < rows) args.part_ml[part] = make_float2(m == -INFINITY ? m : m + log_ref, l);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        l[k] += __shfl_xor_sync(0xffffffffu, l[k], 1);
+        l[k] += __shfl_xor_sync(0xffffffffu, l[k], 2);
+        const int r = warp * 32 + 8 * k + (lane >> 2);
+        if ((lane & 3) == 0 && r < rows) args.part_ml[part - row + r] = make_float2(m[k] == -INFINITY ? m[k] : m[k] + log_ref, l[k]);
+      }
       uint32_t buf[2][32];
       tc_load32(o_at, buf[0]);
 #pragma unroll
