@@ -273,8 +273,8 @@ static int plan_attention(const hfk_prefix_attention_desc *d, int ctas, AttnPlan
   const size_t parts = p->ctas > 0 ? (size_t)p->warps + (size_t)line.items(seqs) : 0;
   const auto round = [](size_t n) { return (n + 255) & ~(size_t)255; };
   p->cu_bytes = round((size_t)(seqs + 1) * sizeof(int));
-  p->ml_bytes = round(parts * 16 * sizeof(float2));
-  p->o_bytes = round(parts * 16 * d->head_dim * sizeof(float));
+  p->ml_bytes = round(parts * kItemRows * sizeof(float2));
+  p->o_bytes = round(parts * kItemRows * d->head_dim * sizeof(float));
   p->prefix_ml_bytes = round((size_t)p->splits * d->kv_heads * rows * sizeof(float2));
   p->prefix_o_bytes = round((size_t)p->splits * d->kv_heads * rows * d->head_dim * sizeof(float));
   return HFK_OK;
@@ -333,7 +333,10 @@ static cudaError_t launch_attention(const AttnArgs &a, const AttnPlan &p, unsign
     if ((e = allow_smem(k, smem)) != cudaSuccess) return e;
     if ((e = launch_behind(k, p.tensor, p.ctas, kLineWarps * 32, smem, s, join.a)) != cudaSuccess) return e;
   }
-  return launch_behind(shared_prefix_join_kernel<T, D>, true, a.seqs * a.kv_heads * a.group, kJoinWarps * 32, 0, s, join);
+  const int rows = a.seqs * a.kv_heads * a.group, resident = sm_count() * kJoinWarpsPerSm;
+  if (rows * 4 <= resident) return launch_behind(shared_prefix_join_kernel<T, D, 4>, true, rows, 128, 0, s, join);
+  if (rows * 2 <= resident) return launch_behind(shared_prefix_join_kernel<T, D, 2>, true, rows, 64, 0, s, join);
+  return launch_behind(shared_prefix_join_kernel<T, D, 1>, true, rows, 32, 0, s, join);
 }
 template <typename T, int kFmt>
 static cudaError_t launch_attention(const AttnArgs &a, int head_dim, const AttnPlan &p, unsigned char *w, cudaStream_t s) {

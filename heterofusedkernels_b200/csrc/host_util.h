@@ -54,6 +54,8 @@ constexpr int kMigrateCtasPerSm = 2;
 constexpr int kGatherDequantCtasPerSm = 4;
 // Attention: CTAs of eight warps per SM (their rings take its shared memory).
 constexpr int kAttnCtasPerSm = 1;
+// Warps of the join that an SM holds at once (about 72 registers a thread).
+constexpr int kJoinWarpsPerSm = 28;
 // Rows of queries (sequences x query heads of a K/V head) above which the prefix goes to the tensor-core kernel, and
 // what a CTA of it costs beyond its key tiles, in tiles.
 constexpr int kPrefixTensorMinRows = 32;

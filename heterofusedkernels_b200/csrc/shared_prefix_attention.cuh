@@ -45,8 +45,8 @@ struct AttnArgs {
   float scale_log2;               // scale * log2 e
   // partial results (workspace)
   int *cu;                        // [seqs + 1] first tile of each sequence, per (K/V head, row tile)
-  float2 *part_ml;                // [parts][16]  (m, l)
-  float *part_o;                  // [parts][16][head_dim]
+  float2 *part_ml;                // [parts][kItemRows]  (m, l)
+  float *part_o;                  // [parts][kItemRows][head_dim]
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -69,6 +69,13 @@ __device__ __forceinline__ void mma16816<__half>(float (&c)[4], const uint32_t (
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// Transpose of an 8 x 8 matrix of 16-bit numbers; thread 4g + t holds row g, columns 2t and 2t + 1.
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
 }
 
 // ---- codes to fp16: the four codes of a word as two pairs, exact ------------------------------------------
@@ -106,22 +113,23 @@ __device__ __forceinline__ uint32_t pair_to_half(uint32_t w, float factor) {
 }
 
 // ---- how the work is laid out -------------------------------------------------------------------------------
-// An ITEM is 16 rows of queries against one range of keys: for the prefix a (K/V head, 16 of the seqs * group
-// rows), for a sequence's own keys a (sequence, K/V head, 16 of the group's rows).  Keys go by tiles of 16, of an 8-bit cache by tiles of 32: 8 KB at head_dim 128.
+// An ITEM is 8 rows of queries against one range of keys: for the prefix a (K/V head, 8 of the seqs * group
+// rows), for a sequence's own keys a (sequence, K/V head, 8 of the group's rows).  Keys go by tiles of 16, of an 8-bit cache by tiles of 32: 8 KB at head_dim 128.
 // All tiles of all items form one line, items of the prefix first, that is cut into equal pieces, one to a
 // WARP: none has more than one tile more than another, whatever the lengths are (they are known on the
 // device only).  A piece may end one item and begin the next.  The part of warp w of item i has the number
 // w + i: along the line either grows, so no two parts share a number and there are at most warps + items.
+constexpr int kItemRows = 8;
 __host__ __device__ constexpr int tile_keys(int fmt) { return fmt == HFK_KV_RAW ? 16 : 32; }
 
 struct AttnLine {
-  int row_tiles, own_tiles;       // tiles of 16 rows: of the prefix's rows, of a group
+  int row_tiles, own_tiles;       // tiles of kItemRows rows: of the prefix's rows, of a group
   int prefix_items, prefix_tiles; // tiles of keys of an item
   int per_seq;                    // items of a sequence
   int tile;                       // keys of a tile
   __host__ __device__ AttnLine(int seqs, int kv_heads, int group, int prefix_len, int tile) : tile(tile) {
-    row_tiles = (seqs * group + 15) / 16;
-    own_tiles = (group + 15) / 16;
+    row_tiles = (seqs * group + kItemRows - 1) / kItemRows;
+    own_tiles = (group + kItemRows - 1) / kItemRows;
     prefix_tiles = (prefix_len + tile - 1) / tile;
     prefix_items = prefix_tiles > 0 ? row_tiles * kv_heads : 0;
     per_seq = kv_heads * own_tiles;
@@ -201,8 +209,8 @@ __device__ __forceinline__ LineItem line_item(const AttnArgs &a, const AttnLine 
     x.tile = at - x.ordinal * line.prefix_tiles;
     x.tiles = line.prefix_tiles;
     x.h = x.ordinal / line.row_tiles;
-    x.row0 = (x.ordinal - x.h * line.row_tiles) * 16;
-    x.rows = min(16, a.seqs * a.group - x.row0);
+    x.row0 = (x.ordinal - x.h * line.row_tiles) * kItemRows;
+    x.rows = min(kItemRows, a.seqs * a.group - x.row0);
     x.seq = 0;
     x.len = a.prefix_len;
     x.table = a.prefix_table;
@@ -221,8 +229,8 @@ __device__ __forceinline__ LineItem line_item(const AttnArgs &a, const AttnLine 
     x.tile = v - hg * x.tiles;
     x.ordinal = line.prefix_items + lo * line.per_seq + hg;
     x.h = hg / line.own_tiles;
-    x.row0 = (hg - x.h * line.own_tiles) * 16;
-    x.rows = min(16, a.group - x.row0);
+    x.row0 = (hg - x.h * line.own_tiles) * kItemRows;
+    x.rows = min(kItemRows, a.group - x.row0);
     x.len = (int)own_length(a, lo, false);
     x.table = a.tables;
     x.table_at = (int64_t)lo * a.table_stride;
@@ -263,7 +271,10 @@ struct alignas(128) LineRing {
 // with asynchronous copies that run ahead over the ends of items; nothing in the CTA waits for anything else.
 // In the ring the 16-byte chunks of a row are XORed with bits of the row's number, so that the fragments' reads
 // (K: four neighbouring chunks of two rows; V: two neighbouring chunks of four rows, two apart) hit all banks.
-// The order of the products over head_dim, and of the columns of o, is free, so a lane takes 16 contiguous bytes of
+// Both products are taken transposed, scores^T = K Q^T and o^T = V^T weights^T: keys and head_dim fill the 16 rows of the
+// instruction and the queries, of which a group has few, its 8 columns.  (With the queries as the 16 rows, half or more of
+// the instructions, exponentials and accumulators were of rows that do not exist.)
+// The order of the products over head_dim, and of the rows of o^T, is free, so a lane takes 16 contiguous bytes of
 // a row where the operand layout would have it take two, and V needs no transposition: a lane that holds the same
 // columns of four rows packs its operands with byte permutations.
 //
@@ -280,7 +291,7 @@ __global__ void __launch_bounds__(kLineWarps * 32, 1) shared_prefix_attention_ke
   constexpr int kVe = kVb / kElt;                         // values of a V chunk
   constexpr int kE = 16 / kElt;                           // values of a K chunk
   constexpr int kCpr = kRow / 16, kRowsPass = 32 / kCpr;  // copies: chunks of a row, rows of a warp's pass
-  constexpr int kN = kKeys / 8;                           // blocks of 8 keys
+  constexpr int kM = kKeys / 16;                          // blocks of 16 keys
   constexpr bool kCodes = kFmt != kFmtRaw;
   extern __shared__ __align__(128) unsigned char smem_raw[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -317,6 +328,11 @@ __global__ void __launch_bounds__(kLineWarps * 32, 1) shared_prefix_attention_ke
   };
   int load_stage = 0, changes = 0;
   const int chunk = lane % kCpr, sub = lane / kCpr;
+  const int step = kRowsPass * a.kv_heads * kRow;             // bytes from pass to pass of a group in one page
+  // where row `sub` of a pass goes in the ring: K, V; and what the number of the pass's first row changes in V's
+  const uint32_t k_to = sub * kRow + (kCpr >= 8 ? chunk ^ ((sub & 1) << 2) : chunk) * 16;
+  const uint32_t v_to = sub * kRow + (kCpr >= 8 ? chunk ^ (((sub >> 1) & 3) << 1) : chunk ^ ((sub >> 1) & 3)) * 16;
+  auto v_flip = [](int r) -> uint32_t { return kCpr >= 8 ? (uint32_t)((r >> 1) & 3) << 5 : (uint32_t)((r >> 1) & 3) << 4; };
   auto load_group = [&](int group, int part) -> uint32_t {     // group `part` of the tile; returns which keys count
     const int key0 = group * 16;
     const uint32_t kb = smem_addr(ring.k[load_stage]) + part * 16 * kRow, vb = smem_addr(ring.v[load_stage]) + part * 16 * kRow;
@@ -332,24 +348,32 @@ __global__ void __launch_bounds__(kLineWarps * 32, 1) shared_prefix_attention_ke
       const uint32_t b = a.block.div((uint32_t)key0);
       const uint32_t row = ((uint32_t)key0 - b * a.block.d) * a.kv_heads + in.h;
       const int64_t from = page + (int64_t)(row + sub * a.kv_heads) * kRow + chunk * 16;
-      const int step = kRowsPass * a.kv_heads * kRow;       // bytes from pass to pass, less than a page
       const unsigned char *kp = a.k_cache + from, *vp = a.v_cache + from;
+      const unsigned char *sp = (lane < 16 ? a.k_cache : a.v_cache) + page + a.scales_at + (int64_t)(row + (lane & 15) * a.kv_heads) * 4;
+      if (left >= 16) {                                     // nearly always: no lane is left out
+        if (kCodes) cp_async4(sb, sp, true);
+#pragma unroll
+        for (int r = 0; r < 16; r += kRowsPass) {
+          cp_async16(kb + k_to + r * kRow, kp, true);
+          cp_async16(vb + (v_to ^ v_flip(r)) + r * kRow, vp, true);
+          kp += step;
+          vp += step;
+        }
+        return 0xffffu;
+      }
       if (kCodes) {
         const bool mine = (lane & 15) < left;
-        cp_async4(sb, (lane < 16 ? a.k_cache : a.v_cache) + page + a.scales_at + (mine ? (int64_t)(row + (lane & 15) * a.kv_heads) * 4 : 0), mine);
+        cp_async4(sb, mine ? sp : a.k_cache, mine);
       }
-#pragma unroll
+#pragma unroll 1
       for (int r = 0; r < 16; r += kRowsPass) {
-        const int at = r + sub;
-        const bool mine = at < left;
-        const int kc = kCpr >= 8 ? chunk ^ ((at & 1) << 2) : chunk;
-        const int vc = kCpr >= 8 ? chunk ^ (((at >> 1) & 3) << 1) : chunk ^ ((at >> 1) & 3);
-        cp_async16(kb + at * kRow + kc * 16, mine ? kp : a.k_cache, mine);
-        cp_async16(vb + at * kRow + vc * 16, mine ? vp : a.v_cache, mine);
+        const bool mine = r + sub < left;
+        cp_async16(kb + k_to + r * kRow, mine ? kp : a.k_cache, mine);
+        cp_async16(vb + (v_to ^ v_flip(r)) + r * kRow, mine ? vp : a.v_cache, mine);
         kp += step;
         vp += step;
       }
-      return left >= 16 ? 0xffffu : (1u << max(left, 0)) - 1u;
+      return (1u << max(left, 0)) - 1u;
     }
     const int key = key0 + (lane & 15);
     const bool inside = key < in.len;
@@ -359,15 +383,12 @@ __global__ void __launch_bounds__(kLineWarps * 32, 1) shared_prefix_attention_ke
     const int64_t page = ok ? id * a.block_stride : 0;
     const int64_t off = ok ? page + (int64_t)row * kRow : -1;
     if (kCodes) cp_async4(sb, (lane < 16 ? a.k_cache : a.v_cache) + page + a.scales_at + (ok ? (int64_t)row * 4 : 0), ok);
-#pragma unroll
+#pragma unroll 1
     for (int r = 0; r < 16; r += kRowsPass) {
-      const int at = r + sub;
-      const int64_t o = __shfl_sync(0xffffffffu, off, at);
+      const int64_t o = __shfl_sync(0xffffffffu, off, r + sub);
       const int64_t from = (o < 0 ? 0 : o) + chunk * 16;
-      const int kc = kCpr >= 8 ? chunk ^ ((at & 1) << 2) : chunk;
-      const int vc = kCpr >= 8 ? chunk ^ (((at >> 1) & 3) << 1) : chunk ^ ((at >> 1) & 3);
-      cp_async16(kb + at * kRow + kc * 16, a.k_cache + from, o >= 0);
-      cp_async16(vb + at * kRow + vc * 16, a.v_cache + from, o >= 0);
+      cp_async16(kb + k_to + r * kRow, a.k_cache + from, o >= 0);
+      cp_async16(vb + (v_to ^ v_flip(r)) + r * kRow, a.v_cache + from, o >= 0);
     }
     return __ballot_sync(0xffffffffu, ok) & 0xffffu;
   };
@@ -399,33 +420,31 @@ __global__ void __launch_bounds__(kLineWarps * 32, 1) shared_prefix_attention_ke
     ++loads;
     cp_async_commit();        // one group a tile, empty before the first and behind the last one
   };
-  // queries: rows g and g + 8, the chunks this lane also takes of K
-  uint32_t qf[D / 16][4];
+  // queries: row g, the chunks this lane also takes of K
+  uint32_t qf[D / 16][2];
   auto load_queries = [&](const LineItem &x) {
+    const int r = x.row0 + g;
+    const bool ok = g < x.rows;
+    const int s = x.seq + (ok ? (int)a.per_group.div((uint32_t)r) : 0);
+    const unsigned char *qp = a.q + s * a.q_seq + (int64_t)(x.h * a.group + (ok ? r - (s - x.seq) * a.group : 0)) * a.q_head;
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      const int r = x.row0 + g + 8 * half;
-      const bool ok = g + 8 * half < x.rows;
-      const int s = x.seq + (ok ? (int)a.per_group.div((uint32_t)r) : 0);
-      const unsigned char *qp = a.q + s * a.q_seq + (int64_t)(x.h * a.group + (ok ? r - (s - x.seq) * a.group : 0)) * a.q_head;
+    for (int c = 0; c < kKc; ++c)
 #pragma unroll
-      for (int c = 0; c < kKc; ++c)
-#pragma unroll
-        for (int j = 0; j < kE / 8; ++j) {
-          uint4 w = make_uint4(0, 0, 0, 0);
-          if (ok) w = *reinterpret_cast<const uint4 *>(qp + ((c * 4 + t) * kE + j * 8) * 2);
-          const int ks = c * (kE / 4) + j * 2;
-          qf[ks][half] = w.x;
-          qf[ks][half + 2] = w.y;
-          qf[ks + 1][half] = w.z;
-          qf[ks + 1][half + 2] = w.w;
-        }
-    }
+      for (int j = 0; j < kE / 8; ++j) {
+        uint4 w = make_uint4(0, 0, 0, 0);
+        if (ok) w = *reinterpret_cast<const uint4 *>(qp + ((c * 4 + t) * kE + j * 8) * 2);
+        const int ks = c * (kE / 4) + j * 2;
+        qf[ks][0] = w.x;
+        qf[ks][1] = w.y;
+        qf[ks + 1][0] = w.z;
+        qf[ks + 1][1] = w.w;
+      }
   };
   int stage = 0, items = 0;
   LineItem x;
+  // rows of queries 2t and 2t + 1: what their products are multiplied by, maximum, sum (of this lane's keys)
   float by[2], m[2], l[2], ref, unit;
-  float o[D / 8][4];
+  float o[D / 16][4];
 #pragma unroll 1
   for (int at = begin - kStages; at < end; ++at) {
     __syncwarp();             // the stage that is loaded now has been read by every lane
@@ -440,103 +459,105 @@ __global__ void __launch_bounds__(kLineWarps * 32, 1) shared_prefix_attention_ke
     cp_async_wait<kStages - 1>();
     __syncwarp();             // every lane's copies of this tile have arrived
     if (first) {
-by[0] = by[1] = a.scale_log2;              // what a row's products are multiplied by
+      by[0] = by[1] = a.scale_log2;
       if constexpr (kCodes && !std::is_same<T, __half>::value) {
+        float top = 0.f;
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          float top = 0.f;
+        for (int k = 0; k < D / 16; ++k) top = fmaxf(top, fmaxf(largest_of_pair(qf[k][0]), largest_of_pair(qf[k][1])));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const int e = shift_to_half(top);        // of row g
+        const float f = power_of_two(e), back = power_of_two(-e);
 #pragma unroll
-          for (int k = 0; k < D / 16; ++k) top = fmaxf(top, fmaxf(largest_of_pair(qf[k][half]), largest_of_pair(qf[k][half + 2])));
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-          const int e = shift_to_half(top);
-          const float f = power_of_two(e);
-#pragma unroll
-          for (int k = 0; k < D / 16; ++k) {
-            qf[k][half] = pair_to_half(qf[k][half], f);
-            qf[k][half + 2] = pair_to_half(qf[k][half + 2], f);
-          }
-          by[half] *= power_of_two(-e);
+        for (int k = 0; k < D / 16; ++k) {
+          qf[k][0] = pair_to_half(qf[k][0], f);
+          qf[k][1] = pair_to_half(qf[k][1], f);
         }
+        by[0] *= __shfl_sync(0xffffffffu, back, 8 * t);
+        by[1] *= __shfl_sync(0xffffffffu, back, 8 * t + 4);
       }
       m[0] = m[1] = -INFINITY;
       l[0] = l[1] = ref = unit = 0.f;
 #pragma unroll
-      for (int j = 0; j < D / 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
+      for (int j = 0; j < D / 16; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
     }
     {
       const unsigned char *ks = ring.k[stage], *vs = ring.v[stage];
       const uint32_t valid = ring.valid[stage];
 
-      // scores of 16 rows and kKeys keys: s[n][0..1] row g, s[n][2..3] row g + 8, keys 8n + 2t, 8n + 2t + 1
-      float s[kN][4];
+      // scores of kKeys keys and 8 rows: s[n][0..1] key 16n + g, rows 2t and 2t + 1; s[n][2..3] key 16n + g + 8
+      float s[kM][4];
 #pragma unroll
-      for (int n = 0; n < kN; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+      for (int n = 0; n < kM; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
 #pragma unroll
-      for (int c = 0; c < kKc; ++c)
+      for (int c = 0; c < kKc; ++c) {
+        const int at16 = kCpr >= 8 ? (c * 4 + t) ^ ((g & 1) << 2) : c * 4 + t;   // rows g and g + 8 have the same parity
 #pragma unroll
-        for (int n = 0; n < kN; ++n) {
-          const int kr = g + 8 * n;
-          const int at16 = kCpr >= 8 ? (c * 4 + t) ^ ((kr & 1) << 2) : c * 4 + t;
-          const uint4 kw = *reinterpret_cast<const uint4 *>(ks + kr * kRow + at16 * 16);
-          const uint32_t w[4] = {kw.x, kw.y, kw.z, kw.w};
+        for (int n = 0; n < kM; ++n) {
+          const unsigned char *kr = ks + (16 * n + g) * kRow + at16 * 16;
+          const uint4 k0 = *reinterpret_cast<const uint4 *>(kr), k1 = *reinterpret_cast<const uint4 *>(kr + 8 * kRow);
+          const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
           if constexpr (!kCodes) {
-            mma16816<M>(s[n], qf[2 * c], w[0], w[1]);
-            mma16816<M>(s[n], qf[2 * c + 1], w[2], w[3]);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const uint32_t ka[4] = {w0[2 * i], w1[2 * i], w0[2 * i + 1], w1[2 * i + 1]};
+              mma16816<M>(s[n], ka, qf[2 * c + i][0], qf[2 * c + i][1]);
+            }
           } else {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              uint32_t b0, b1;
-              codes_to_pairs<kFmt>(w[i], b0, b1);
-              mma16816<M>(s[n], qf[4 * c + i], b0, b1);
+              uint32_t ka[4];
+              codes_to_pairs<kFmt>(w0[i], ka[0], ka[2]);
+              codes_to_pairs<kFmt>(w1[i], ka[1], ka[3]);
+              mma16816<M>(s[n], ka, qf[4 * c + i][0], qf[4 * c + i][1]);
             }
           }
         }
-      float sv[kN][2];        // scales of the values
-      float top[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-      for (int n = 0; n < kN; ++n) {
-        float2 sk = make_float2(1.f, 1.f);
-        if (kCodes) {
-          sk = *reinterpret_cast<const float2 *>(&ring.scales[stage][8 * n + 2 * t]);
-          const float2 f = *reinterpret_cast<const float2 *>(&ring.scales[stage][kKeys + 8 * n + 2 * t]);
-          sv[n][0] = f.x;
-          sv[n][1] = f.y;
-        }
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          s[n][2 * r] *= kCodes ? by[r] * sk.x : by[r];
-          s[n][2 * r + 1] *= kCodes ? by[r] * sk.y : by[r];
-        }
       }
+      float sv[kM][2];        // scales of the values of keys 16n + g and 16n + g + 8
+#pragma unroll
+      for (int n = 0; n < kM; ++n)
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          float f = 1.f;
+          if (kCodes) {
+            f = ring.scales[stage][16 * n + 8 * y + g];
+            sv[n][y] = ring.scales[stage][kKeys + 16 * n + 8 * y + g];
+          }
+          s[n][2 * y] *= kCodes ? by[0] * f : by[0];
+          s[n][2 * y + 1] *= kCodes ? by[1] * f : by[1];
+        }
       constexpr uint32_t kAll = kKeys == 32 ? 0xffffffffu : 0xffffu;
       if (valid != kAll) {
 #pragma unroll
-        for (int n = 0; n < kN; ++n)
+        for (int n = 0; n < kM; ++n)
 #pragma unroll
-          for (int e = 0; e < 2; ++e)
-            if (!(valid >> (8 * n + 2 * t + e) & 1)) s[n][e] = s[n][2 + e] = -INFINITY;
+          for (int y = 0; y < 2; ++y)
+            if (!(valid >> (16 * n + 8 * y + g) & 1)) s[n][2 * y] = s[n][2 * y + 1] = -INFINITY;
       }
+      float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-      for (int n = 0; n < kN; ++n)
+      for (int n = 0; n < kM; ++n)
 #pragma unroll
-        for (int r = 0; r < 2; ++r) top[r] = fmaxf(top[r], fmaxf(s[n][2 * r], s[n][2 * r + 1]));
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
-        top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
-      }
-      // m follows a row's maximum only where it is 2^8 behind: weights up to 2^8 are as exact as weights up to 1
-      bool move = top[0] > m[0] + 8.f || top[1] > m[1] + 8.f;
+        for (int r = 0; r < 2; ++r) top[r] = fmaxf(top[r], fmaxf(s[n][r], s[n][2 + r]));
+      // m follows a row's maximum only where it is 2^8 behind: weights up to 2^8 are as exact as weights up to 1.
       // fp16 weights of an 8-bit cache: weight * scale may leave fp16's range, so o is kept in units of (a quarter or
-      // more of) the largest scale of a value so far
+      // more of) the largest scale of a value so far.
+      bool move = top[0] > m[0] + 8.f || top[1] > m[1] + 8.f;
       float big = 0.f;
       if (kCodes) {
 #pragma unroll
-        for (int n = 0; n < kN; ++n) big = max_nan(big, max_nan(sv[n][0], sv[n][1]));
+        for (int n = 0; n < kM; ++n) big = max_nan(big, max_nan(sv[n][0], sv[n][1]));
         move = move || !(big <= 4.f * ref);       // also a NaN
       }
       if (__any_sync(0xffffffffu, move)) {
+        // the tile's maxima: over the lanes of equal t
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) {
+          top[0] = fmaxf(top[0], __shfl_xor_sync(0xffffffffu, top[0], d));
+          top[1] = fmaxf(top[1], __shfl_xor_sync(0xffffffffu, top[1], d));
+          if (kCodes) big = max_nan(big, __shfl_xor_sync(0xffffffffu, big, d));
+        }
         float alpha[2];
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
@@ -545,49 +566,40 @@ by[0] = by[1] = a.scale_log2;              // what a row's products are multipli
           m[r] = next;
           l[r] *= alpha[r];
         }
-        if (kCodes) {
-          big = max_nan(big, __shfl_xor_sync(0xffffffffu, big, 1));
-          big = max_nan(big, __shfl_xor_sync(0xffffffffu, big, 2));
-          if (!(big <= 4.f * ref)) {              // the same in every lane
-            alpha[0] *= ref / big;
-            alpha[1] *= ref / big;
-            ref = big;
-            unit = 1.f / big;
-          }
+        if (kCodes && !(big <= 4.f * ref)) {      // the same in every lane
+          alpha[0] *= ref / big;
+          alpha[1] *= ref / big;
+          ref = big;
+          unit = 1.f / big;
         }
 #pragma unroll
-        for (int j = 0; j < D / 8; ++j) {
+        for (int j = 0; j < D / 16; ++j) {
           o[j][0] *= alpha[0];
-          o[j][1] *= alpha[0];
-          o[j][2] *= alpha[1];
+          o[j][1] *= alpha[1];
+          o[j][2] *= alpha[0];
           o[j][3] *= alpha[1];
         }
       }
+      const float safe[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};
+      // o^T: block j = c * kVe / 2 + i has, of chunk c * 8 + g of a row, values 2i (o[j][0..1], rows 2t and 2t + 1) and
+      // 2i + 1 (o[j][2..3])
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const float safe = m[r] == -INFINITY ? 0.f : m[r];
-        float sum = 0.f;
+      for (int n = 0; n < kM; ++n) {
+        uint32_t pw[2];
 #pragma unroll
-        for (int n = 0; n < kN; ++n)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const float p = ex2(s[n][2 * r + e] - safe);
-            sum += p;
-            s[n][2 * r + e] = kCodes ? p * (sv[n][e] * unit) : p;
-          }
-        l[r] += sum;
-      }
-      // o column q (0..7) of block j = c * kVe + e holds value (c * 8 + q) * kVe + e of the head
-#pragma unroll
-      for (int step = 0; step < kKeys / 16; ++step) {
-        const uint32_t pf[4] = {Pair<M>::pack(s[2 * step][0], s[2 * step][1]), Pair<M>::pack(s[2 * step][2], s[2 * step][3]),
-                                Pair<M>::pack(s[2 * step + 1][0], s[2 * step + 1][1]), Pair<M>::pack(s[2 * step + 1][2], s[2 * step + 1][3])};
+        for (int y = 0; y < 2; ++y) {
+          const float p0 = ex2(s[n][2 * y] - safe[0]), p1 = ex2(s[n][2 * y + 1] - safe[1]);
+          l[0] += p0;
+          l[1] += p1;
+          const float f = kCodes ? sv[n][y] * unit : 1.f;
+          pw[y] = transpose8(kCodes ? Pair<M>::pack(p0 * f, p1 * f) : Pair<M>::pack(p0, p1));
+        }
 #pragma unroll
         for (int c = 0; c < kVc; ++c) {
           uint32_t w[4][4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const int vr = 16 * step + 2 * t + (i & 1) + 8 * (i >> 1);
+            const int vr = 16 * n + 2 * t + (i & 1) + 8 * (i >> 1);
             if constexpr (kVb == 16) {
               const uint4 x4 = *reinterpret_cast<const uint4 *>(vs + vr * kRow + (((c * 8 + g) ^ (((vr >> 1) & 3) << 1)) * 16));
               w[i][0] = x4.x;
@@ -603,18 +615,17 @@ by[0] = by[1] = a.scale_log2;              // what a row's products are multipli
 #pragma unroll
           for (int i = 0; i < kVb / 4; ++i) {
             if constexpr (!kCodes) {
-              mma16816<M>(o[c * kVe + 2 * i], pf, __byte_perm(w[0][i], w[1][i], 0x5410), __byte_perm(w[2][i], w[3][i], 0x5410));
-              mma16816<M>(o[c * kVe + 2 * i + 1], pf, __byte_perm(w[0][i], w[1][i], 0x7632), __byte_perm(w[2][i], w[3][i], 0x7632));
+              const uint32_t va[4] = {__byte_perm(w[0][i], w[1][i], 0x5410), __byte_perm(w[0][i], w[1][i], 0x7632),
+                                      __byte_perm(w[2][i], w[3][i], 0x5410), __byte_perm(w[2][i], w[3][i], 0x7632)};
+              mma16816<M>(o[c * (kVe / 2) + i], va, pw[0], pw[1]);
             } else {
-              uint32_t x0, x1, x2, x3, y0, y1, y2, y3;
-              codes_to_pairs<kFmt>(__byte_perm(w[0][i], w[1][i], 0x5140), x0, x1);
-              codes_to_pairs<kFmt>(__byte_perm(w[0][i], w[1][i], 0x7362), x2, x3);
-              codes_to_pairs<kFmt>(__byte_perm(w[2][i], w[3][i], 0x5140), y0, y1);
-              codes_to_pairs<kFmt>(__byte_perm(w[2][i], w[3][i], 0x7362), y2, y3);
-              mma16816<M>(o[c * kVe + 4 * i], pf, x0, y0);
-              mma16816<M>(o[c * kVe + 4 * i + 1], pf, x1, y1);
-              mma16816<M>(o[c * kVe + 4 * i + 2], pf, x2, y2);
-              mma16816<M>(o[c * kVe + 4 * i + 3], pf, x3, y3);
+              uint32_t va[4], vb[4];
+              codes_to_pairs<kFmt>(__byte_perm(w[0][i], w[1][i], 0x5140), va[0], va[1]);
+              codes_to_pairs<kFmt>(__byte_perm(w[0][i], w[1][i], 0x7362), vb[0], vb[1]);
+              codes_to_pairs<kFmt>(__byte_perm(w[2][i], w[3][i], 0x5140), va[2], va[3]);
+              codes_to_pairs<kFmt>(__byte_perm(w[2][i], w[3][i], 0x7362), vb[2], vb[3]);
+              mma16816<M>(o[c * (kVe / 2) + 2 * i], va, pw[0], pw[1]);
+              mma16816<M>(o[c * (kVe / 2) + 2 * i + 1], vb, pw[0], pw[1]);
             }
           }
         }
@@ -624,27 +635,25 @@ by[0] = by[1] = a.scale_log2;              // what a row's products are multipli
     ++x.tile;
     if (x.tile != x.tiles && at + 1 != end) continue;
 
-    // this warp's part of the item: lane (g, t) has columns 2t and 2t + 1 of every block, which is, for a chunk c, kVe
-    // values in a row of the head each
+    // this warp's part of the item: lane (g, t) has kVe neighbouring values of each chunk, of two rows
     const int64_t part = (int64_t)me + x.ordinal;
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-      const int row = g + 8 * r;
+#pragma unroll
+      for (int d = 4; d < 32; d <<= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], d);
+      const int row = 2 * t + r;
       if (row < x.rows) {
-        if (t == 0) a.part_ml[part * 16 + row] = make_float2(m[r], l[r]);
+        if (g == 0) a.part_ml[part * kItemRows + row] = make_float2(m[r], l[r]);
         const float back = kCodes ? ref : 1.f;
-        float *dst = a.part_o + (part * 16 + row) * D;
+        float *dst = a.part_o + (part * kItemRows + row) * D;
 #pragma unroll
         for (int c = 0; c < kVc; ++c)
 #pragma unroll
-          for (int y = 0; y < 2; ++y)
-#pragma unroll
-            for (int e = 0; e < kVe; e += 4)
-              *reinterpret_cast<float4 *>(dst + (c * 8 + 2 * t + y) * kVe + e) =
-                  make_float4(o[c * kVe + e][2 * r + y] * back, o[c * kVe + e + 1][2 * r + y] * back, o[c * kVe + e + 2][2 * r + y] * back,
-                              o[c * kVe + e + 3][2 * r + y] * back);
+          for (int e = 0; e < kVe; e += 4) {
+            const int j = c * (kVe / 2) + e / 2;
+            *reinterpret_cast<float4 *>(dst + (c * 8 + g) * kVe + e) =
+                make_float4(o[j][r] * back, o[j][2 + r] * back, o[j + 1][r] * back, o[j + 1][2 + r] * back);
+          }
       }
     }
   }
@@ -662,11 +671,12 @@ struct JoinArgs {
   const float *prefix_o;
 };
 
-// Four warps a row, each with every fourth part and up to eight loads of a part under way: the parts (some dozens of a
-// row) are in L2, and the time is that of the chain of their loads.
-constexpr int kJoinWarps = 4, kJoinAhead = 8;
-template <typename T, int D>
-__global__ void __launch_bounds__(kJoinWarps * 32) shared_prefix_join_kernel(const __grid_constant__ JoinArgs args) {
+// kJoinWarps warps a row, each with every kJoinWarps-th part and up to eight loads of a part under way: the parts (some
+// dozens of a row) are in L2, and the time is that of the chain of their loads, so all rows should be at it at once: four
+// warps a row where that fits, else two, else one (2048 rows of 20 parts: 10 us with four, which take two turns).
+constexpr int kJoinAhead = 8;
+template <typename T, int D, int kJoinWarps>
+__global__ void __launch_bounds__(kJoinWarps * 32, 28 / kJoinWarps) shared_prefix_join_kernel(const __grid_constant__ JoinArgs args) {
   __shared__ float sums[kJoinWarps][D + 1];
   const AttnArgs &a = args.a;
   const int row = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -687,13 +697,13 @@ __global__ void __launch_bounds__(kJoinWarps * 32) shared_prefix_join_kernel(con
       int item, from, tiles, place;
       if (k == 0) {
         const int r = s * a.group + g;
-        item = h * line.row_tiles + r / 16;
-        place = r % 16;
+        item = h * line.row_tiles + r / kItemRows;
+        place = r % kItemRows;
         from = item * line.prefix_tiles;
         tiles = line.prefix_tiles;
       } else {
-        const int hg = h * line.own_tiles + g / 16;
-        place = g % 16;
+        const int hg = h * line.own_tiles + g / kItemRows;
+        place = g % kItemRows;
         tiles = behind - before;
         from = in_prefix + before * line.per_seq + hg * tiles;
         item = line.prefix_items + s * line.per_seq + hg;
@@ -701,7 +711,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) shared_prefix_join_kernel(con
       if (tiles > 0) {
         const int w0 = warp_of_tile(from, warps, total), w1 = warp_of_tile(from + tiles - 1, warps, total);
         count[k] = w1 - w0 + 1;
-        first[k] = ((int64_t)w0 + item) * 16 + place;
+        first[k] = ((int64_t)w0 + item) * kItemRows + place;
       }
     }
   }
@@ -713,27 +723,14 @@ __global__ void __launch_bounds__(kJoinWarps * 32) shared_prefix_join_kernel(con
   const int parts = count[0] + count[1] + count[2];
   auto part_of = [&](int i, const float2 *&ml, const float *&o) {
     const bool p0 = i < count[0], p1 = i < count[0] + count[1];
-    const int64_t at = p0 ? first[0] + (int64_t)i * 16 : p1 ? first[1] + (int64_t)(i - count[0]) * 16 : first[2] + (i - count[0] - count[1]) * stride;
+    const int64_t at = p0 ? first[0] + (int64_t)i * kItemRows : p1 ? first[1] + (int64_t)(i - count[0]) * kItemRows : first[2] + (i - count[0] - count[1]) * stride;
     ml = (p1 ? a.part_ml : args.prefix_ml) + at;
     o = (p1 ? a.part_o : args.prefix_o) + at * D;
   };
-  // the largest maximum: every warp looks at all
-  float big = -INFINITY;
-  for (int i = lane; i < parts; i += 32) {
-    const float2 *ml;
-    const float *o;
-    part_of(i, ml, o);
-    big = fmaxf(big, ml->x);
-  }
-#pragma unroll
-  for (int d = 16; d > 0; d >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, d));
   constexpr int kPer = D / 32;
-  float l = 0.f, sum[kPer];
-#pragma unroll
-  for (int e = 0; e < kPer; ++e) sum[e] = 0.f;
-  for (int i0 = warp; i0 < parts; i0 += kJoinWarps * kJoinAhead) {
-    float2 ml[kJoinAhead];
-    float o[kJoinAhead][kPer];
+  float2 ml[kJoinAhead];
+  float o[kJoinAhead][kPer];
+  auto fetch = [&](int i0) {
 #pragma unroll
     for (int u = 0; u < kJoinAhead; ++u) {
       const int i = i0 + u * kJoinWarps;
@@ -758,6 +755,23 @@ __global__ void __launch_bounds__(kJoinWarps * 32) shared_prefix_join_kernel(con
         }
       }
     }
+  };
+  fetch(warp);                // on their way while the maximum is found
+  // the largest maximum: every warp looks at all
+  float big = -INFINITY;
+  for (int i = lane; i < parts; i += 32) {
+    const float2 *mp;
+    const float *op;
+    part_of(i, mp, op);
+    big = fmaxf(big, mp->x);
+  }
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, d));
+  float l = 0.f, sum[kPer];
+#pragma unroll
+  for (int e = 0; e < kPer; ++e) sum[e] = 0.f;
+#pragma unroll 1
+  for (int i0 = warp; i0 < parts;) {
 #pragma unroll
     for (int u = 0; u < kJoinAhead; ++u) {
       const float f = big == -INFINITY ? 1.f : ex2(ml[u].x - big);
@@ -765,13 +779,14 @@ __global__ void __launch_bounds__(kJoinWarps * 32) shared_prefix_join_kernel(con
 #pragma unroll
       for (int e = 0; e < kPer; ++e) sum[e] += o[u][e] * f;
     }
+    i0 += kJoinWarps * kJoinAhead;
+    if (i0 < parts) fetch(i0);
   }
 #pragma unroll
   for (int e = 0; e < kPer; ++e) sums[warp][lane * kPer + e] = sum[e];
   if (lane == 0) sums[warp][D] = l;
   __syncthreads();
-  const int v = threadIdx.x * 2;
-  if (v < D) {
+  for (int v = threadIdx.x * 2; v < D; v += kJoinWarps * 64) {
     float2 r = make_float2(0.f, 0.f);
     l = 0.f;
 #pragma unroll
@@ -782,7 +797,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) shared_prefix_join_kernel(con
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;   // a NaN stays
     *reinterpret_cast<uint32_t *>(a.out + s * a.out_seq + (int64_t)head * a.out_head + v * 2) = Pair<T>::pack(r.x * inv, r.y * inv);
-    if (a.lse != nullptr && threadIdx.x == 0) a.lse[(int64_t)s * q_heads + head] = l == 0.f ? -INFINITY : kLn2 * (big + log2f(l));
+    if (a.lse != nullptr && v == 0) a.lse[(int64_t)s * q_heads + head] = l == 0.f ? -INFINITY : kLn2 * (big + log2f(l));
   }
 }
 
