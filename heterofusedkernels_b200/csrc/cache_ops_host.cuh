@@ -57,10 +57,8 @@ static int validate_written(const char *op, const char *name, const hfk_rows &r,
 // ---- writing ------------------------------------------------------------------------------------------------
 template <typename T, int kFmt, bool kRope, int kLanes>
 static cudaError_t launch_kv_write(const KvWriteArgs &a, cudaStream_t stream) {
-  constexpr int kThreads = 256;
-  constexpr int kGroups = kThreads / kLanes;
-  const uint32_t ctas = (a.rows + kGroups - 1) / kGroups;
-  kv_write_kernel<T, kFmt, kRope, kLanes, 1, kThreads><<<ctas, kThreads, 0, stream>>>(a);
+  constexpr int kThreads = 128, kGroups = kThreads / kLanes;
+  kv_write_kernel<T, kFmt, kRope, kLanes, kThreads><<<(a.rows + kGroups - 1) / kGroups, kThreads, 0, stream>>>(a);
   return cudaGetLastError();
 }
 
@@ -73,9 +71,9 @@ static cudaError_t launch_kv_write(const KvWriteArgs &a, int fmt, cudaStream_t s
 
 template <typename T, bool kRope>
 static cudaError_t launch_kv_write(const KvWriteArgs &a, int fmt, cudaStream_t s) {
-  if (a.head_dim <= 64) return launch_kv_write<T, kRope, 8>(a, fmt, s);
-  if (a.head_dim <= 128) return launch_kv_write<T, kRope, 16>(a, fmt, s);
-  return launch_kv_write<T, kRope, 32>(a, fmt, s);
+  if (a.head_dim <= 64) return launch_kv_write<T, kRope, 4>(a, fmt, s);
+  if (a.head_dim <= 128) return launch_kv_write<T, kRope, 8>(a, fmt, s);
+  return launch_kv_write<T, kRope, 16>(a, fmt, s);
 }
 
 static int kv_write_impl(const char *op, const hfk_kv_write_desc *d, const hfk_norm_rope_desc *n, bool rope, cudaStream_t stream) {

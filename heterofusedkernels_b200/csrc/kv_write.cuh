@@ -39,169 +39,159 @@ struct KvWriteArgs {
 };
 
 
-// A row is handled by kLanes lanes of a warp, eight elements each (kLanes * 8 >= head_dim); a CTA handles
-// kRows consecutive rows for each of its lane groups at a time, all loads first.  Consecutive groups take
-// consecutive heads of a token, so that loads, stores and the 4-byte scales of neighbours fall into the same
-// lines.
-template <typename T, int kFmt, bool kRope, int kLanes, int kRows, int kThreads>
-__global__ void __launch_bounds__(kThreads) kv_write_kernel(const __grid_constant__ KvWriteArgs a) {
+// Two blocks of eight elements of a row to each of kLanes lanes (kLanes * 16 >= head_dim).  Where pairs (i, i + rot/2) are
+// rotated, lane j < rot/16 holds blocks j and j + rot/16, so that either partner is its own; other lanes hold neighbours.
+// Consecutive groups of lanes take consecutive heads of a token, so that loads, stores and the 4-byte scales of
+// neighbours fall into the same lines.
+//
+// Measured: 65536 tokens of 8 heads of 128, fp16 to int8 (407 MB): 102 us with one block a lane (the arithmetic on addresses
+// took as long as the data), 70 with two; 16384 tokens with rotation of 40 heads, fp16 to e4m3 (379 MB): 135 and 80 us.  Two
+// or four rows a thread were slower (85 and 172 us there): what helps is that many warps fit, so CTAs are of 128 threads
+// and the kernel without rotation is held to 32 registers.
+template <typename T, int kFmt, bool kRope, int kLanes, int kThreads>
+__global__ void __launch_bounds__(kThreads, kRope ? 1 : 16) kv_write_kernel(const __grid_constant__ KvWriteArgs a) {
   constexpr int kGroups = kThreads / kLanes;
   const int lane = threadIdx.x % kLanes;
-  const int group = threadIdx.x / kLanes;
-  const bool inside = lane * 8 < a.head_dim;
-  const uint32_t first = blockIdx.x * (uint32_t)(kGroups * kRows) + group;
+  const uint32_t r = blockIdx.x * (uint32_t)kGroups + threadIdx.x / kLanes;
+  const bool inside = lane * 16 < a.head_dim;
+  const int pairs = kRope && !a.interleaved ? a.rot >> 4 : 0;       // lanes with blocks rot/2 apart
+  const int block[2] = {lane < pairs ? lane : 2 * lane, lane < pairs ? lane + pairs : 2 * lane + 1};
 
-  uint4 in[kRows];
-  uint32_t token[kRows], head[kRows];   // head counts q heads, then k heads, then v heads
-  int64_t slot[kRows];
-  int64_t position[kRows];
-  bool live[kRows];
+  bool live = r < a.rows;
+  const uint32_t token = a.per_token.div(live ? r : 0);
+  const int h = (int)((live ? r : 0) - token * a.per_token.d);      // counts q heads, then k heads, then v heads
+  const int64_t slot = load_id(a.slots, a.slots_are_int64, token);
+  const int64_t position = kRope ? load_id(a.positions, a.positions_are_int64, token) : 0;
+  const bool is_q = kRope && h < a.q_heads, is_v = h >= a.q_heads + a.kv_heads;
+  const int kv_head = is_v ? h - a.q_heads - a.kv_heads : h - a.q_heads;
+  const unsigned char *src = is_q   ? a.q + token * a.q_token + h * a.q_head
+                             : is_v ? a.v + token * a.v_token + kv_head * a.v_head
+                                    : a.k + token * a.k_token + kv_head * a.k_head;
+  uint4 in[2];
 #pragma unroll
-  for (int u = 0; u < kRows; ++u) {
-    const uint32_t r = first + u * kGroups;
-    live[u] = r < a.rows;
-    token[u] = a.per_token.div(live[u] ? r : 0);
-    head[u] = (live[u] ? r : 0) - token[u] * a.per_token.d;
-    slot[u] = load_id(a.slots, a.slots_are_int64, token[u]);
-    position[u] = kRope ? load_id(a.positions, a.positions_are_int64, token[u]) : 0;
-    const int h = (int)head[u];
-    const unsigned char *src;
-    if (kRope && h < a.q_heads)
-      src = a.q + token[u] * a.q_token + h * a.q_head;
-    else if (h < a.q_heads + a.kv_heads)
-      src = a.k + token[u] * a.k_token + (h - a.q_heads) * a.k_head;
-    else
-      src = a.v + token[u] * a.v_token + (h - a.q_heads - a.kv_heads) * a.v_head;
-    in[u] = make_uint4(0, 0, 0, 0);
-    if (inside && live[u]) in[u] = *reinterpret_cast<const uint4 *>(src + lane * 16);
+  for (int b = 0; b < 2; ++b) {
+    in[b] = make_uint4(0, 0, 0, 0);
+    if (inside && live) in[b] = *reinterpret_cast<const uint4 *>(src + block[b] * 16);
+  }
+  // a negative slot is padding: nothing of the token is written
+  if (live && slot >= a.num_slots) {
+    raise_status(HFK_DEV_BAD_DEVICE_BLOCK_ID);
+    live = false;
+  }
+  live = live && slot >= 0;
+  if (kRope && live && (position < 0 || position >= a.max_positions)) {
+    raise_status(HFK_DEV_BAD_POSITION);
+    live = false;
+  }
+  unsigned char *page = nullptr;
+  uint32_t place = 0;
+  if (live && !is_q) {
+    const uint32_t b = a.block.div((uint32_t)slot);
+    place = ((uint32_t)slot - b * a.block.d) * a.kv_heads + kv_head;
+    page = (is_v ? a.v_cache : a.k_cache) + (int64_t)b * a.block_stride;
   }
 
+  if constexpr (!kRope && kFmt == kFmtRaw) {
+    if (live && inside) {
+      unsigned char *dst = page + (int64_t)place * a.head_dim * 2;
+      *reinterpret_cast<uint4 *>(dst + block[0] * 16) = in[0];
+      *reinterpret_cast<uint4 *>(dst + block[1] * 16) = in[1];
+    }
+  } else {
+  float x[2][8];
 #pragma unroll
-  for (int u = 0; u < kRows; ++u) {
-    // a negative slot is padding: nothing of the token is written
-    if (live[u] && slot[u] >= a.num_slots) {
-      raise_status(HFK_DEV_BAD_DEVICE_BLOCK_ID);
-      live[u] = false;
-    }
-    live[u] = live[u] && slot[u] >= 0;
-    if (kRope && live[u] && (position[u] < 0 || position[u] >= a.max_positions)) {
-      raise_status(HFK_DEV_BAD_POSITION);
-      live[u] = false;
-    }
-    const int h = (int)head[u];
-    const bool is_q = kRope && h < a.q_heads;
-    const bool is_v = h >= a.q_heads + a.kv_heads;
-    const int kv_head = is_v ? h - a.q_heads - a.kv_heads : h - a.q_heads;
-    unsigned char *page = nullptr;
-    uint32_t place = 0;
-    if (live[u] && !is_q) {
-      const uint32_t b = a.block.div((uint32_t)slot[u]);
-      place = ((uint32_t)slot[u] - b * a.block.d) * a.kv_heads + kv_head;
-      page = (is_v ? a.v_cache : a.k_cache) + (int64_t)b * a.block_stride;
-    }
-
-    if (!kRope && kFmt == kFmtRaw) {
-      if (live[u] && inside)
-        *reinterpret_cast<uint4 *>(page + (int64_t)place * a.head_dim * 2 + lane * 16) = in[u];
-      continue;
-    }
-
-    const uint32_t w[4] = {in[u].x, in[u].y, in[u].z, in[u].w};
-    float x[8];
+  for (int b = 0; b < 2; ++b) {
+    const uint32_t w[4] = {in[b].x, in[b].y, in[b].z, in[b].w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const float2 f = Pair<T>::unpack(w[i]);
-      x[2 * i] = f.x;
-      x[2 * i + 1] = f.y;
+      x[b][2 * i] = f.x;
+      x[b][2 * i + 1] = f.y;
     }
+  }
 
-    if (kRope) {
-      const void *weight = is_q ? a.q_weight : (is_v ? nullptr : a.k_weight);
+  if constexpr (kRope) {
+    const void *weight = is_q ? a.q_weight : (is_v ? nullptr : a.k_weight);
+    if (a.q_weight != nullptr || a.k_weight != nullptr) {
       float sum = 0.f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) sum = fmaf(x[i], x[i], sum);
+      for (int i = 0; i < 8; ++i) sum = fmaf(x[0][i], x[0][i], fmaf(x[1][i], x[1][i], sum));
 #pragma unroll
       for (int d = kLanes / 2; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d, kLanes);
       if (weight != nullptr && inside) {
-        const float r = rsqrtf(sum / (float)a.head_dim + a.eps);
-        const uint4 g = *reinterpret_cast<const uint4 *>(static_cast<const unsigned char *>(weight) + lane * 16);
-        const uint32_t gw[4] = {g.x, g.y, g.z, g.w};
+        const float scale = rsqrtf(sum / (float)a.head_dim + a.eps);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float2 f = Pair<T>::unpack(gw[i]);
-          x[2 * i] = x[2 * i] * r * f.x;
-          x[2 * i + 1] = x[2 * i + 1] * r * f.y;
-        }
-      }
-      const bool turn = live[u] && !is_v && lane * 8 < a.rot;
-      const float *table = a.cos_sin + (turn ? position[u] * a.rot : 0);
-      if (a.interleaved) {
-        if (turn) {
-          const float4 c = *reinterpret_cast<const float4 *>(table + lane * 4);
-          const float4 s = *reinterpret_cast<const float4 *>(table + a.rot / 2 + lane * 4);
-          const float cs[4] = {c.x, c.y, c.z, c.w}, sn[4] = {s.x, s.y, s.z, s.w};
+        for (int b = 0; b < 2; ++b) {
+          const uint4 g = *reinterpret_cast<const uint4 *>(static_cast<const unsigned char *>(weight) + block[b] * 16);
+          const uint32_t gw[4] = {g.x, g.y, g.z, g.w};
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const float lo = x[2 * i], hi = x[2 * i + 1];
-            x[2 * i] = lo * cs[i] - hi * sn[i];
-            x[2 * i + 1] = hi * cs[i] + lo * sn[i];
-          }
-        }
-      } else {
-        const int half = a.rot >> 4;  // lanes per half: rot / 2 elements, eight to a lane
-        const bool low = lane < half;
-        const int partner = low ? lane + half : lane - half;
-        float other[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) other[i] = __shfl_sync(0xffffffffu, x[i], partner & (kLanes - 1), kLanes);
-        if (turn) {
-          const float *cp = table + (low ? lane : lane - half) * 8;
-          const float *sp = cp + a.rot / 2;
-          const float sign = low ? -1.f : 1.f;
-#pragma unroll
-          for (int i = 0; i < 8; i += 4) {
-            const float4 c = *reinterpret_cast<const float4 *>(cp + i);
-            const float4 s = *reinterpret_cast<const float4 *>(sp + i);
-            x[i] = x[i] * c.x + sign * other[i] * s.x;
-            x[i + 1] = x[i + 1] * c.y + sign * other[i + 1] * s.y;
-            x[i + 2] = x[i + 2] * c.z + sign * other[i + 2] * s.z;
-            x[i + 3] = x[i + 3] * c.w + sign * other[i + 3] * s.w;
+            const float2 f = Pair<T>::unpack(gw[i]);
+            x[b][2 * i] = x[b][2 * i] * scale * f.x;
+            x[b][2 * i + 1] = x[b][2 * i + 1] * scale * f.y;
           }
         }
       }
     }
-
-    if (kFmt == kFmtRaw || is_q) {
-      if (live[u] && inside) {
-        unsigned char *dst = is_q ? a.q_out + token[u] * a.qo_token + h * a.qo_head
-                                  : page + (int64_t)place * a.head_dim * 2;
-        *reinterpret_cast<uint4 *>(dst + lane * 16) =
-            make_uint4(Pair<T>::pack(x[0], x[1]), Pair<T>::pack(x[2], x[3]), Pair<T>::pack(x[4], x[5]),
-                       Pair<T>::pack(x[6], x[7]));
-      }
-      if (kFmt == kFmtRaw) continue;
-    }
-
-    if (kFmt != kFmtRaw) {
-      float top = 0.f;
+    if (live && !is_v && lane * 16 < a.rot) {
+      // eight pairs of the lane, of its two blocks or neighbours inside them; four at a time
+      const float *cp = a.cos_sin + position * a.rot + lane * 8, *sp = cp + a.rot / 2;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) top = max_nan(top, fabsf(x[i]));
+      for (int q = 0; q < 2; ++q) {
+        const float4 c4 = *reinterpret_cast<const float4 *>(cp + 4 * q), s4 = *reinterpret_cast<const float4 *>(sp + 4 * q);
+        const float c[4] = {c4.x, c4.y, c4.z, c4.w}, s[4] = {s4.x, s4.y, s4.z, s4.w};
 #pragma unroll
-      for (int d = kLanes / 2; d > 0; d >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, d, kLanes));
-      float scale = __fmul_rn(top, 1.f / top_code<kFmt>());
-      if (scale < kLeastScale) scale = kLeastScale;  // a NaN stays
-      if (scale > 3.4e38f) scale = __uint_as_float(0x7fffffffu);  // an infinity in the row: no code stands for its parts
-      const float inv = __frcp_rn(scale);
-      if (live[u] && !is_q) {
-        if (inside) {
-          uint2 codes;
-          codes.x = float_to_codes<kFmt>(__fmul_rn(x[0], inv), __fmul_rn(x[1], inv), __fmul_rn(x[2], inv), __fmul_rn(x[3], inv));
-          codes.y = float_to_codes<kFmt>(__fmul_rn(x[4], inv), __fmul_rn(x[5], inv), __fmul_rn(x[6], inv), __fmul_rn(x[7], inv));
-          *reinterpret_cast<uint2 *>(page + (int64_t)place * a.head_dim + lane * 8) = codes;
+        for (int i = 0; i < 4; ++i) {
+          if (a.interleaved) {
+            const float lo = x[q][2 * i], hi = x[q][2 * i + 1];
+            x[q][2 * i] = lo * c[i] - hi * s[i];
+            x[q][2 * i + 1] = hi * c[i] + lo * s[i];
+          } else {
+            const float lo = x[0][4 * q + i], hi = x[1][4 * q + i];
+            x[0][4 * q + i] = lo * c[i] - hi * s[i];
+            x[1][4 * q + i] = hi * c[i] + lo * s[i];
+          }
         }
-        if (lane == 0) reinterpret_cast<float *>(page + a.scales_at)[place] = scale;
       }
     }
+  }
+
+  if (kFmt == kFmtRaw || is_q) {
+    if (live && inside) {
+      unsigned char *dst = is_q ? a.q_out + token * a.qo_token + h * a.qo_head : page + (int64_t)place * a.head_dim * 2;
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+        *reinterpret_cast<uint4 *>(dst + block[b] * 16) =
+            make_uint4(Pair<T>::pack(x[b][0], x[b][1]), Pair<T>::pack(x[b][2], x[b][3]), Pair<T>::pack(x[b][4], x[b][5]),
+                       Pair<T>::pack(x[b][6], x[b][7]));
+    }
+  }
+  if constexpr (kFmt != kFmtRaw) {
+    if (__all_sync(0xffffffffu, is_q)) return;   // the other lanes of a warp may hold keys or values
+    float top = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = max_nan(max_nan(top, fabsf(x[0][i])), fabsf(x[1][i]));
+#pragma unroll
+    for (int d = kLanes / 2; d > 0; d >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, d, kLanes));
+    float scale = __fmul_rn(top, 1.f / top_code<kFmt>());
+    if (scale < kLeastScale) scale = kLeastScale;  // a NaN stays
+    if (scale > 3.4e38f) scale = __uint_as_float(0x7fffffffu);  // an infinity in the row: no code stands for its parts
+    const float inv = __frcp_rn(scale);
+    if (live && !is_q) {
+      if (inside) {
+        unsigned char *dst = page + (int64_t)place * a.head_dim;
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          float y[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) y[i] = __fmul_rn(x[b][i], inv);
+          *reinterpret_cast<uint2 *>(dst + block[b] * 8) =
+              make_uint2(float_to_codes<kFmt>(y[0], y[1], y[2], y[3]), float_to_codes<kFmt>(y[4], y[5], y[6], y[7]));
+        }
+      }
+      if (lane == 0) reinterpret_cast<float *>(page + a.scales_at)[place] = scale;
+    }
+  }
   }
 }
 
