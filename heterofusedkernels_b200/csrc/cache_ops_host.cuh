@@ -223,8 +223,8 @@ struct AttnPlan {
   int splits;       // its runs of key tiles
   int ctas, warps;  // of the line
   int seqs;         // sequences a group of launches takes
-  size_t cu_bytes, ml_bytes, o_bytes, prefix_ml_bytes, prefix_o_bytes;
-  size_t bytes() const { return cu_bytes + ml_bytes + o_bytes + prefix_ml_bytes + prefix_o_bytes; }
+  size_t ml_bytes, o_bytes, prefix_ml_bytes, prefix_o_bytes;
+  size_t bytes() const { return 256 + ml_bytes + o_bytes + prefix_ml_bytes + prefix_o_bytes; }
 };
 
 static int plan_attention(const hfk_prefix_attention_desc *d, int ctas, AttnPlan *p) {
@@ -252,13 +252,14 @@ static int plan_attention(const hfk_prefix_attention_desc *d, int ctas, AttnPlan
   p->tensor = d->prefix_len > 0 && rows > kPrefixTensorMinRows;
   p->splits = 0;
   if (p->tensor) {
-    // as many runs as give the least time for the slowest SM: waves of CTAs, each its key tiles and a constant for
-    // filling the pipeline and writing the part
+    // as many runs as give the least time, in key tiles: waves of CTAs, each its tiles and a constant for filling the
+    // pipeline, and for each run its part of every row, which is written and read again
     const int64_t items = d->kv_heads * ((rows + 255) / 256), tiles = (d->prefix_len + kPtKeys - 1) / kPtKeys;
     const int64_t room = ctas > 0 ? std::min(ctas, sms) : sms;
     int64_t best = 0;
     for (int64_t s = 1; s <= std::min<int64_t>(tiles, std::max<int64_t>(1, 2 * room / items)); ++s) {
-      const int64_t cost = ((items * s + room - 1) / room) * ((tiles + s - 1) / s + kPrefixTileOverhead);
+      const int64_t cost = ((items * s + room - 1) / room) * ((tiles + s - 1) / s + kPrefixTileOverhead) * 64 +
+                           s * d->kv_heads * rows * d->head_dim / kPrefixPartValues;
       if (p->splits == 0 || cost < best) {
         best = cost;
         p->splits = (int)s;
@@ -270,7 +271,6 @@ static int plan_attention(const hfk_prefix_attention_desc *d, int ctas, AttnPlan
   p->warps = p->ctas * kLineWarps;
   const size_t parts = p->ctas > 0 ? (size_t)p->warps + (size_t)line.items(seqs) : 0;
   const auto round = [](size_t n) { return (n + 255) & ~(size_t)255; };
-  p->cu_bytes = round((size_t)(seqs + 1) * sizeof(int));
   p->ml_bytes = round(parts * kItemRows * sizeof(float2));
   p->o_bytes = round(parts * kItemRows * d->head_dim * sizeof(float));
   p->prefix_ml_bytes = round((size_t)p->splits * d->kv_heads * rows * sizeof(float2));
@@ -301,9 +301,8 @@ static cudaError_t launch_attention(const AttnArgs &a, const AttnPlan &p, unsign
   join.a = a;
   join.warps = p.warps;
   join.rows = a.seqs * a.group;
-  join.a.cu = reinterpret_cast<int *>(w);
-  join.a.part_ml = reinterpret_cast<float2 *>(w + p.cu_bytes);
-  join.a.part_o = reinterpret_cast<float *>(w + p.cu_bytes + p.ml_bytes);
+  join.a.part_ml = reinterpret_cast<float2 *>(w);
+  join.a.part_o = reinterpret_cast<float *>(w + p.ml_bytes);
   cudaError_t e;
   if (p.tensor) {
     PrefixTensorArgs t = {};
@@ -313,8 +312,8 @@ static cudaError_t launch_attention(const AttnArgs &a, const AttnPlan &p, unsign
     t.rows = join.rows;
     t.row_blocks = (t.rows + 255) / 256;
     t.splits = p.splits;
-    t.part_ml = reinterpret_cast<float2 *>(w + p.cu_bytes + p.ml_bytes + p.o_bytes);
-    t.part_o = reinterpret_cast<float *>(w + p.cu_bytes + p.ml_bytes + p.o_bytes + p.prefix_ml_bytes);
+    t.part_ml = reinterpret_cast<float2 *>(w + p.ml_bytes + p.o_bytes);
+    t.part_o = reinterpret_cast<float *>(w + p.ml_bytes + p.o_bytes + p.prefix_ml_bytes);
     auto k = prefix_tensor_kernel<T, kFmt, D>;
     const size_t smem = sizeof(PrefixSmem<D>) + 1024;
     if ((e = allow_smem(k, smem)) != cudaSuccess) return e;
@@ -332,6 +331,7 @@ static cudaError_t launch_attention(const AttnArgs &a, const AttnPlan &p, unsign
     if ((e = launch_behind(k, p.tensor, p.ctas, kLineWarps * 32, smem, s, join.a)) != cudaSuccess) return e;
   }
   const int rows = a.seqs * a.kv_heads * a.group, resident = sm_count() * kJoinWarpsPerSm;
+  if (rows * 16 <= resident) return launch_behind(shared_prefix_join_kernel<T, D, 16>, true, rows, 512, 0, s, join);
   if (rows * 4 <= resident) return launch_behind(shared_prefix_join_kernel<T, D, 4>, true, rows, 128, 0, s, join);
   if (rows * 2 <= resident) return launch_behind(shared_prefix_join_kernel<T, D, 2>, true, rows, 64, 0, s, join);
   return launch_behind(shared_prefix_join_kernel<T, D, 1>, true, rows, 32, 0, s, join);

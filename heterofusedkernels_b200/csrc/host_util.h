@@ -57,9 +57,11 @@ constexpr int kGatherDequantCtasPerSm = 2;
 constexpr int kAttnCtasPerSm = 1;
 // Warps of the join that an SM holds at once (about 72 registers a thread).
 constexpr int kJoinWarpsPerSm = 28;
-// Rows of queries (sequences x query heads of a K/V head) above which the prefix goes to the tensor-core kernel, and
-// what a CTA of it costs beyond its key tiles, in tiles.
+// Rows of queries (sequences x query heads of a K/V head) above which the prefix goes to the tensor-core kernel.
 constexpr int kPrefixTensorMinRows = 32;
+// What a CTA of that kernel costs beyond its key tiles, in tiles of about 2.6 us, and how many values of parts (8 bytes to
+// and from L2 each) cost a 64th of that.
 constexpr int kPrefixTileOverhead = 3;
+constexpr int kPrefixPartValues = 15000;
 
 }  // namespace hfk

@@ -44,7 +44,6 @@ struct AttnArgs {
   int tile;                       // keys of a tile of the line
   float scale_log2;               // scale * log2 e
   // partial results (workspace)
-  int *cu;                        // [seqs + 1] first tile of each sequence, per (K/V head, row tile)
   float2 *part_ml;                // [parts][kItemRows]  (m, l)
   float *part_o;                  // [parts][kItemRows][head_dim]
 };
@@ -141,10 +140,8 @@ struct AttnLine {
   }
 };
 
-// Warps that take part: each at least kLeastTiles tiles (a part costs a start-up and a place in the join), and with
-// fewer tiles than that one warp; so none of them is without a tile.
-constexpr int kLeastTiles = 2;
-__device__ __forceinline__ int line_warps(int warps, int total) { return max(min(1, total), min(warps, total / kLeastTiles)); }
+// Warps that take part: with fewer tiles than warps one tile each, so none of them is without a tile.
+__device__ __forceinline__ int line_warps(int warps, int total) { return min(warps, total); }
 // The first tile of warp w, and the warp that has tile x: w has [total w / warps, total (w + 1) / warps).
 __device__ __forceinline__ int first_tile(int w, int warps, int total) { return (int)((int64_t)total * w / warps); }
 __device__ __forceinline__ int warp_of_tile(int x, int warps, int total) { return (int)(((int64_t)warps * (x + 1) - 1) / total); }
@@ -301,8 +298,6 @@ __global__ void __launch_bounds__(kLineWarps * 32, 1) shared_prefix_attention_ke
 
   launch_next();
   scan_tiles<kLineWarps * 32>(a, cu, warp_sums);
-  if (blockIdx.x == 0)
-    for (int s = threadIdx.x; s <= a.seqs; s += kLineWarps * 32) a.cu[s] = cu[s];
   const AttnLine line(a.seqs, a.kv_heads, a.group, a.prefix_len, kKeys);
   const int total = line.prefix_items * line.prefix_tiles + cu[a.seqs] * line.per_seq;
   const int warps = line_warps((int)gridDim.x * kLineWarps, total);
@@ -317,12 +312,12 @@ __global__ void __launch_bounds__(kLineWarps * 32, 1) shared_prefix_attention_ke
   in.tile = -1;               // no item yet
   int load_at = begin, loads = 0;
   // Pages of a multiple of 16 tokens: a group lies in one page, and lane j holds the id of the page of group ids_from + j
-  // of the item.  Other pages: lane j holds the id of the page of key j & 15 of the group.
+  // of the item.  Other pages: lane j holds the id of the page of key j of the tile.
   const bool whole = a.block.d % 16 == 0;
   int64_t id = -1;
   int ids_from = 0;
   auto fetch_ids = [&](int group) {
-    const int64_t key = whole ? ((int64_t)group + lane) * 16 : (int64_t)group * 16 + (lane & 15);
+    const int64_t key = whole ? ((int64_t)group + lane) * 16 : (int64_t)group * 16 + lane % kKeys;
     id = key < in.len ? load_id(in.table, a.ids_are_int64, in.table_at + a.block.div((uint32_t)key)) : -1;
     ids_from = group;
   };
@@ -377,10 +372,11 @@ __global__ void __launch_bounds__(kLineWarps * 32, 1) shared_prefix_attention_ke
     }
     const int key = key0 + (lane & 15);
     const bool inside = key < in.len;
-    const bool ok = inside && id >= 0 && id < a.num_blocks;
+    const int64_t id_of_key = __shfl_sync(0xffffffffu, id, part * 16 + (lane & 15));
+    const bool ok = inside && id_of_key >= 0 && id_of_key < a.num_blocks;
     if (inside && !ok) raise_status(HFK_DEV_BAD_DEVICE_BLOCK_ID);
     const uint32_t row = ((uint32_t)key - a.block.div((uint32_t)key) * a.block.d) * a.kv_heads + in.h;
-    const int64_t page = ok ? id * a.block_stride : 0;
+    const int64_t page = ok ? id_of_key * a.block_stride : 0;
     const int64_t off = ok ? page + (int64_t)row * kRow : -1;
     if (kCodes) cp_async4(sb, (lane < 16 ? a.k_cache : a.v_cache) + page + a.scales_at + (ok ? (int64_t)row * 4 : 0), ok);
 #pragma unroll 1
@@ -398,10 +394,8 @@ __global__ void __launch_bounds__(kLineWarps * 32, 1) shared_prefix_attention_ke
         uint32_t mask = 0;
         const int group = in.tile * (kKeys / 16);
 #pragma unroll 1
-        for (int part = 0; part < kKeys / 16; ++part) {
-          if (part > 0 && !whole) fetch_ids(group + part);
+        for (int part = 0; part < kKeys / 16; ++part)
           mask |= load_group(group + part, part) << (16 * part);
-        }
         if (lane == 0) ring.valid[load_stage] = mask;
         load_stage = load_stage + 1 == kStages ? 0 : load_stage + 1;
         ++load_at;
@@ -672,25 +666,33 @@ struct JoinArgs {
 };
 
 // kJoinWarps warps a row, each with every kJoinWarps-th part and up to eight loads of a part under way: the parts (some
-// dozens of a row) are in L2, and the time is that of the chain of their loads, so all rows should be at it at once: four
-// warps a row where that fits, else two, else one (2048 rows of 20 parts: 10 us with four, which take two turns).
+// dozens of a row, up to a warp's share of the line each) are in L2, and the time is that of the chain of their loads, so all
+// rows should be at it at once: 16 warps a row where that fits, else four, two, one (2048 rows of 20 parts: 10 us with four,
+// which take two turns, 8.5 with two).
 constexpr int kJoinAhead = 8;
 template <typename T, int D, int kJoinWarps>
-__global__ void __launch_bounds__(kJoinWarps * 32, 28 / kJoinWarps) shared_prefix_join_kernel(const __grid_constant__ JoinArgs args) {
+__global__ void __launch_bounds__(kJoinWarps * 32, kJoinWarps > 14 ? 1 : 28 / kJoinWarps) shared_prefix_join_kernel(const __grid_constant__ JoinArgs args) {
   __shared__ float sums[kJoinWarps][D + 1];
   const AttnArgs &a = args.a;
   const int row = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int q_heads = a.kv_heads * a.group;
   const int s = row / q_heads, head = row - s * q_heads, h = (int)a.per_group.div((uint32_t)head), g = head - h * a.group;
-  launch_wait();
-  // list k: parts first[k] + step[k] i in rows of (m, l) and of o, i < count[k]
+  // list k: parts first[k] + step[k] i in rows of (m, l) and of o, i < count[k].  Their places follow from the lengths alone,
+  // so they are worked out while the kernels that write the parts still run.
   int count[3] = {0, 0, 0};
   int64_t first[3] = {0, 0, 0};
   if (args.warps > 0) {
     const AttnLine line(a.seqs, a.kv_heads, a.group, a.prefix_len, a.tile);
     const int in_prefix = line.prefix_items * line.prefix_tiles;
-    const int before = a.cu[s], behind = a.cu[s + 1];
-    const int total = in_prefix + a.cu[a.seqs] * line.per_seq;
+    int before = 0, all = 0;                     // tiles of the sequences before s, and of all
+    for (int i = lane; i < a.seqs; i += 32) {
+      const int n = (int)((own_length(a, i, false) + a.tile - 1) / a.tile);
+      all += n;
+      before += i < s ? n : 0;
+    }
+    before = __reduce_add_sync(0xffffffffu, before);
+    const int total = in_prefix + __reduce_add_sync(0xffffffffu, all) * line.per_seq;
+    const int tiles_s = (int)((own_length(a, s, false) + a.tile - 1) / a.tile);
     const int warps = line_warps(args.warps, total);
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
@@ -704,7 +706,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32, 28 / kJoinWarps) shared_prefi
       } else {
         const int hg = h * line.own_tiles + g / kItemRows;
         place = g % kItemRows;
-        tiles = behind - before;
+        tiles = tiles_s;
         from = in_prefix + before * line.per_seq + hg * tiles;
         item = line.prefix_items + s * line.per_seq + hg;
       }
@@ -756,6 +758,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32, 28 / kJoinWarps) shared_prefi
       }
     }
   };
+  launch_wait();
   fetch(warp);                // on their way while the maximum is found
   // the largest maximum: every warp looks at all
   float big = -INFINITY;
