@@ -407,7 +407,9 @@ class PagedKVCache:
         runs the kernel: "dst" pulls (peer loads), "src" pushes (peer stores).  The launch goes to the
         current stream of that GPU."""
         assert other.layers == self.layers and other.block_bytes == self.block_bytes
-        assert other.kv_format == self.kv_format and other.page_shape == self.page_shape
+        assert other.kv_format == self.kv_format
+        if self.kv_format != _pkg.capi.HFK_KV_RAW:    # codes and scales lie where the geometry says
+            assert (other.block_size, other.kv_heads, other.head_dim) == (self.block_size, self.kv_heads, self.head_dim)
         dev = other.device if run_on == "dst" else self.device
         key = (id(other), dev)
         cached = getattr(self, "_migrate_tabs", None)

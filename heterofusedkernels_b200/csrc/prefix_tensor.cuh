@@ -639,7 +639,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) prefix_tensor_kernel(const __gr
       tile_max<kFmt>(s_at, sm.sk[mt], scale, top);
       float turn = 1.f;                          // of every row
       if (kWide) {
-        float big = max_nan(max_nan(sm.sv[mt][lane], sm.sv[mt][lane + 32]), max_nan(sm.sv[mt][lane + 64], sm.sv[mt][lane + 96]));
+        float big = max_nan(max_nan(fabsf(sm.sv[mt][lane]), fabsf(sm.sv[mt][lane + 32])), max_nan(fabsf(sm.sv[mt][lane + 64]), fabsf(sm.sv[mt][lane + 96])));
 #pragma unroll
         for (int d = 16; d > 0; d >>= 1) big = max_nan(big, __shfl_xor_sync(0xffffffffu, big, d));
         if (!(big <= 4.f * ref)) {               // also a NaN

@@ -541,7 +541,7 @@ __global__ void __launch_bounds__(kLineWarps * 32, 1) shared_prefix_attention_ke
       float big = 0.f;
       if (kCodes) {
 #pragma unroll
-        for (int n = 0; n < kM; ++n) big = max_nan(big, max_nan(sv[n][0], sv[n][1]));
+        for (int n = 0; n < kM; ++n) big = max_nan(big, max_nan(fabsf(sv[n][0]), fabsf(sv[n][1])));
         move = move || !(big <= 4.f * ref);       // also a NaN
       }
       if (__any_sync(0xffffffffu, move)) {

@@ -353,6 +353,90 @@ def test_shared_prefix_attention(op, cuda_device, fmt, dtype, shape):
     check_attention(c, out, lse)
 
 
+LONG = [
+    # rows on both sides of a tile of 128 and of a block of 256; key tiles on both sides of 128; many tiles for a CTA
+    (1, 8, 128, 16, 2900, [20] * 5), (2, 1, 128, 16, 1157, [3] * 128), (1, 3, 64, 32, 900, [0, 5] * 22), (1, 7, 128, 128, 641, [1] * 37),
+    (1, 2, 128, 16, 128, [0] * 129), (3, 40, 64, 8, 257, [17]), (1, 11, 128, 7, 390, [9, 0, 30, 2]),
+]
+
+
+@pytest.mark.parametrize("fmt", ["raw", "e4m3", "int8"])
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("shape", LONG, ids=[str(i) for i in range(len(LONG))])
+def test_attention_behind_a_longer_prefix(op, cuda_device, fmt, dtype, shape):
+    """More than 32 rows of queries to a K/V head: the tensor-core kernel, with one CTA (every tile of the prefix in one run)
+    and with as many as it likes."""
+    c = attention_case(fmt, dtype, *shape, seed=11)
+    for aiv in (None, 1):
+        out, lse = run_attention(op, c, cuda_device, aiv=aiv)
+        assert status() == 0
+        check_attention(c, out, lse)
+    again, lse_again = run_attention(op, c, cuda_device, aiv=1)
+    assert torch.equal(out, again) and torch.equal(lse, lse_again)
+
+
+@pytest.mark.parametrize("fmt", ["raw", "e4m3"])
+@pytest.mark.parametrize("seqs", [3, 60])
+@pytest.mark.parametrize("scale", [-0.11, 0.0, 3.0])
+def test_attention_with_any_finite_scale(op, cuda_device, fmt, seqs, scale):
+    """Negative scales turn the order of the keys round, 0 makes them equal; keys that do not count stay out."""
+    c = attention_case(fmt, BF16, 1, 4, 128, 16, 133, [7, 0, 20] * (seqs // 3), seed=2, q_gain=0.5)
+    c["scale"] = scale
+    out, lse = run_attention(op, c, cuda_device)
+    check_attention(c, out, lse)
+
+
+@pytest.mark.parametrize("fmt", ["raw", "e4m3", "int8"])
+@pytest.mark.parametrize("seqs", [2, 50])
+def test_attention_bad_prefix_pages_and_rising_maxima(op, cuda_device, fmt, seqs):
+    """Pages that are not there, among them the first tile's whole, and keys whose scores rise from tile to tile, so that the
+    maximum in use has to follow; both ways the prefix is read."""
+    c = attention_case(fmt, BF16, 1, 2, 64, 16, 700, [5] * seqs, seed=6)
+    steep = torch.linspace(0.05, 6, 700)
+    x = torch.randn(700, 1, 64, generator=gen(3)).sign() * steep[:, None, None]
+    at = torch.arange(700)
+    slots = c["prefix_table"][at // 16] * 16 + at % 16
+    o.write(x.to(BF16), c["k"], slots, 16, fmt)
+    c["q"] = (torch.randn(seqs, 2, 64, generator=gen(4)).sign() * 0.7).to(BF16)
+    out, lse = run_attention(op, c, cuda_device)
+    assert status() == 0
+    check_attention(c, out, lse)
+    c["prefix_table"][:8] = -1                                     # keys 0..127
+    c["prefix_table"][20] = 10 ** 6
+    out, lse = run_attention(op, c, cuda_device)
+    assert status() == 0x1
+    check_attention(c, out, lse)
+    c["prefix_table"][:] = -7
+    c["lens"] = torch.zeros(seqs, dtype=torch.int64)
+    out, lse = run_attention(op, c, cuda_device)
+    assert status() == 0x1
+    check_attention(c, out, lse)
+
+
+@pytest.mark.parametrize("seqs", [2, 40])
+def test_attention_queries_of_very_different_magnitude(op, cuda_device, seqs):
+    """bf16 queries over an 8-bit cache become fp16 numbers times a power of two: rows from 1e-30 to 1e30, and zeros."""
+    c = attention_case("e4m3", BF16, 1, 4, 128, 16, 150, [12] * seqs, seed=7)
+    power = torch.linspace(-30, -1, seqs * 4).view(seqs, 4, 1)
+    c["q"] = (torch.randn(seqs, 4, 128, generator=gen(1)) * 10.0 ** power).to(BF16)
+    c["q"][0, 0] = 0
+    out, lse = run_attention(op, c, cuda_device)
+    check_attention(c, out, lse)
+    c["q"] = (torch.randn(seqs, 4, 128, generator=gen(1)).double() * 10.0 ** (power.double() + 31)).to(BF16)
+    c["scale"] = 1e-30
+    out, lse = run_attention(op, c, cuda_device)
+    check_attention(c, out, lse)
+
+
+def test_attention_passes_nan_and_inf_of_queries_on(op, cuda_device):
+    for fmt, seqs in (("raw", 2), ("raw", 40), ("int8", 2), ("int8", 40)):
+        c = attention_case(fmt, BF16, 1, 2, 64, 16, 40, [3] * seqs, seed=1)
+        c["q"][0, 1, 5], c["q"][1, 0, 0] = float("nan"), float("inf")
+        out, _ = run_attention(op, c, cuda_device)
+        assert out[0, 1].isnan().all() and out[1, 0].isnan().all()
+        assert not out[0, 0].isnan().any() and not out[1, 1].isnan().any()
+
+
 @pytest.mark.parametrize("fmt,dtype", [("e4m3", FP16), ("int8", FP16), ("int8", BF16), ("raw", BF16)])
 def test_attention_scales_over_many_orders_of_magnitude(op, cuda_device, fmt, dtype):
     """Rows of the cache whose magnitudes differ by up to 2^20: weight times scale leaves the range of fp16 that is held with full precision."""
@@ -463,6 +547,42 @@ def test_calls_on_several_streams_and_replayed_graphs(op, cuda_device):
     assert status() == 0
 
 
+def test_a_captured_call_with_a_shared_prefix_replays(op, cuda_device):
+    """The three dependent launches (prefix, own tokens, join) in a graph, two graphs replayed in turn and on two streams."""
+    graphs = []
+    for seed in (1, 2):
+        c = attention_case("e4m3", BF16, 2, 4, 128, 16, 600, [30, 0, 77] * 5, seed=seed)
+        d = {n: c[n].to(cuda_device) for n in ("q", "k", "v", "prefix_table", "tables", "lens")}
+        out, lse = torch.empty_like(d["q"]), torch.empty(d["q"].shape[:2], device=cuda_device)
+
+        def call(c=c, d=d, out=out, lse=lse):
+            op.shared_prefix_attention(d["q"], out, d["k"], d["v"], d["prefix_table"], 600, d["tables"], d["lens"], 16, 2, 1, c["scale"], lse)
+
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            call()
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            call()
+        graphs.append((c, d, out, lse, graph))
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for turn in range(3):
+        for i, (c, d, out, lse, graph) in enumerate(graphs):
+            c["q"] = torch.randn(15, 8, 128, generator=gen(50 + turn + 10 * i)).to(BF16)
+            d["q"].copy_(c["q"])
+            out.zero_()
+        torch.cuda.synchronize()
+        for (c, d, out, lse, graph), s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                graph.replay()
+        torch.cuda.synchronize()
+        for c, d, out, lse, graph in graphs:
+            check_attention(c, out, lse)
+    assert status() == 0
+
+
 # ------------------------------------------------------------- used together ---
 @pytest.mark.parametrize("fmt", ["e4m3", "int8"])
 @pytest.mark.parametrize("mover", [None, 1, 2, "staged"])
@@ -508,6 +628,35 @@ def test_an_8_bit_cache_through_prompt_swap_and_decoding(op, cuda_device, fmt, m
         c = dict(fmt=fmt, q=q.cpu(), k=cache.k_caches[layer].cpu(), v=cache.v_caches[layer].cpu(), prefix_table=front, prefix=prompt,
                  tables=own, lens=torch.tensor([17, 17]), block=block, heads=heads, dim=dim, scale=dim ** -0.5)
         check_attention(c, out, lse)
+    assert cache.status() == 0
+
+
+def test_an_8_bit_cache_in_the_layer_wise_pipeline_and_migration(op, cuda_device):
+    from heterofusedkernels_b200.connector import LayerwisePrefetcher, QuantizedPagedKVCache
+
+    cache = QuantizedPagedKVCache(3, 16, 16, 4, 64, "int8", cuda_device, host_slots=24, pool_layout="layer_major", dtype=FP32)
+    other = QuantizedPagedKVCache(3, 20, 16, 4, 64, "int8", cuda_device, dtype=FP32)
+    for t in other.k_caches + other.v_caches:
+        t.zero_()
+    x = torch.randn(3, 100, 2, 4, 64, generator=gen(1)).to(BF16).to(cuda_device)
+    for layer in range(3):
+        cache.write(layer, x[layer, :, 0], x[layer, :, 1], torch.arange(100, device=cuda_device))
+    want = cache.paged_gather(torch.arange(7)[None], torch.tensor([100]))
+    assert want[0].dtype == FP32
+    ids, slots = torch.arange(7, device=cuda_device), torch.arange(3, 10, device=cuda_device)
+    pipe = LayerwisePrefetcher(cache)
+    pipe.evict((0, 3), ids, slots)
+    pipe.quiesce()
+    pipe.prefetch((0, 3), ids + 8, slots)
+    pipe.quiesce()
+    cache.migrate_to(other, ids + 8, ids + 11)
+    for where, first in ((cache, 8), (other, 11)):
+        got = where.paged_gather(torch.arange(first, first + 7)[None], torch.tensor([100]))
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    with pytest.raises(AssertionError):
+        cache.migrate_to(QuantizedPagedKVCache(3, 4, 16, 4, 64, "e4m3", cuda_device), ids[:1], ids[:1])
+    with pytest.raises(ValueError, match="mover"):
+        cache.paged_gather(torch.arange(7)[None], torch.tensor([100]), mover=1)
     assert cache.status() == 0
 
 
