@@ -13,6 +13,12 @@
 // in its softmax, the tensor cores work on the other: per 128 keys and tile, at head_dim 128, both products take about
 // 1024 clocks of the tensor cores and the 128 x 128 exponentials 1024 clocks of the special function units.
 //
+// Measured: 8 items of 256 rows against 32768 keys, e4m3 (34 GFLOP): 57 us, of which 12 pass before the first tile's
+// scores and behind the last one's, 33 with the softmax left out (a tile's two products take 1450 clocks, the operands
+// from shared memory being at its bandwidth), the rest is softmax that nothing hides.  Steps to there: 105 us at first;
+// 92 with the queries loaded a row's worth at a time and the parts' rows leaving as bulk copies; 64 with packed fp32
+// arithmetic; 57 with short loops instead of unrolled ones (warps waited for instructions) and four rows a thread.
+//
 // o is rescaled only where a row's maximum rises by more than 2^8 above the one in use: weights up to 2^8 are as
 // exact as weights up to 1, and l and o stay in the same units, so nothing is lost.
 //

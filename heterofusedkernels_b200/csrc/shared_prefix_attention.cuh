@@ -275,7 +275,9 @@ struct alignas(128) LineRing {
 // a row where the operand layout would have it take two, and V needs no transposition: a lane that holds the same
 // columns of four rows packs its operands with byte permutations.
 //
-// Bound by HBM for long sequences; for short ones by the chain from a sequence's length over its page ids to its rows.
+// Bound by HBM for long sequences: 8 of 16384 to 131072 tokens, 8 heads of 128, bf16 (2.4 GB) 355 to 375 us, 6.4 to 6.8 TB/s;
+// for short ones by the chain from a sequence's length over its page ids to its rows (about 5 us), and of 8-bit caches by
+// what eight warps an SM can hide of a tile's latencies (50 MB 18 us).
 template <typename T, int kFmt, int D>
 __global__ void __launch_bounds__(kLineWarps * 32, 1) shared_prefix_attention_kernel(const __grid_constant__ AttnArgs a) {
   using Ring = LineRing<kFmt, D>;
