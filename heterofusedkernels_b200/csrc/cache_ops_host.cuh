@@ -55,25 +55,27 @@ static int validate_written(const char *op, const char *name, const hfk_rows &r,
 }
 
 // ---- writing ------------------------------------------------------------------------------------------------
-template <typename T, int kFmt, bool kRope, int kLanes>
+template <typename T, int kFmt, bool kRope, int kLanes, int kUnits>
 static cudaError_t launch_kv_write(const KvWriteArgs &a, cudaStream_t stream) {
   constexpr int kThreads = 128, kGroups = kThreads / kLanes;
-  kv_write_kernel<T, kFmt, kRope, kLanes, kThreads><<<(a.rows + kGroups - 1) / kGroups, kThreads, 0, stream>>>(a);
+  kv_write_kernel<T, kFmt, kRope, kLanes, kUnits, kThreads><<<(a.rows + kGroups - 1) / kGroups, kThreads, 0, stream>>>(a);
   return cudaGetLastError();
 }
-
-template <typename T, bool kRope, int kLanes>
+template <typename T, bool kRope, int kLanes, int kUnits>
 static cudaError_t launch_kv_write(const KvWriteArgs &a, int fmt, cudaStream_t s) {
-  if (fmt == HFK_KV_E4M3) return launch_kv_write<T, kFmtE4m3, kRope, kLanes>(a, s);
-  if (fmt == HFK_KV_INT8) return launch_kv_write<T, kFmtInt8, kRope, kLanes>(a, s);
-  return launch_kv_write<T, kFmtRaw, kRope, kLanes>(a, s);
+  if (fmt == HFK_KV_E4M3) return launch_kv_write<T, kFmtE4m3, kRope, kLanes, kUnits>(a, s);
+  if (fmt == HFK_KV_INT8) return launch_kv_write<T, kFmtInt8, kRope, kLanes, kUnits>(a, s);
+  return launch_kv_write<T, kFmtRaw, kRope, kLanes, kUnits>(a, s);
 }
-
+template <typename T, bool kRope, int kUnits>
+static cudaError_t launch_kv_write(const KvWriteArgs &a, int fmt, cudaStream_t s) {
+  if (a.head_dim <= 64) return launch_kv_write<T, kRope, 4 / kUnits, kUnits>(a, fmt, s);
+  if (a.head_dim <= 128) return launch_kv_write<T, kRope, 8 / kUnits, kUnits>(a, fmt, s);
+  return launch_kv_write<T, kRope, 16 / kUnits, kUnits>(a, fmt, s);
+}
 template <typename T, bool kRope>
 static cudaError_t launch_kv_write(const KvWriteArgs &a, int fmt, cudaStream_t s) {
-  if (a.head_dim <= 64) return launch_kv_write<T, kRope, 4>(a, fmt, s);
-  if (a.head_dim <= 128) return launch_kv_write<T, kRope, 8>(a, fmt, s);
-  return launch_kv_write<T, kRope, 16>(a, fmt, s);
+  return a.rows < kWriteWideRows ? launch_kv_write<T, kRope, 1>(a, fmt, s) : launch_kv_write<T, kRope, 2>(a, fmt, s);
 }
 
 static int kv_write_impl(const char *op, const hfk_kv_write_desc *d, const hfk_norm_rope_desc *n, bool rope, cudaStream_t stream) {

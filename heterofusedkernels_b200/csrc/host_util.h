@@ -50,6 +50,10 @@ constexpr int kDefaultStagedLanes = 1;
 constexpr long long kStagedMaxCopyBytes = 64ll << 20;
 // Block migration: 512-thread CTAs per SM (peer loads over NVLink need megabytes in flight).
 constexpr int kMigrateCtasPerSm = 2;
+// kv_write: rows from which a lane takes 32 elements of a row, not 16.  16 finish sooner while every warp is resident and a
+// call lasts as long as one row's chain, 32 take fewer instructions.  Rotated, 48 rows a token, e4m3: 2.42 us with 16 and 2.74
+// with 32 for one token, 3.53 and 3.76 for 256, 5.03 and 4.50 for 512, 13.7 and 12.4 for 2048.
+constexpr unsigned kWriteWideRows = 1u << 14;
 // Reading an 8-bit cache back: 256-thread CTAs per SM, eight 8-byte loads a lane in flight.  6.9 GB (64 sequences, 4 layers):
 // 1113 us with 2, 1186 with 4, 1157 with 8 and half the loads a lane.
 constexpr int kGatherDequantCtasPerSm = 2;

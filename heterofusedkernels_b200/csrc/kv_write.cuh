@@ -39,23 +39,28 @@ struct KvWriteArgs {
 };
 
 
-// Two blocks of eight elements of a row to each of kLanes lanes (kLanes * 16 >= head_dim).  Where pairs (i, i + rot/2) are
-// rotated, lane j < rot/16 holds blocks j and j + rot/16, so that either partner is its own; other lanes hold neighbours.
-// Consecutive groups of lanes take consecutive heads of a token, so that loads, stores and the 4-byte scales of
-// neighbours fall into the same lines.
+// A row goes to kLanes lanes by units of two blocks of eight elements, kUnits to a lane (kLanes * kUnits * 16 >= head_dim).
+// Where pairs (i, i + rot/2) are rotated, unit q < rot/16 is blocks q and q + rot/16, so that a lane has either partner;
+// other units are neighbouring blocks.  Consecutive groups of lanes take consecutive heads of a token, so that loads, stores
+// and the 4-byte scales of neighbours fall into the same lines.
 //
-// Measured: 65536 tokens of 8 heads of 128, fp16 to int8 (407 MB): 102 us with one block a lane (the arithmetic on addresses
-// took as long as the data), 70 with two; 16384 tokens with rotation of 40 heads, fp16 to e4m3 (379 MB): 135 and 80 us.  Two
-// or four rows a thread were slower (85 and 172 us there): what helps is that many warps fit, so CTAs are of 128 threads
-// and the kernel without rotation is held to 32 registers.
-template <typename T, int kFmt, bool kRope, int kLanes, int kThreads>
-__global__ void __launch_bounds__(kThreads, kRope ? 1 : 16) kv_write_kernel(const __grid_constant__ KvWriteArgs a) {
+// HBM bounds the bytes, and close behind it the instructions: those for a row's addresses and its scale are the same
+// however many elements a lane has.  Measured: 65536 tokens of 8 heads of 128, fp16 to int8 (407 MB): 102 us with 8 elements a
+// lane, 70 with 16, 65 with 32; 16384 tokens with rotation of 40 heads, fp16 to e4m3 (379 MB): 135, 80 and 77 us.  Two or four
+// rows a thread were slower (85 and 172 us there), and so were CTAs of 256 threads (70 and 81 us with 32 elements).  Few
+// rows take one unit a lane (kWriteWideRows); without rotation that form is held to 32 registers, so that all warps fit.
+template <typename T, int kFmt, bool kRope, int kLanes, int kUnits, int kThreads>
+__global__ void __launch_bounds__(kThreads, kRope || kUnits > 1 ? 1 : 16) kv_write_kernel(const __grid_constant__ KvWriteArgs a) {
   constexpr int kGroups = kThreads / kLanes;
   const int lane = threadIdx.x % kLanes;
   const uint32_t r = blockIdx.x * (uint32_t)kGroups + threadIdx.x / kLanes;
-  const bool inside = lane * 16 < a.head_dim;
-  const int pairs = kRope && !a.interleaved ? a.rot >> 4 : 0;       // lanes with blocks rot/2 apart
-  const int block[2] = {lane < pairs ? lane : 2 * lane, lane < pairs ? lane + pairs : 2 * lane + 1};
+  const int pairs = kRope && !a.interleaved ? a.rot >> 4 : 0;       // units of blocks rot/2 apart
+  auto unit = [&](int u) { return lane + kLanes * u; };
+  auto inside = [&](int u) { return unit(u) * 16 < a.head_dim; };
+  auto block = [&](int u, int b) {
+    const int q = unit(u);
+    return q < pairs ? q + b * pairs : 2 * q + b;
+  };
 
   bool live = r < a.rows;
   const uint32_t token = a.per_token.div(live ? r : 0);
@@ -67,12 +72,14 @@ __global__ void __launch_bounds__(kThreads, kRope ? 1 : 16) kv_write_kernel(cons
   const unsigned char *src = is_q   ? a.q + token * a.q_token + h * a.q_head
                              : is_v ? a.v + token * a.v_token + kv_head * a.v_head
                                     : a.k + token * a.k_token + kv_head * a.k_head;
-  uint4 in[2];
+  uint4 in[kUnits][2];
 #pragma unroll
-  for (int b = 0; b < 2; ++b) {
-    in[b] = make_uint4(0, 0, 0, 0);
-    if (inside && live) in[b] = *reinterpret_cast<const uint4 *>(src + block[b] * 16);
-  }
+  for (int u = 0; u < kUnits; ++u)
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      in[u][b] = make_uint4(0, 0, 0, 0);
+      if (live && inside(u)) in[u][b] = *reinterpret_cast<const uint4 *>(src + block(u, b) * 16);
+    }
   // a negative slot is padding: nothing of the token is written
   if (live && slot >= a.num_slots) {
     raise_status(HFK_DEV_BAD_DEVICE_BLOCK_ID);
@@ -92,106 +99,124 @@ __global__ void __launch_bounds__(kThreads, kRope ? 1 : 16) kv_write_kernel(cons
   }
 
   if constexpr (!kRope && kFmt == kFmtRaw) {
-    if (live && inside) {
-      unsigned char *dst = page + (int64_t)place * a.head_dim * 2;
-      *reinterpret_cast<uint4 *>(dst + block[0] * 16) = in[0];
-      *reinterpret_cast<uint4 *>(dst + block[1] * 16) = in[1];
-    }
-  } else {
-  float x[2][8];
+    if (!live) return;
+    unsigned char *dst = page + (int64_t)place * a.head_dim * 2;
 #pragma unroll
-  for (int b = 0; b < 2; ++b) {
-    const uint32_t w[4] = {in[b].x, in[b].y, in[b].z, in[b].w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 f = Pair<T>::unpack(w[i]);
-      x[b][2 * i] = f.x;
-      x[b][2 * i + 1] = f.y;
-    }
-  }
-
-  if constexpr (kRope) {
-    const void *weight = is_q ? a.q_weight : (is_v ? nullptr : a.k_weight);
-    if (a.q_weight != nullptr || a.k_weight != nullptr) {
-      float sum = 0.f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) sum = fmaf(x[0][i], x[0][i], fmaf(x[1][i], x[1][i], sum));
-#pragma unroll
-      for (int d = kLanes / 2; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d, kLanes);
-      if (weight != nullptr && inside) {
-        const float scale = rsqrtf(sum / (float)a.head_dim + a.eps);
-#pragma unroll
-        for (int b = 0; b < 2; ++b) {
-          const uint4 g = *reinterpret_cast<const uint4 *>(static_cast<const unsigned char *>(weight) + block[b] * 16);
-          const uint32_t gw[4] = {g.x, g.y, g.z, g.w};
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float2 f = Pair<T>::unpack(gw[i]);
-            x[b][2 * i] = x[b][2 * i] * scale * f.x;
-            x[b][2 * i + 1] = x[b][2 * i + 1] * scale * f.y;
-          }
-        }
+    for (int u = 0; u < kUnits; ++u)
+      if (inside(u)) {
+        *reinterpret_cast<uint4 *>(dst + block(u, 0) * 16) = in[u][0];
+        *reinterpret_cast<uint4 *>(dst + block(u, 1) * 16) = in[u][1];
       }
-    }
-    if (live && !is_v && lane * 16 < a.rot) {
-      // eight pairs of the lane, of its two blocks or neighbours inside them; four at a time
-      const float *cp = a.cos_sin + position * a.rot + lane * 8, *sp = cp + a.rot / 2;
+  } else {
+    float x[kUnits][2][8];
 #pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        const float4 c4 = *reinterpret_cast<const float4 *>(cp + 4 * q), s4 = *reinterpret_cast<const float4 *>(sp + 4 * q);
-        const float c[4] = {c4.x, c4.y, c4.z, c4.w}, s[4] = {s4.x, s4.y, s4.z, s4.w};
+    for (int u = 0; u < kUnits; ++u)
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        const uint32_t w[4] = {in[u][b].x, in[u][b].y, in[u][b].z, in[u][b].w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          if (a.interleaved) {
-            const float lo = x[q][2 * i], hi = x[q][2 * i + 1];
-            x[q][2 * i] = lo * c[i] - hi * s[i];
-            x[q][2 * i + 1] = hi * c[i] + lo * s[i];
-          } else {
-            const float lo = x[0][4 * q + i], hi = x[1][4 * q + i];
-            x[0][4 * q + i] = lo * c[i] - hi * s[i];
-            x[1][4 * q + i] = hi * c[i] + lo * s[i];
+          const float2 f = Pair<T>::unpack(w[i]);
+          x[u][b][2 * i] = f.x;
+          x[u][b][2 * i + 1] = f.y;
+        }
+      }
+
+    if constexpr (kRope) {
+      const void *weight = is_q ? a.q_weight : (is_v ? nullptr : a.k_weight);
+      if (a.q_weight != nullptr || a.k_weight != nullptr) {
+        float sum = 0.f;
+#pragma unroll
+        for (int u = 0; u < kUnits; ++u)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) sum = fmaf(x[u][0][i], x[u][0][i], fmaf(x[u][1][i], x[u][1][i], sum));
+#pragma unroll
+        for (int d = kLanes / 2; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d, kLanes);
+        if (weight != nullptr) {
+          const float scale = rsqrtf(sum / (float)a.head_dim + a.eps);
+#pragma unroll
+          for (int u = 0; u < kUnits; ++u)
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+              if (!inside(u)) continue;
+              const uint4 g = *reinterpret_cast<const uint4 *>(static_cast<const unsigned char *>(weight) + block(u, b) * 16);
+              const uint32_t gw[4] = {g.x, g.y, g.z, g.w};
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const float2 f = Pair<T>::unpack(gw[i]);
+                x[u][b][2 * i] = x[u][b][2 * i] * scale * f.x;
+                x[u][b][2 * i + 1] = x[u][b][2 * i + 1] * scale * f.y;
+              }
+            }
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < kUnits; ++u) {
+        if (!live || is_v || unit(u) * 16 >= a.rot) continue;
+        // eight pairs of the unit, of its two blocks or neighbours inside them; four at a time
+        const float *cp = a.cos_sin + position * a.rot + unit(u) * 8, *sp = cp + a.rot / 2;
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          const float4 c4 = *reinterpret_cast<const float4 *>(cp + 4 * q), s4 = *reinterpret_cast<const float4 *>(sp + 4 * q);
+          const float c[4] = {c4.x, c4.y, c4.z, c4.w}, s[4] = {s4.x, s4.y, s4.z, s4.w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if (a.interleaved) {
+              const float lo = x[u][q][2 * i], hi = x[u][q][2 * i + 1];
+              x[u][q][2 * i] = lo * c[i] - hi * s[i];
+              x[u][q][2 * i + 1] = hi * c[i] + lo * s[i];
+            } else {
+              const float lo = x[u][0][4 * q + i], hi = x[u][1][4 * q + i];
+              x[u][0][4 * q + i] = lo * c[i] - hi * s[i];
+              x[u][1][4 * q + i] = hi * c[i] + lo * s[i];
+            }
           }
         }
       }
     }
-  }
 
-  if (kFmt == kFmtRaw || is_q) {
-    if (live && inside) {
-      unsigned char *dst = is_q ? a.q_out + token * a.qo_token + h * a.qo_head : page + (int64_t)place * a.head_dim * 2;
+    if (kFmt == kFmtRaw || is_q) {
+      if (live) {
+        unsigned char *dst = is_q ? a.q_out + token * a.qo_token + h * a.qo_head : page + (int64_t)place * a.head_dim * 2;
 #pragma unroll
-      for (int b = 0; b < 2; ++b)
-        *reinterpret_cast<uint4 *>(dst + block[b] * 16) =
-            make_uint4(Pair<T>::pack(x[b][0], x[b][1]), Pair<T>::pack(x[b][2], x[b][3]), Pair<T>::pack(x[b][4], x[b][5]),
-                       Pair<T>::pack(x[b][6], x[b][7]));
+        for (int u = 0; u < kUnits; ++u)
+#pragma unroll
+          for (int b = 0; b < 2; ++b)
+            if (inside(u))
+              *reinterpret_cast<uint4 *>(dst + block(u, b) * 16) =
+                  make_uint4(Pair<T>::pack(x[u][b][0], x[u][b][1]), Pair<T>::pack(x[u][b][2], x[u][b][3]),
+                             Pair<T>::pack(x[u][b][4], x[u][b][5]), Pair<T>::pack(x[u][b][6], x[u][b][7]));
+      }
     }
-  }
-  if constexpr (kFmt != kFmtRaw) {
-    if (__all_sync(0xffffffffu, is_q)) return;   // the other lanes of a warp may hold keys or values
-    float top = 0.f;
+    if constexpr (kFmt != kFmtRaw) {
+      if (__all_sync(0xffffffffu, is_q)) return;   // the other lanes of a warp may hold keys or values
+      float top = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) top = max_nan(max_nan(top, fabsf(x[0][i])), fabsf(x[1][i]));
+      for (int u = 0; u < kUnits; ++u)
 #pragma unroll
-    for (int d = kLanes / 2; d > 0; d >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, d, kLanes));
-    float scale = __fmul_rn(top, 1.f / top_code<kFmt>());
-    if (scale < kLeastScale) scale = kLeastScale;  // a NaN stays
-    if (scale > 3.4e38f) scale = __uint_as_float(0x7fffffffu);  // an infinity in the row: no code stands for its parts
-    const float inv = __frcp_rn(scale);
-    if (live && !is_q) {
-      if (inside) {
+        for (int i = 0; i < 8; ++i) top = max_nan(max_nan(top, fabsf(x[u][0][i])), fabsf(x[u][1][i]));
+#pragma unroll
+      for (int d = kLanes / 2; d > 0; d >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, d, kLanes));
+      float scale = __fmul_rn(top, 1.f / top_code<kFmt>());
+      if (scale < kLeastScale) scale = kLeastScale;  // a NaN stays
+      if (scale > 3.4e38f) scale = __uint_as_float(0x7fffffffu);  // an infinity in the row: no code stands for its parts
+      const float inv = __frcp_rn(scale);
+      if (live && !is_q) {
         unsigned char *dst = page + (int64_t)place * a.head_dim;
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
-          float y[8];
+        for (int u = 0; u < kUnits; ++u)
 #pragma unroll
-          for (int i = 0; i < 8; ++i) y[i] = __fmul_rn(x[b][i], inv);
-          *reinterpret_cast<uint2 *>(dst + block[b] * 8) =
-              make_uint2(float_to_codes<kFmt>(y[0], y[1], y[2], y[3]), float_to_codes<kFmt>(y[4], y[5], y[6], y[7]));
-        }
+          for (int b = 0; b < 2; ++b) {
+            float y[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) y[i] = __fmul_rn(x[u][b][i], inv);
+            if (inside(u))
+              *reinterpret_cast<uint2 *>(dst + block(u, b) * 8) =
+                  make_uint2(float_to_codes<kFmt>(y[0], y[1], y[2], y[3]), float_to_codes<kFmt>(y[4], y[5], y[6], y[7]));
+          }
+        if (lane == 0) reinterpret_cast<float *>(page + a.scales_at)[place] = scale;
       }
-      if (lane == 0) reinterpret_cast<float *>(page + a.scales_at)[place] = scale;
     }
-  }
   }
 }
 

@@ -83,6 +83,13 @@ def test_kv_write_is_bit_exact(op, cuda_device, fmt, dtype, tokens, heads, dim, 
     assert status() == 0
 
 
+@pytest.mark.parametrize("fmt", ["raw", "e4m3", "int8"])
+@pytest.mark.parametrize("dtype,tokens,heads,dim,block", [(BF16, 8200, 1, 128, 16), (FP16, 1030, 8, 64, 16), (BF16, 2800, 3, 48, 8),
+                                                          (FP16, 1700, 5, 256, 7), (BF16, 9000, 1, 16, 16), (FP16, 1400, 6, 112, 32)])
+def test_kv_write_of_many_rows_is_bit_exact(op, cuda_device, fmt, dtype, tokens, heads, dim, block):
+    test_kv_write_is_bit_exact(op, cuda_device, fmt, dtype, tokens, heads, dim, block)
+
+
 def test_kv_write_rows_with_inf_or_nan_read_back_as_nan(op, cuda_device):
     for fmt in ("e4m3", "int8"):
         x = torch.ones(3, 2, 64, dtype=BF16)
@@ -186,6 +193,15 @@ def test_qk_norm_rope_write(op, cuda_device, fmt, dtype, tokens, heads, group, d
     # in place
     op.qk_norm_rope_write(dq, dk, dv, dq, kc, vc, up(slots), up(positions), up(table), block, FMT[fmt], up(wq), up(wk), eps, interleaved)
     assert torch.equal(dq[live.to(cuda_device)], out[live.to(cuda_device)])
+
+
+@pytest.mark.parametrize("fmt", ["raw", "e4m3", "int8"])
+@pytest.mark.parametrize("dtype,tokens,heads,group,dim,rot,interleaved,norm", [
+    (BF16, 1400, 2, 4, 128, 128, False, "qk"), (FP16, 1000, 2, 7, 128, 64, True, "qk"), (BF16, 5500, 1, 1, 64, 64, False, ""),
+    (FP16, 1400, 3, 2, 96, 96, False, "k"), (BF16, 1700, 2, 3, 256, 32, True, "q"), (FP16, 1700, 1, 8, 48, 16, False, "qk"),
+    (BF16, 2100, 2, 2, 80, 48, False, "qk"), (BF16, 2100, 2, 2, 128, 0, False, "qk"), (FP16, 2100, 2, 2, 16, 16, False, "qk")])
+def test_qk_norm_rope_write_of_many_rows(op, cuda_device, fmt, dtype, tokens, heads, group, dim, rot, interleaved, norm):
+    test_qk_norm_rope_write(op, cuda_device, fmt, dtype, tokens, heads, group, dim, rot, interleaved, norm)
 
 
 def test_norm_rope_position_outside_the_table_is_skipped_and_reported(op, cuda_device):
