@@ -47,6 +47,9 @@ def values(pages, block_size, heads, dim, fmt):
 def write(rows, pages, slots, block_size, fmt):
     """In place; rows [tokens, heads, dim]."""
     heads, dim = rows.shape[1:]
+    if fmt != "raw":
+        codes, scales = split_pages(pages, block_size, heads, dim, fmt)
+        row_codes, row_scales = encode(rows, fmt)
     for t, slot in enumerate(slots.tolist()):
         if slot < 0 or slot >= pages.shape[0] * block_size:
             continue
@@ -54,10 +57,8 @@ def write(rows, pages, slots, block_size, fmt):
         if fmt == "raw":
             pages[b, at] = rows[t]
         else:
-            codes, scales = split_pages(pages, block_size, heads, dim, fmt)
-            c, s = encode(rows[t], fmt)
-            codes.view(torch.uint8)[b, at] = c.view(torch.uint8)
-            scales[b, at] = s
+            codes.view(torch.uint8)[b, at] = row_codes.view(torch.uint8)[t]
+            scales[b, at] = row_scales[t]
     return pages
 
 
@@ -68,12 +69,12 @@ def norm_rope(x, positions, cos_sin, weight, eps, interleaved):
         x = x / (x.square().mean(-1, keepdim=True) + eps).sqrt() * weight.double()
     half = cos_sin.shape[1] // 2
     out = x.clone()
+    i = torch.arange(half)
+    a, b = (2 * i, 2 * i + 1) if interleaved else (i, i + half)
     for t, p in enumerate(positions.tolist()):
-        for i in range(half):
-            c, s = float(cos_sin[p, i]), float(cos_sin[p, half + i])
-            a, b = (2 * i, 2 * i + 1) if interleaved else (i, i + half)
-            out[t, :, a] = x[t, :, a] * c - x[t, :, b] * s
-            out[t, :, b] = x[t, :, b] * c + x[t, :, a] * s
+        c, s = cos_sin[p, :half].double(), cos_sin[p, half:].double()
+        out[t, :, a] = x[t, :, a] * c - x[t, :, b] * s
+        out[t, :, b] = x[t, :, b] * c + x[t, :, a] * s
     return out
 
 
