@@ -573,7 +573,7 @@ void paged_gather_dequant(const at::Tensor &kLayerPtrs, const at::Tensor &vLayer
   d.ids_are_int64 = blockTables.scalar_type() == at::kLong ? 1 : 0;
   d.num_seqs = blockTables.size(0);
   d.max_blocks_per_seq = blockTables.size(1);
-  d.block_table_stride = std::max(blockTables.stride(0), blockTables.size(1));
+  d.block_table_stride = blockTables.size(0) > 1 ? blockTables.stride(0) : blockTables.size(1);  // one row has no stride that matters
   d.block_size = blockSize;
   d.device_block_stride = deviceBlockStride.has_value()
                               ? deviceBlockStride.value()

@@ -715,7 +715,8 @@ def test_refusals_on_the_device(op, cuda_device):
     op.shared_prefix_attention(*good)
     for i, bad, text in [(5, 33, "needs 3"), (9, 3, "multiple of kvHeads"), (0, z(2, 4, 96), "out must have"), (4, pre.int(), "same dtype"),
                          (7, lens[:1], "num_seqs"), (8, 8, "blockSize"), (3, cache[:2], "same shape"), (6, tab.t(), "num_seqs"),
-                         (1, z(2, 1, 64).expand(2, 4, 64), "overlap"), (5, -1, "negative")]:
+                         (1, z(2, 1, 64).expand(2, 4, 64), "overlap"), (5, -1, "negative"),
+                         (6, tab[:1].expand(2, 1), "block_table_stride")]:
         args = list(good)
         args[i] = bad
         with pytest.raises(RuntimeError, match=text):
@@ -745,7 +746,8 @@ def test_refusals_on_the_device(op, cuda_device):
     out = torch.zeros(1, 16, 2, 64, device=cuda_device)
     ptr = torch.tensor([page.data_ptr()], device=cuda_device)
     for args, text in [((ptr, ptr, out, out, tab, lens, 16, 3, 0), "paged_gather reads"), ((ptr, ptr, out.double(), out.double(), tab, lens, 16, 3, 1), "float32"),
-                       ((ptr, ptr, out, out, tab, lens, 16, 3, 1, 1024), "smaller than one"), ((ptr, ptr, out, out, tab, lens.int(), 16, 3, 1), "same dtype")]:
+                       ((ptr, ptr, out, out, tab, lens, 16, 3, 1, 1024), "smaller than one"), ((ptr, ptr, out, out, tab, lens.int(), 16, 3, 1), "same dtype"),
+                       ((ptr, ptr, out, out, tab[:1].expand(3, tab.shape[1]), lens[:1].repeat(3), 16, 3, 1), "block_table_stride")]:
         with pytest.raises(RuntimeError, match=text):
             op.paged_gather_dequant(*args)
     torch.cuda.synchronize()
