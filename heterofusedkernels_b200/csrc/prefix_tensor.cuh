@@ -42,6 +42,7 @@ struct PrefixTensorArgs {
 };
 
 constexpr int kPtThreads = 512, kPtRows = 128, kPtKeys = 128, kPtStages = 4, kPtMeta = 4;
+constexpr int kSameScale = 10, kSharedBack = 40;   // powers of two, of bf16 queries that become fp16 numbers
 
 template <int D>
 struct PrefixSmem {
@@ -56,8 +57,8 @@ struct PrefixSmem {
   uint64_t full[kPtStages], empty[kPtStages], meta[kPtMeta], s_full[2], p_full[2], o_full, q_full;
   uint32_t tmem;
   int failed;
-  uint32_t q_top;                                // bits of the largest finite |query|
-  float q_back;                                  // what undoes the queries' scaling
+  uint32_t q_top, q_low;                         // bits of the largest finite |query| of any row, and of the row whose is least
+  float q_back;                                  // what undoes the queries' scaling, the part that all rows share
 };
 static_assert(256 * (128 * 4 + 16) <= 2 * PrefixSmem<128>::kTile + kPtStages * PrefixSmem<128>::kTile, "o fits");
 static_assert(256 * (64 * 4 + 16) <= 2 * PrefixSmem<64>::kTile + kPtStages * PrefixSmem<64>::kTile, "o fits");
@@ -191,10 +192,10 @@ __device__ __forceinline__ void rescale(uint32_t o_at, float factor) {
   }
 }
 
-// Scores of keys that do not count become -inf (the last tile of the prefix, pages that are not there), so that
-// what follows needs one form only: every copy of the code below costs instruction cache, and the kernel waited for
-// instructions when it had four.
-__device__ __forceinline__ void mask_scores(uint32_t s_at, const uint32_t *valid) {
+// Scores of keys that do not count become -inf (the last tile of the prefix, pages that are not there), and the others are
+// multiplied by a factor of the row (1 but for queries of mixed magnitudes), so that what follows needs one form only:
+// every copy of the code below costs instruction cache, and the kernel waited for instructions when it had four.
+__device__ __forceinline__ void amend_scores(uint32_t s_at, const uint32_t *valid, float factor) {
 #pragma unroll 1
   for (int c = 0; c < 4; ++c) {
     uint32_t s[32];
@@ -202,8 +203,7 @@ __device__ __forceinline__ void mask_scores(uint32_t s_at, const uint32_t *valid
     tc_wait_load();
     const uint32_t bits = valid[c];
 #pragma unroll
-    for (int e = 0; e < 32; ++e)
-      if (!(bits >> e & 1)) s[e] = 0xff800000u;
+    for (int e = 0; e < 32; ++e) s[e] = bits >> e & 1 ? __float_as_uint(__uint_as_float(s[e]) * factor) : 0xff800000u;
     tc_store32(s_at + c * 32, s);
   }
   tc_wait_store();
@@ -345,6 +345,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) prefix_tensor_kernel(const __gr
     mbar_init(&sm.q_full, tiles * 128);
     sm.failed = 0;
     sm.q_top = 0;
+    sm.q_low = 0xffffffffu;
     sm.q_back = 1.f;
     mbar_fence_init();
   }
@@ -596,7 +597,8 @@ __global__ void __launch_bounds__(kPtThreads, 1) prefix_tensor_kernel(const __gr
     constexpr float kLeastRef = 7.9e-31f;        // 2^-100: its reciprocal times 2^8 and many keys is finite
     float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, l[4] = {0.f, 0.f, 0.f, 0.f}, ref = kLeastRef, log_ref = kWide ? -100.f : 0.f;
     const float scale = a.scale_log2 == 0.f ? kLeastScale : a.scale_log2;   // 0 times the -inf of a masked key is NaN
-    bool ok = true;
+    bool ok = true, mixed = false;
+    float row_back = 1.f;                        // of row `lane`: what undoes its own part of the queries' scaling
     {                                            // this warp's 32 rows of queries, zero behind the last one
       constexpr int kChunks = D / 8, kRowsPass = 32 / kChunks;
       const uint32_t flip = args.negate ? 0x80008000u : 0u;
@@ -610,20 +612,44 @@ __global__ void __launch_bounds__(kPtThreads, 1) prefix_tensor_kernel(const __gr
         w[k] = make_uint4(0, 0, 0, 0);
         if (row < rows) w[k] = *reinterpret_cast<const uint4 *>(a.q + sq * a.q_seq + (int64_t)(h * a.group + r - sq * a.group) * a.q_head + chunk * 16);
       }
-      if constexpr (kScaleQ) {                   // one power of two for all rows of the CTA
-        float top = 0.f;
+      if constexpr (kScaleQ) {
+        // largest of each row: over its kChunks lanes, each of which ends with one row
+        static_assert(kPasses == kChunks, "a row for each lane");
+        float top[kPasses];
 #pragma unroll
         for (int k = 0; k < kPasses; ++k)
-          top = fmaxf(fmaxf(top, fmaxf(largest_of_pair(w[k].x), largest_of_pair(w[k].y))), fmaxf(largest_of_pair(w[k].z), largest_of_pair(w[k].w)));
-        const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
-        if (lane == 0) atomicMax(&sm.q_top, bits);
+          top[k] = fmaxf(fmaxf(largest_of_pair(w[k].x), largest_of_pair(w[k].y)), fmaxf(largest_of_pair(w[k].z), largest_of_pair(w[k].w)));
+#pragma unroll
+        for (int d = kChunks / 2; d > 0; d >>= 1)
+#pragma unroll
+          for (int k = 0; k < d; ++k) {
+            const bool upper = (lane & d) != 0;
+            const float theirs = __shfl_xor_sync(0xffffffffu, upper ? top[k] : top[k + d], d);
+            top[k] = fmaxf(upper ? top[k + d] : top[k], theirs);
+          }
+        const uint32_t bits = __float_as_uint(top[0]);   // of row chunk * kRowsPass + lane / kChunks; rows of zeros do not count
+        const uint32_t most = __reduce_max_sync(0xffffffffu, bits), least = __reduce_min_sync(0xffffffffu, bits == 0 ? 0xffffffffu : bits);
+        if (lane == 0) {
+          atomicMax(&sm.q_top, most);
+          atomicMin(&sm.q_low, least);
+        }
         asm volatile("bar.sync 2, %0;" ::"r"(tiles * 128) : "memory");
-        const int e = shift_to_half(__uint_as_float(*reinterpret_cast<volatile uint32_t *>(&sm.q_top)));
-        const float f = power_of_two(e);
-        if (threadIdx.x == 0) sm.q_back = power_of_two(-e);
+        const uint32_t high = *reinterpret_cast<volatile uint32_t *>(&sm.q_top), low = *reinterpret_cast<volatile uint32_t *>(&sm.q_low);
+        // One power of two for all rows where the largest of each lies within 2^kSameScale of the others' (2^-25, half the least
+        // fp16 step, is then 2^(kSameScale - 39) of a row's largest).  Else each row has its own, and amend_scores undoes it; up
+        // to 2^kSharedBack stays in q_back, so that scores of huge queries stay finite as long as their products with the keys'
+        // scales are.
+        mixed = high > low && high - low > (uint32_t)kSameScale << 23;
+        const int all = shift_to_half(__uint_as_float(high)), e = mixed ? shift_to_half(top[0]) : all;
+        const int shared = mixed ? min(-all, kSharedBack) : -all;
+        if (threadIdx.x == 0) sm.q_back = power_of_two(shared);
+        if (mixed) row_back = __shfl_sync(0xffffffffu, power_of_two(max(-126, -e - shared)), (lane % kRowsPass) * kChunks + lane / kRowsPass);
+        const float own = power_of_two(e);
 #pragma unroll
-        for (int k = 0; k < kPasses; ++k)
+        for (int k = 0; k < kPasses; ++k) {
+          const float f = __shfl_sync(0xffffffffu, own, (lane & ~(kChunks - 1)) + k);
           w[k] = make_uint4(pair_to_half(w[k].x, f), pair_to_half(w[k].y, f), pair_to_half(w[k].z, f), pair_to_half(w[k].w, f));
+        }
       }
 #pragma unroll
       for (int k = 0; k < kPasses; ++k) {
@@ -640,7 +666,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) prefix_tensor_kernel(const __gr
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tc_fence_after();
-      if ((sm.valid[mt][0] & sm.valid[mt][1] & sm.valid[mt][2] & sm.valid[mt][3]) != 0xffffffffu) mask_scores(s_at, sm.valid[mt]);
+      if (mixed || (sm.valid[mt][0] & sm.valid[mt][1] & sm.valid[mt][2] & sm.valid[mt][3]) != 0xffffffffu) amend_scores(s_at, sm.valid[mt], row_back);
       float top[4], factor[4], origin[4];
       tile_max<kFmt>(s_at, sm.sk[mt], scale, top);
       float turn = 1.f;                          // of every row

@@ -11,8 +11,9 @@
 // A row without any key (no prefix, length 0) is 0 with lse = -inf.
 //
 // 8-bit cache: codes are exact in fp16, so the products run on codes in fp16; the scale of a key multiplies its score,
-// the scale of a value its weight.  bf16 queries become fp16 numbers times a power of two that brings the largest to
-// 2^14: they have fewer bits than fp16, so only what is 2^29 times smaller than the largest loses any, 2^-40 of it.
+// the scale of a value its weight.  bf16 queries become fp16 numbers times a power of two of their row that brings its largest
+// to 2^14: they have fewer bits than fp16, so only what is 2^29 times smaller than that loses any, 2^-39 of it.
+// (Where the prefix goes to the tensor cores, rows of like magnitude share a power of two: 2^-29 there.)
 // Weights are fp16 then, four times as exact as bf16 ones.  (The conversion of e4m3 to fp16 is one instruction for two
 // codes; to bf16 it is five, which made up a third of the work of a tile.)
 #pragma once

@@ -1,0 +1,79 @@
+"""shared_prefix_attention where magnitudes differ: between the queries of a batch, and between the values of a row's keys.
+
+Tolerances, per element of a row of queries, with p the softmax weights and u = eps / 2 of the output's type:
+* u * (sum p|v| + |out|) for the weights' and the output's rounding, and (2 d + 64 * 2^-24) sum p|v| for scores that are off
+  by at most d, exp2 and the join.  d = (D + 8) * 2^-24 * scale * max_j sum |q||k_j|, and for bf16 queries that became fp16
+  numbers D * 2^-29 * scale * max|q| * max|k|: a row's power of two leaves its largest at 2^4 or more, where 2^-25, half the
+  least fp16 step, is 2^-29 of it.
+* Weights (of an 8-bit cache: times the value's scale) are fp16 numbers relative to the largest of their row so far, which is
+  at 2^6 or more: one below 2^-14 is off by 2^-25, 2^-31 of the largest.  Over n keys n * 2^-31 * max_j p_j max|v_j|.
+"""
+import math
+
+import pytest
+import torch
+
+from oracle import cache_ops_oracle as o
+from tests.test_gpu_cache_ops import BF16, FP16, attention_case, gen, run_attention, status
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def op(cuda_device):
+    import pcie_through  # noqa: F401
+
+    torch.ops.pcie_through.device_status()
+    return torch.ops.pcie_through
+
+
+def check_rows(c, out, lse, rows):
+    """The rows of queries that `rows` ([seqs, q_heads] truth values) names, against the definition in 64 bits."""
+    k, v = (o.values(c[x], c["block"], c["heads"], c["dim"], c["fmt"]).double() for x in ("k", "v"))
+    kp, ok = o.rows_of(k, c["prefix_table"], c["prefix"], c["block"])
+    vp, _ = o.rows_of(v, c["prefix_table"], c["prefix"], c["block"])
+    assert ok.all()
+    out, lse = out.cpu().double(), lse.cpu().double()
+    u, group = torch.finfo(c["q"].dtype).eps / 2, c["q"].shape[1] // c["heads"]
+    assert rows.any()
+    for s, head in rows.nonzero().tolist():
+        n, h = int(c["lens"][s]), head // group
+        kk = torch.cat([kp, o.rows_of(k, c["tables"][s], n, c["block"])[0]])[:, h]
+        vv = torch.cat([vp, o.rows_of(v, c["tables"][s], n, c["block"])[0]])[:, h]
+        q = c["q"][s, head].double()
+        z = kk @ q * c["scale"]
+        p = torch.softmax(z, 0)
+        want, spread = p @ vv, p @ vv.abs()
+        d = (c["dim"] + 8) * 2 ** -24 * abs(c["scale"]) * (kk.abs() @ q.abs()).max()
+        if c["fmt"] != "raw" and c["q"].dtype == BF16:
+            d = d + c["dim"] * 2 ** -29 * abs(c["scale"]) * q.abs().max() * kk.abs().max()
+        tol = u * (spread + want.abs()) + (2 * d + 64 * 2 ** -24) * spread
+        if c["fmt"] != "raw" or c["q"].dtype == FP16:
+            tol = tol + len(kk) * 2 ** -31 * (p * vv.abs().amax(1)).max()
+        if c["q"].dtype == FP16:
+            tol = tol + 2 ** -25                                   # the output's least step
+        worst = float(((out[s, head] - want).abs() / tol).max())
+        assert worst <= 1, f"row {s}, {head}: {worst:.2f} of the bound"
+        true_lse = torch.logsumexp(z, 0)
+        assert abs(lse[s, head] - true_lse) <= d + 64 * 2 ** -24 * (1 + true_lse.abs())
+
+
+# ------------------------------------------------------------------ queries ---
+@pytest.mark.parametrize("fmt", ["e4m3", "int8", "raw"])
+@pytest.mark.parametrize("seqs,group,dim,aiv", [(40, 4, 128, None), (9, 4, 64, 1), (70, 5, 128, 1), (2, 4, 128, None)])
+def test_a_row_does_not_see_its_neighbours_queries(op, cuda_device, fmt, seqs, group, dim, aiv):
+    """Ordinary rows of a batch in which single heads have queries of 1e6 to the largest finite number, as rows that nobody
+    wrote (padding of a captured batch) may have."""
+    c = attention_case(fmt, BF16, 1, group, dim, 16, 300, [5, 0, 33] * (seqs // 3) + [1] * (seqs % 3), seed=1)
+    ordinary = torch.ones(seqs, group, dtype=torch.bool)
+    for i, power in enumerate((1e6, 1e10, 1e12, 1e20, 1e30, 3e38)):
+        s, head = (i * 7 + 1) % seqs, i % group
+        c["q"][s, head] = (torch.randn(dim, generator=gen(i)).clamp(-1, 1) * power).to(BF16)
+        ordinary[s, head] = False
+    ordinary[0] = True
+    c["q"][0] = (torch.randn(group, dim, generator=gen(9)) * 2).to(BF16)
+    out, lse = run_attention(op, c, cuda_device, aiv=aiv)
+    assert status() == 0
+    check_rows(c, out, lse, ordinary)
+    # the same rows in a batch of ordinary queries: what a row gets does not hang on the others beyond rounding
+    assert out.isfinite().all(-1)[ordinary.to(cuda_device)].all()
