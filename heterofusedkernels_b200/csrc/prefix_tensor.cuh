@@ -510,8 +510,9 @@ __global__ void __launch_bounds__(kPtThreads, 1) prefix_tensor_kernel(const __gr
       };
       constexpr std::integral_constant<int, 0> kK{};
       constexpr std::integral_constant<int, 1> kV{};
-      // `key` and `next` run ahead: sm.off and the scales of tile i + 2 are written when all warps are done with tile i
-      // (nobody reads those of tile i - 2 any more then).
+      // `key` and `next` run ahead.  The places and scales of tile i + 2 take those of tile i - 2: its rows were fetched two
+      // barriers ago, and a thread that found its V stage free again knows that the softmax is done with it.  They are written
+      // ahead of the barrier of tile i, behind which every warp fetches the rows of all of them.
       write_places(0, key);
       producers();
       fetch(0, kK);
@@ -531,9 +532,9 @@ __global__ void __launch_bounds__(kPtThreads, 1) prefix_tensor_kernel(const __gr
         if (i + 1 < n) fetch(i + 1, kK);
         widen(i, kV);
         if (i + 1 < n) fetch(i + 1, kV);
-        producers();
         write_places(i + 2, key);
         write_scales(i + 2, key);
+        producers();
         key = key_of(i + 3, next);
         next = page_of(i + 4);
       }

@@ -77,3 +77,22 @@ def test_a_row_does_not_see_its_neighbours_queries(op, cuda_device, fmt, seqs, g
     check_rows(c, out, lse, ordinary)
     # the same rows in a batch of ordinary queries: what a row gets does not hang on the others beyond rounding
     assert out.isfinite().all(-1)[ordinary.to(cuda_device)].all()
+
+
+@pytest.mark.parametrize("fmt,dtype,dim", [("e4m3", BF16, 128), ("int8", FP16, 128), ("int8", BF16, 64), ("raw", BF16, 128)])
+def test_alternating_batches_give_the_same_bits(op, cuda_device, fmt, dtype, dim):
+    """Two batches with caches, pages and prefixes of their own, in turn: what a CTA's shared memory holds of the call before is
+    never used (the places of a tile's rows are all written when the first of them is read)."""
+    cases = [attention_case(fmt, dtype, 1, 4, dim, 16, prefix, [3, 0, 20] * 4, seed=prefix) for prefix in (1900, 700)]
+    dev = [{n: c[n].to(cuda_device) for n in ("q", "k", "v", "prefix_table", "tables", "lens")} for c in cases]
+    for aiv in (1, None):
+        first = [run_attention(op, c, cuda_device, aiv=aiv) for c in cases]
+        for c, (out, lse) in zip(cases, first):
+            check_rows(c, out, lse, torch.ones(c["q"].shape[:2], dtype=torch.bool))
+        out, lse = [torch.empty_like(x) for x in first[0]]
+        for _ in range(100):
+            for c, d, (want, want_lse) in zip(cases, dev, first):
+                op.shared_prefix_attention(d["q"], out, d["k"], d["v"], d["prefix_table"], c["prefix"], d["tables"], d["lens"], 16, 1,
+                                           {"raw": 0, "e4m3": 1, "int8": 2}[fmt], c["scale"], lse, None, aiv)
+                assert torch.equal(out, want) and torch.equal(lse, want_lse)
+    assert status() == 0
