@@ -70,7 +70,7 @@ def build_capi(force: bool = False, verbose: bool = False, ptxas_info: bool = Fa
     if not force and not _stale(out, deps):
         return out
     nvcc = str(_cuda_home() / "bin" / "nvcc")
-    cmd = [nvcc, "-O3", "-std=c++17", "-lineinfo", "-split-compile", "0", *ARCH_FLAGS, "-shared", "-Xcompiler",
+    cmd = [nvcc, "-O3", "-std=c++17", "-lineinfo", *ARCH_FLAGS, "-shared", "-Xcompiler",
            "-fPIC,-Wall", "-cudart", "static"]
     if ptxas_info:
         cmd += ["-Xptxas", "-v"]
