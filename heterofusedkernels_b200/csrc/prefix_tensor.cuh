@@ -43,6 +43,7 @@ struct PrefixTensorArgs {
 
 constexpr int kPtThreads = 512, kPtRows = 128, kPtKeys = 128, kPtStages = 4, kPtMeta = 4;
 constexpr int kSameScale = 10, kSharedBack = 40;   // powers of two, of bf16 queries that become fp16 numbers
+constexpr int kSameValues = 4;                     // ... and of the scales of a tile's values
 
 template <int D>
 struct PrefixSmem {
@@ -53,6 +54,8 @@ struct PrefixSmem {
   int64_t off[kPtMeta][kPtKeys];                 // byte offset of a key's row, -1: leave out
   alignas(16) float sk[kPtMeta][kPtKeys];         // scales of keys (times scale * log2 e) and of values
   alignas(16) float sv[kPtMeta][kPtKeys];
+  alignas(16) uint32_t sv_high[kPtMeta][4];       // bits of the largest and least |scale of a value| of 32 keys that count
+  alignas(16) uint32_t sv_low[kPtMeta][4];
   uint32_t valid[kPtMeta][4];
   uint64_t full[kPtStages], empty[kPtStages], meta[kPtMeta], s_full[2], p_full[2], o_full, q_full;
   uint32_t tmem;
@@ -135,8 +138,7 @@ __device__ __forceinline__ void tc_store_pairs(uint32_t addr, const uint32_t *r)
   asm volatile("tcgen05.st.sync.aligned.16x128b.x4.b32 [%8], {%0,%1,%2,%3,%4,%5,%6,%7};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]),
                "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(addr));
 }
-__device__ __forceinline__ void tc_wait_load() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-// The same for one tc_load32, whose registers nothing may read earlier; other memory is free to move across.
+// For one tc_load32, whose registers nothing may read earlier; other memory is free to move across.
 __device__ __forceinline__ void tc_wait_load(uint32_t (&r)[32]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;"
                : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]),
@@ -185,7 +187,7 @@ __device__ __forceinline__ void rescale(uint32_t o_at, float factor) {
   for (int c = 0; c < D / 32; ++c) {
     uint32_t s[32];
     tc_load32(o_at + c * 32, s);
-    tc_wait_load();
+    tc_wait_load(s);
 #pragma unroll
     for (int e = 0; e < 32; ++e) s[e] = __float_as_uint(__uint_as_float(s[e]) * factor);
     tc_store32(o_at + c * 32, s);
@@ -200,7 +202,7 @@ __device__ __forceinline__ void amend_scores(uint32_t s_at, const uint32_t *vali
   for (int c = 0; c < 4; ++c) {
     uint32_t s[32];
     tc_load32(s_at + c * 32, s);
-    tc_wait_load();
+    tc_wait_load(s);
     const uint32_t bits = valid[c];
 #pragma unroll
     for (int e = 0; e < 32; ++e) s[e] = bits >> e & 1 ? __float_as_uint(__uint_as_float(s[e]) * factor) : 0xff800000u;
@@ -257,15 +259,47 @@ __device__ __forceinline__ void tile_max(uint32_t s_at, const float *sk, float s
   }
 }
 
-// Weights 2^(score - origin) of the tile's 128 keys, times the values' scales, take the place of the scores (behind what
-// has been read); adds this thread's columns of them, before the scales, to l.
+// log2 of the largest weight times scale of a value, of each of the four rows over the tile: for tiles whose scales differ
+// much (see below), so it is written for size.
+__device__ __forceinline__ void tile_reach(uint32_t s_at, const float *sk, const float *sv, const float (&origin)[4], float (&reach)[4]) {
+  const int t2 = (threadIdx.x & 3) * 2;
+  reach[0] = reach[1] = reach[2] = reach[3] = -INFINITY;
+#pragma unroll 1
+  for (int c = 0; c < 4; ++c) {
+    uint32_t s[32];
+    load_scores(s_at + c * 32, s);
+    tc_wait_load(s);
+#pragma unroll
+    for (int n = 0; n < 4; ++n)
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const float f = sk[c * 32 + n * 8 + t2 + x], log_sv = lg2(fabsf(sv[c * 32 + n * 8 + t2 + x]));   // a NaN is left out
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          reach[k] = fmaxf(reach[k], __fmul_rn(__uint_as_float(s[16 * (k >> 1) + 4 * n + 2 * (k & 1) + x]), f) - origin[k] + log_sv);
+      }
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    reach[k] = fmaxf(reach[k], __shfl_xor_sync(0xffffffffu, reach[k], 1));
+    reach[k] = fmaxf(reach[k], __shfl_xor_sync(0xffffffffu, reach[k], 2));
+  }
+}
+
+// Weights 2^(score - origin) of the tile's 128 keys, of an 8-bit cache times 2^e of the row and the values' scales, take the
+// place of the scores (behind what has been read); adds this thread's columns of them, without these two, to l.
 template <typename M, int kFmt>
-__device__ __forceinline__ void tile_weights(uint32_t s_at, const float *sk, const float *sv, float scale, const float (&origin)[4], float (&l)[4]) {
+__device__ __forceinline__ void tile_weights(uint32_t s_at, const float *sk, const float *sv, float scale, const float (&origin)[4],
+                                             const float (&e)[4], float (&l)[4]) {
   const int t2 = (threadIdx.x & 3) * 2;
   const uint64_t factor = pair_of(scale, scale);
-  uint64_t total[4] = {0, 0, 0, 0}, minus[4];
+  uint64_t total[4] = {0, 0, 0, 0}, minus[4], shift[4];
 #pragma unroll
-  for (int k = 0; k < 4; ++k) minus[k] = pair_of(-origin[k], -origin[k]);
+  for (int k = 0; k < 4; ++k) {
+    const float f = ex2(e[k]);
+    minus[k] = pair_of(-origin[k], -origin[k]);
+    if (kFmt != kFmtRaw) shift[k] = pair_of(f, f);
+  }
   uint32_t buf[2][32];
   auto weigh = [&](int c, const uint32_t (&s)[32]) {
     uint32_t w[16];
@@ -283,7 +317,7 @@ __device__ __forceinline__ void tile_weights(uint32_t s_at, const float *sk, con
         const float2 x = of_pair(fma2(score, kFmt == kFmtRaw ? factor : pair_of(f.x, f.y), minus[k]));
         uint64_t p = pair_of(ex2(x.x), ex2(x.y));
         total[k] = add2(total[k], p);
-        if (kFmt != kFmtRaw) p = mul2(p, pair_of(g.x, g.y));
+        if (kFmt != kFmtRaw) p = mul2(mul2(p, shift[k]), pair_of(g.x, g.y));
         const float2 y = of_pair(p);
         w[8 * (k >> 1) + 2 * n + (k & 1)] = Pair<M>::pack(y.x, y.y);
       }
@@ -414,6 +448,14 @@ __global__ void __launch_bounds__(kPtThreads, 1) prefix_tensor_kernel(const __gr
       }
       const uint32_t word = __ballot_sync(0xffffffffu, k.ok);
       if (lane == 0) sm.valid[m][p >> 5] = word;
+      if (kWide) {
+        const uint32_t bits = __float_as_uint(k.sv) & 0x7fffffffu;
+        const uint32_t high = __reduce_max_sync(0xffffffffu, bits), low = __reduce_min_sync(0xffffffffu, k.ok ? bits : 0x7f800000u);
+        if (lane == 0) {
+          sm.sv_high[m][p >> 5] = high;
+          sm.sv_low[m][p >> 5] = low;
+        }
+      }
       mbar_arrive(&sm.meta[m]);
     };
     auto producers = [&]() {
@@ -593,10 +635,9 @@ __global__ void __launch_bounds__(kPtThreads, 1) prefix_tensor_kernel(const __gr
     const int j = warp / 4;
     const uint32_t lanes = (uint32_t)(warp % 4) << 21;   // first TMEM lane of this warp, in bits 16 and up
     const uint32_t s_at = tmem + j * 128 + lanes, o_at = tmem + 256 + j * D + lanes;
-    // Weights are taken at the origin m + log2(ref), ref a quarter or more of the largest scale of a value so far: the
-    // products with the scales then stay within fp16, whatever the scales are.  (l is at the same origin.)
-    constexpr float kLeastRef = 7.9e-31f;        // 2^-100: its reciprocal times 2^8 and many keys is finite
-    float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, l[4] = {0.f, 0.f, 0.f, 0.f}, ref = kLeastRef, log_ref = kWide ? -100.f : 0.f;
+    float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, l[4] = {0.f, 0.f, 0.f, 0.f};
+    float e[4] = {kMostShift, kMostShift, kMostShift, kMostShift};    // of an 8-bit cache: see kWeightHigh
+    float origin[4] = {0.f, 0.f, 0.f, 0.f};      // m, 0 without a key
     const float scale = a.scale_log2 == 0.f ? kLeastScale : a.scale_log2;   // 0 times the -inf of a masked key is NaN
     bool ok = true, mixed = false;
     float row_back = 1.f;                        // of row `lane`: what undoes its own part of the queries' scaling
@@ -668,43 +709,58 @@ __global__ void __launch_bounds__(kPtThreads, 1) prefix_tensor_kernel(const __gr
       if (!ok) break;
       tc_fence_after();
       if (mixed || (sm.valid[mt][0] & sm.valid[mt][1] & sm.valid[mt][2] & sm.valid[mt][3]) != 0xffffffffu) amend_scores(s_at, sm.valid[mt], row_back);
-      float top[4], factor[4], origin[4];
+      float top[4];
       tile_max<kFmt>(s_at, sm.sk[mt], scale, top);
-      float turn = 1.f;                          // of every row
-      if (kWide) {
-        float big = max_nan(max_nan(fabsf(sm.sv[mt][lane]), fabsf(sm.sv[mt][lane + 32])), max_nan(fabsf(sm.sv[mt][lane + 64]), fabsf(sm.sv[mt][lane + 96])));
-#pragma unroll
-        for (int d = 16; d > 0; d >>= 1) big = max_nan(big, __shfl_xor_sync(0xffffffffu, big, d));
-        if (!(big <= 4.f * ref)) {               // also a NaN
-          turn = ref / big;
-          ref = big;
-          log_ref = log2f(ref);
-        }
-        __syncwarp();
+      // log2 of the largest weight times scale of a value is at most that of the largest weight plus that of the largest scale
+      float log_sv = 0.f;
+      uint32_t high = 0, low = 0;
+      if constexpr (kWide) {
+        const uint4 h4 = *reinterpret_cast<const uint4 *>(sm.sv_high[mt]), l4 = *reinterpret_cast<const uint4 *>(sm.sv_low[mt]);
+        high = max(max(h4.x, h4.y), max(h4.z, h4.w));
+        low = min(min(l4.x, l4.y), min(l4.z, l4.w));
+        log_sv = lg2(__uint_as_float(high));     // a NaN is passed on by the product
       }
-      // the rows' maxima in use, and whether o and l have to follow
-      bool follow = false;
+      bool move = false;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        factor[k] = turn;
-        if (top[k] > m[k] + 8.f) {
-          factor[k] *= ex2(m[k] - top[k]);
-          m[k] = top[k];
-        }
-        follow = follow || factor[k] != 1.f;
-        l[k] *= factor[k];
-        origin[k] = (m[k] == -INFINITY ? 0.f : m[k]) + log_ref;
+        move = move || top[k] > m[k] + 8.f;
+        if (kWide) move = move || !(top[k] - origin[k] + log_sv + e[k] <= kWeightLimit);
       }
-      if (i > 0 && __any_sync(0xffffffffu, follow)) {
-        float mine = 1.f;                        // factor of row `lane`: thread 4 (lane % 8) has it, number lane / 8
+      if (__any_sync(0xffffffffu, move)) {       // the rows' maxima in use, and e; o and l follow
+        float factor[4], reach[4];               // log2 of what o is multiplied by; log2 of the largest weight times scale
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          const float f = __shfl_sync(0xffffffffu, factor[k], (lane & 7) * 4);
-          if (lane >> 3 == k) mine = f;
+          factor[k] = 0.f;
+          if (top[k] > m[k] + 8.f) {
+            factor[k] = m[k] - top[k];
+            m[k] = top[k];
+            l[k] *= ex2(factor[k]);
+          }
+          origin[k] = m[k] == -INFINITY ? 0.f : m[k];
+          reach[k] = top[k] - origin[k] + log_sv;
         }
-        rescale<D>(o_at, mine);
+        if constexpr (kWide) {
+          // where the scales of the tile lie within 2^kSameValues of each other that is at most so much too high
+          if (high > low && high - low > (uint32_t)kSameValues << 23) tile_reach(s_at, sm.sk[mt], sm.sv[mt], origin, reach);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float before = e[k] - factor[k];
+            e[k] = fminf(before, kMostShift);
+            if (reach[k] + e[k] > kWeightLimit) e[k] = floorf(kWeightHigh - reach[k]);
+            factor[k] = e[k] - before;
+          }
+        }
+        if (i > 0) {
+          float mine = 0.f;                      // factor of row `lane`: thread 4 (lane % 8) has it, number lane / 8
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float f = __shfl_sync(0xffffffffu, factor[k], (lane & 7) * 4);
+            if (lane >> 3 == k) mine = f;
+          }
+          rescale<D>(o_at, ex2(mine));
+        }
       }
-      tile_weights<M, kFmt>(s_at, sm.sk[mt], sm.sv[mt], scale, origin, l);
+      tile_weights<M, kFmt>(s_at, sm.sk[mt], sm.sv[mt], scale, origin, e, l);
       tc_wait_store();
       tc_fence_before();
       mbar_arrive(&sm.p_full[j]);
@@ -724,19 +780,28 @@ __global__ void __launch_bounds__(kPtThreads, 1) prefix_tensor_kernel(const __gr
         l[k] += __shfl_xor_sync(0xffffffffu, l[k], 1);
         l[k] += __shfl_xor_sync(0xffffffffu, l[k], 2);
         const int r = warp * 32 + 8 * k + (lane >> 2);
-        if ((lane & 3) == 0 && r < rows) args.part_ml[part - row + r] = make_float2(m[k] == -INFINITY ? m[k] : m[k] + log_ref, l[k]);
+        if ((lane & 3) == 0 && r < rows) args.part_ml[part - row + r] = make_float2(m[k], l[k]);
+      }
+      float back = 1.f;                          // brings o of row `lane` to the origin of l
+      if constexpr (kWide) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float f = __shfl_sync(0xffffffffu, e[k], (lane & 7) * 4);
+          if (lane >> 3 == k) back = ex2(-f);
+        }
       }
       uint32_t buf[2][32];
       tc_load32(o_at, buf[0]);
 #pragma unroll
       for (int c = 0; c < D / 32; ++c) {
         uint32_t (&s)[32] = buf[c & 1];
-        tc_wait_load();
+        tc_wait_load(s);
         if (c + 1 < D / 32) tc_load32(o_at + (c + 1) * 32, buf[(c + 1) & 1]);
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-          *reinterpret_cast<float4 *>(mine + c * 128 + e * 16) =
-              make_float4(__uint_as_float(s[4 * e]), __uint_as_float(s[4 * e + 1]), __uint_as_float(s[4 * e + 2]), __uint_as_float(s[4 * e + 3]));
+        for (int i = 0; i < 8; ++i)
+          *reinterpret_cast<float4 *>(mine + c * 128 + i * 16) =
+              make_float4(__uint_as_float(s[4 * i]) * back, __uint_as_float(s[4 * i + 1]) * back, __uint_as_float(s[4 * i + 2]) * back,
+                          __uint_as_float(s[4 * i + 3]) * back);
       }
       fence_async_proxy();
       if (row < rows) {

@@ -14,8 +14,12 @@
 // the scale of a value its weight.  bf16 queries become fp16 numbers times a power of two of their row that brings its largest
 // to 2^14: they have fewer bits than fp16, so only what is 2^29 times smaller than that loses any, 2^-39 of it.
 // (Where the prefix goes to the tensor cores, rows of like magnitude share a power of two: 2^-29 there.)
-// Weights are fp16 then, four times as exact as bf16 ones.  (The conversion of e4m3 to fp16 is one instruction for two
-// codes; to bf16 it is five, which made up a third of the work of a tile.)
+// Weights, times the value's scale, are fp16 then.  fp16 has few exponents, so they are taken relative to the largest such
+// product of their own row: 2^e, a whole power, brings it to about 2^kWeightHigh, and o is rescaled when it passes 2^kWeightLimit.
+// What is below 2^-14 is off by 2^-25 at most, 2^-31 of the largest, whatever the scales are and whichever keys have them.  The
+// sum l of the weights without the scales has the origin m, o the origin m - e, and where a part is written o is brought to m.
+// (The conversion of e4m3 to fp16 is one instruction for two codes; to bf16 it is five, which made up a third of the work of a
+// tile.)
 #pragma once
 
 #include <type_traits>
@@ -49,6 +53,14 @@ struct AttnArgs {
   float *part_o;                  // [parts][kItemRows][head_dim]
 };
 
+// e of an 8-bit cache is at most kMostShift, so that 2^(8 + e) is an fp32 number: scales below 2^-108 lose bits.
+constexpr float kWeightHigh = 10.f, kWeightLimit = 15.f, kMostShift = 118.f;
+
+__device__ __forceinline__ float lg2(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -440,7 +452,7 @@ __global__ void __launch_bounds__(kLineWarps * 32, 1) shared_prefix_attention_ke
   int stage = 0, items = 0;
   LineItem x;
   // rows of queries 2t and 2t + 1: what their products are multiplied by, maximum, sum (of this lane's keys)
-  float by[2], m[2], l[2], ref, unit;
+  float by[2], m[2], l[2], e[2], f[2];      // of an 8-bit cache e (see kWeightHigh) and f = 2^e
   float o[D / 16][4];
 #pragma unroll 1
   for (int at = begin - kStages; at < end; ++at) {
@@ -463,18 +475,20 @@ __global__ void __launch_bounds__(kLineWarps * 32, 1) shared_prefix_attention_ke
         for (int k = 0; k < D / 16; ++k) top = fmaxf(top, fmaxf(largest_of_pair(qf[k][0]), largest_of_pair(qf[k][1])));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const int e = shift_to_half(top);        // of row g
-        const float f = power_of_two(e), back = power_of_two(-e);
+        const int shift = shift_to_half(top);    // of row g
+        const float up = power_of_two(shift), down = power_of_two(-shift);
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {
-          qf[k][0] = pair_to_half(qf[k][0], f);
-          qf[k][1] = pair_to_half(qf[k][1], f);
+          qf[k][0] = pair_to_half(qf[k][0], up);
+          qf[k][1] = pair_to_half(qf[k][1], up);
         }
-        by[0] *= __shfl_sync(0xffffffffu, back, 8 * t);
-        by[1] *= __shfl_sync(0xffffffffu, back, 8 * t + 4);
+        by[0] *= __shfl_sync(0xffffffffu, down, 8 * t);
+        by[1] *= __shfl_sync(0xffffffffu, down, 8 * t + 4);
       }
       m[0] = m[1] = -INFINITY;
-      l[0] = l[1] = ref = unit = 0.f;
+      l[0] = l[1] = 0.f;
+      e[0] = e[1] = kMostShift;
+      f[0] = f[1] = ex2(kMostShift);
 #pragma unroll
       for (int j = 0; j < D / 16; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
     }
@@ -516,13 +530,13 @@ __global__ void __launch_bounds__(kLineWarps * 32, 1) shared_prefix_attention_ke
       for (int n = 0; n < kM; ++n)
 #pragma unroll
         for (int y = 0; y < 2; ++y) {
-          float f = 1.f;
+          float sk = 1.f;
           if (kCodes) {
-            f = ring.scales[stage][16 * n + 8 * y + g];
+            sk = ring.scales[stage][16 * n + 8 * y + g];
             sv[n][y] = ring.scales[stage][kKeys + 16 * n + 8 * y + g];
           }
-          s[n][2 * y] *= kCodes ? by[0] * f : by[0];
-          s[n][2 * y + 1] *= kCodes ? by[1] * f : by[1];
+          s[n][2 * y] *= kCodes ? by[0] * sk : by[0];
+          s[n][2 * y + 1] *= kCodes ? by[1] * sk : by[1];
         }
       constexpr uint32_t kAll = kKeys == 32 ? 0xffffffffu : 0xffffu;
       if (valid != kAll) {
@@ -537,15 +551,15 @@ __global__ void __launch_bounds__(kLineWarps * 32, 1) shared_prefix_attention_ke
       for (int n = 0; n < kM; ++n)
 #pragma unroll
         for (int r = 0; r < 2; ++r) top[r] = fmaxf(top[r], fmaxf(s[n][r], s[n][2 + r]));
-      // m follows a row's maximum only where it is 2^8 behind: weights up to 2^8 are as exact as weights up to 1.
-      // fp16 weights of an 8-bit cache: weight * scale may leave fp16's range, so o is kept in units of (a quarter or
-      // more of) the largest scale of a value so far.
+      // m follows a row's maximum only where it is 2^8 behind: weights up to 2^8 are as exact as weights up to 1.  Of an 8-bit
+      // cache also e, where a weight times its value's scale passes 2^kWeightLimit; it is at most (largest weight) * (largest scale).
       bool move = top[0] > m[0] + 8.f || top[1] > m[1] + 8.f;
-      float big = 0.f;
       if (kCodes) {
+        float big = 0.f;                          // a NaN is left out here and passed on by the product
 #pragma unroll
-        for (int n = 0; n < kM; ++n) big = max_nan(big, max_nan(fabsf(sv[n][0]), fabsf(sv[n][1])));
-        move = move || !(big <= 4.f * ref);       // also a NaN
+        for (int n = 0; n < kM; ++n) big = fmaxf(big, fmaxf(fabsf(sv[n][0]), fabsf(sv[n][1])));
+        big = lg2(big);
+        move = move || top[0] - m[0] + big + e[0] > kWeightLimit || top[1] - m[1] + big + e[1] > kWeightLimit;
       }
       if (__any_sync(0xffffffffu, move)) {
         // the tile's maxima: over the lanes of equal t
@@ -553,21 +567,38 @@ __global__ void __launch_bounds__(kLineWarps * 32, 1) shared_prefix_attention_ke
         for (int d = 4; d < 32; d <<= 1) {
           top[0] = fmaxf(top[0], __shfl_xor_sync(0xffffffffu, top[0], d));
           top[1] = fmaxf(top[1], __shfl_xor_sync(0xffffffffu, top[1], d));
-          if (kCodes) big = max_nan(big, __shfl_xor_sync(0xffffffffu, big, d));
         }
-        float alpha[2];
+        float alpha[2], rise[2];
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          const float next = top[r] > m[r] + 8.f ? top[r] : m[r];
-          alpha[r] = next == m[r] ? 1.f : ex2(m[r] - next);
-          m[r] = next;
+          rise[r] = top[r] > m[r] + 8.f ? top[r] - m[r] : 0.f;     // infinite at the first key
+          alpha[r] = ex2(-rise[r]);
+          m[r] = rise[r] > 0.f ? top[r] : m[r];
           l[r] *= alpha[r];
         }
-        if (kCodes && !(big <= 4.f * ref)) {      // the same in every lane
-          alpha[0] *= ref / big;
-          alpha[1] *= ref / big;
-          ref = big;
-          unit = 1.f / big;
+        if constexpr (kCodes) {
+          float reach[2] = {-INFINITY, -INFINITY};   // log2 of the largest weight times scale
+#pragma unroll
+          for (int n = 0; n < kM; ++n)
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+              const float log_sv = lg2(fabsf(sv[n][y]));
+              reach[0] = fmaxf(reach[0], s[n][2 * y] - m[0] + log_sv);
+              reach[1] = fmaxf(reach[1], s[n][2 * y + 1] - m[1] + log_sv);
+            }
+#pragma unroll
+          for (int d = 4; d < 32; d <<= 1) {
+            reach[0] = fmaxf(reach[0], __shfl_xor_sync(0xffffffffu, reach[0], d));
+            reach[1] = fmaxf(reach[1], __shfl_xor_sync(0xffffffffu, reach[1], d));
+          }
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const float before = e[r] + rise[r];
+            e[r] = fminf(before, kMostShift);
+            if (reach[r] + e[r] > kWeightLimit) e[r] = floorf(kWeightHigh - reach[r]);
+            alpha[r] = ex2(e[r] - before);
+            f[r] = ex2(e[r]);
+          }
         }
 #pragma unroll
         for (int j = 0; j < D / 16; ++j) {
@@ -588,8 +619,7 @@ __global__ void __launch_bounds__(kLineWarps * 32, 1) shared_prefix_attention_ke
           const float p0 = ex2(s[n][2 * y] - safe[0]), p1 = ex2(s[n][2 * y + 1] - safe[1]);
           l[0] += p0;
           l[1] += p1;
-          const float f = kCodes ? sv[n][y] * unit : 1.f;
-          pw[y] = transpose8(kCodes ? Pair<M>::pack(p0 * f, p1 * f) : Pair<M>::pack(p0, p1));
+          pw[y] = transpose8(kCodes ? Pair<M>::pack(p0 * f[0] * sv[n][y], p1 * f[1] * sv[n][y]) : Pair<M>::pack(p0, p1));
         }
 #pragma unroll
         for (int c = 0; c < kVc; ++c) {
@@ -641,7 +671,7 @@ __global__ void __launch_bounds__(kLineWarps * 32, 1) shared_prefix_attention_ke
       const int row = 2 * t + r;
       if (row < x.rows) {
         if (g == 0) a.part_ml[part * kItemRows + row] = make_float2(m[r], l[r]);
-        const float back = kCodes ? ref : 1.f;
+        const float back = kCodes ? ex2(-e[r]) : 1.f;
         float *dst = a.part_o + (part * kItemRows + row) * D;
 #pragma unroll
         for (int c = 0; c < kVc; ++c)

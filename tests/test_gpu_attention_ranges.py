@@ -96,3 +96,86 @@ def test_alternating_batches_give_the_same_bits(op, cuda_device, fmt, dtype, dim
                                            {"raw": 0, "e4m3": 1, "int8": 2}[fmt], c["scale"], lse, None, aiv)
                 assert torch.equal(out, want) and torch.equal(lse, want_lse)
     assert status() == 0
+
+
+# ------------------------------------------------------- scales of the values ---
+def placed_case(fmt, dtype, dim, seqs, group, prefix, score, size, seed=0):
+    """One K/V head; key j of the prefix has the score score[j] log2 e^-1 for every row (in units of log2, up to the cache's
+    rounding) and values of about 2^size[j]."""
+    c = attention_case(fmt, dtype, 1, group, dim, 16, prefix, [2] * seqs, seed=seed)
+    g = gen(seed + 40)
+    c["q"] = (0.01 * torch.randn(seqs, group, dim, generator=g)).to(dtype)
+    c["q"][..., 0] = 2
+    k = 0.01 * torch.randn(prefix, 1, dim, generator=g)
+    k[:, 0, 0] = torch.as_tensor(score) * math.log(2) / 2
+    c["scale"] = 1.0
+    v = torch.randn(prefix, 1, dim, generator=g) * 2.0 ** torch.as_tensor(size, dtype=torch.float32)[:, None, None]
+    at = torch.arange(prefix)
+    slots = c["prefix_table"][at // 16] * 16 + at % 16
+    o.write(k.to(dtype), c["k"], slots, 16, fmt)
+    o.write(v.to(dtype), c["v"], slots, 16, fmt)
+    for s in range(seqs):                                          # the own tokens: far below
+        rows = torch.zeros(2, 1, dim)
+        rows[:, 0, 0] = -200
+        mine = c["tables"][s, 0] * 16 + torch.arange(2)
+        o.write(rows.to(dtype), c["k"], mine, 16, fmt)
+    return c
+
+
+def check_all(op, device, c):
+    for aiv in (None, 1):
+        out, lse = run_attention(op, c, device, aiv=aiv)
+        assert status() == 0
+        check_rows(c, out, lse, torch.ones(c["q"].shape[:2], dtype=torch.bool))
+
+
+@pytest.mark.parametrize("fmt,dtype", [("e4m3", BF16), ("int8", BF16), ("e4m3", FP16), ("int8", FP16)])
+@pytest.mark.parametrize("seqs", [2, 40])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_a_large_value_that_a_row_does_not_weigh(op, cuda_device, fmt, dtype, seqs, dim):
+    """One key of the prefix has values 2^14 (fp16: 2^10) or, in bf16, 2^20 to 2^90 times the others' and a weight of 2^-60 and
+    less: the others keep their bits, wherever the key lies."""
+    n = 500
+    for power, far in ((14, 60), (20, 60), (90, 190)) if dtype == BF16 else ((10, 60),):
+        for place in (0, 130, n - 1):
+            score, size = -torch.rand(n, generator=gen(power)) * 9, torch.zeros(n)
+            score[place], size[place] = -far, power
+            check_all(op, cuda_device, placed_case(fmt, dtype, dim, seqs, 2, n, score, size, seed=place))
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("seqs", [2, 40])
+@pytest.mark.parametrize("rise", [0.03, 0.3, -0.3])
+def test_value_scales_that_rise_along_the_prefix(op, cuda_device, fmt, seqs, rise):
+    """Values of 2^(rise j), so that o is rescaled from tile to tile while the rows' maxima stay; with the scores falling by as
+    much every key counts, and with steep scores only one side does."""
+    n = 400
+    j = torch.arange(n)
+    for slope in (0.0, -rise, -1.1 * rise):
+        check_all(op, cuda_device, placed_case(fmt, BF16, 128, seqs, 2, n, slope * j - max(0.0, slope * n), rise * j - max(0.0, rise * n / 2), seed=3))
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("seqs", [2, 40])
+def test_a_first_key_with_a_large_weight_and_small_values(op, cuda_device, fmt, seqs):
+    """The first key takes nearly all weight and has values of 2^-12 of the others' or none at all."""
+    n = 300
+    score, size = torch.full((n,), -16.0) - torch.rand(n, generator=gen(2)) * 4, torch.zeros(n)
+    score[0] = 0
+    for small in (-12, -200):
+        size[0] = small
+        check_all(op, cuda_device, placed_case(fmt, BF16, 128, seqs, 2, n, score, size, seed=4))
+    c = placed_case(fmt, BF16, 128, seqs, 2, n, score, torch.full((n,), -200.0), seed=5)     # values of nothing but zeros
+    out, _ = run_attention(op, dict(c, lens=torch.zeros(seqs, dtype=torch.int64)), cuda_device)
+    assert (out == 0).all() and status() == 0
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("seqs", [2, 40])
+def test_values_of_nearly_the_largest_number(op, cuda_device, fmt, seqs):
+    """Values of 2^120, and next to them values of 1 with a weight 2^100 times as large: sum and result stay finite and right."""
+    n = 200
+    score = -torch.rand(n, generator=gen(2)) * 30
+    check_all(op, cuda_device, placed_case(fmt, BF16, 128, seqs, 2, n, score, torch.full((n,), 120.0), seed=6))
+    size = torch.where(torch.arange(n) % 3 == 0, 100.0, 0.0)
+    check_all(op, cuda_device, placed_case(fmt, BF16, 128, seqs, 2, n, score - size, size, seed=7))
