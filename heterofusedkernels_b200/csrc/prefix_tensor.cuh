@@ -164,11 +164,6 @@ __device__ __forceinline__ float2 of_pair(uint64_t v) {
   asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
   return r;
 }
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
 __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
   uint64_t r;
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
@@ -177,6 +172,12 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
 __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   uint64_t r;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+// A sum that no multiplication before it is drawn into (mul.rn.f32x2 and add.rn.f32x2 became one fma): rounded towards zero.
+__device__ __forceinline__ uint64_t add2_apart(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rz.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
 
@@ -288,6 +289,8 @@ __device__ __forceinline__ void tile_reach(uint32_t s_at, const float *sk, const
 
 // Weights 2^(score - origin) of the tile's 128 keys, of an 8-bit cache times 2^e of the row and the values' scales, take the
 // place of the scores (behind what has been read); adds this thread's columns of them, without these two, to l.
+// The score is rounded before the origin is taken off it, as it was when the origin was found: with one rounding for both the
+// largest score of 2^28 would be up to 2^4 above its own origin, and its weight no fp16 number.
 template <typename M, int kFmt>
 __device__ __forceinline__ void tile_weights(uint32_t s_at, const float *sk, const float *sv, float scale, const float (&origin)[4],
                                              const float (&e)[4], float (&l)[4]) {
@@ -314,7 +317,7 @@ __device__ __forceinline__ void tile_weights(uint32_t s_at, const float *sk, con
       for (int k = 0; k < 4; ++k) {
         const int i = 16 * (k >> 1) + 4 * n + 2 * (k & 1);
         const uint64_t score = pair_of(__uint_as_float(s[i]), __uint_as_float(s[i + 1]));
-        const float2 x = of_pair(fma2(score, kFmt == kFmtRaw ? factor : pair_of(f.x, f.y), minus[k]));
+        const float2 x = of_pair(add2_apart(mul2(score, kFmt == kFmtRaw ? factor : pair_of(f.x, f.y)), minus[k]));
         uint64_t p = pair_of(ex2(x.x), ex2(x.y));
         total[k] = add2(total[k], p);
         if (kFmt != kFmtRaw) p = mul2(mul2(p, shift[k]), pair_of(g.x, g.y));

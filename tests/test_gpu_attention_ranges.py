@@ -98,6 +98,35 @@ def test_alternating_batches_give_the_same_bits(op, cuda_device, fmt, dtype, dim
     assert status() == 0
 
 
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("scale", [0.11, -0.11])
+def test_queries_that_grow_from_row_to_row(op, cuda_device, fmt, scale):
+    """Rows of all magnitudes from 2^-30 to 2^30, with scores of order one in the rows that `scale` suits, masked pages and an
+    odd end of the prefix in the same tiles."""
+    c = attention_case(fmt, BF16, 1, 8, 128, 16, 517, [3] * 8, seed=5)
+    power = torch.linspace(-30, 30, 64).round().view(8, 8, 1)
+    c["q"] = (torch.randn(8, 8, 128, generator=gen(1)) * 2.0 ** power).to(BF16)
+    c["q"][3, 3] = 0
+    c["scale"] = scale
+    for aiv in (None, 1):
+        out, lse = run_attention(op, c, cuda_device, aiv=aiv)
+        assert status() == 0
+        check_rows(c, out, lse, torch.ones(8, 8, dtype=torch.bool))
+
+
+@pytest.mark.parametrize("seqs", [2, 40])
+@pytest.mark.parametrize("dtype,powers", [(BF16, (8, 20, 25, 31, 40, 70)), (FP16, (8, 13))])
+def test_scores_of_any_magnitude(op, cuda_device, seqs, dtype, powers):
+    """16-bit caches, queries of up to 2^70: the scores' last place is far above one, and the largest has the weight 1."""
+    c = attention_case("raw", dtype, 1, 4, 128, 16, 300, [5] * seqs, seed=8)
+    c["scale"] = 1.0
+    for power in powers:
+        c["q"] = (torch.randn(seqs, 4, 128, generator=gen(power)).clamp(-3, 3) * 2.0 ** power).to(dtype)
+        out, lse = run_attention(op, c, cuda_device)
+        assert status() == 0
+        check_rows(c, out, lse, torch.ones(seqs, 4, dtype=torch.bool))
+
+
 # ------------------------------------------------------- scales of the values ---
 def placed_case(fmt, dtype, dim, seqs, group, prefix, score, size, seed=0):
     """One K/V head; key j of the prefix has the score score[j] log2 e^-1 for every row (in units of log2, up to the cache's
