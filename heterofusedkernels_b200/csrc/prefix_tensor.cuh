@@ -287,8 +287,9 @@ __device__ __forceinline__ void tile_reach(uint32_t s_at, const float *sk, const
   }
 }
 
-// Weights 2^(score - origin) of the tile's 128 keys, of an 8-bit cache times 2^e of the row and the values' scales, take the
-// place of the scores (behind what has been read); adds this thread's columns of them, without these two, to l.
+// Weights 2^(score - origin) of the tile's 128 keys, of an 8-bit cache times 2^e of the row and the values' scales, of an fp16
+// cache times raw_shift, take the place of the scores (behind what has been read); adds this thread's columns of them,
+// without these factors, to l.
 // The score is rounded before the origin is taken off it, as it was when the origin was found: with one rounding for both the
 // largest score of 2^28 would be up to 2^4 above its own origin, and its weight no fp16 number.
 template <typename M, int kFmt>
@@ -301,7 +302,7 @@ __device__ __forceinline__ void tile_weights(uint32_t s_at, const float *sk, con
   for (int k = 0; k < 4; ++k) {
     const float f = ex2(e[k]);
     minus[k] = pair_of(-origin[k], -origin[k]);
-    if (kFmt != kFmtRaw) shift[k] = pair_of(f, f);
+    shift[k] = kFmt == kFmtRaw ? pair_of(raw_shift<M>(), raw_shift<M>()) : pair_of(f, f);
   }
   uint32_t buf[2][32];
   auto weigh = [&](int c, const uint32_t (&s)[32]) {
@@ -320,7 +321,8 @@ __device__ __forceinline__ void tile_weights(uint32_t s_at, const float *sk, con
         const float2 x = of_pair(add2_apart(mul2(score, kFmt == kFmtRaw ? factor : pair_of(f.x, f.y)), minus[k]));
         uint64_t p = pair_of(ex2(x.x), ex2(x.y));
         total[k] = add2(total[k], p);
-        if (kFmt != kFmtRaw) p = mul2(mul2(p, shift[k]), pair_of(g.x, g.y));
+        if (kFmt != kFmtRaw || raw_shift<M>() != 1.f) p = mul2(p, shift[k]);
+        if (kFmt != kFmtRaw) p = mul2(p, pair_of(g.x, g.y));
         const float2 y = of_pair(p);
         w[8 * (k >> 1) + 2 * n + (k & 1)] = Pair<M>::pack(y.x, y.y);
       }
@@ -785,7 +787,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) prefix_tensor_kernel(const __gr
         const int r = warp * 32 + 8 * k + (lane >> 2);
         if ((lane & 3) == 0 && r < rows) args.part_ml[part - row + r] = make_float2(m[k], l[k]);
       }
-      float back = 1.f;                          // brings o of row `lane` to the origin of l
+      float back = kWide ? 1.f : 1.f / raw_shift<M>();   // brings o of row `lane` to the origin of l
       if constexpr (kWide) {
 #pragma unroll
         for (int k = 0; k < 4; ++k) {

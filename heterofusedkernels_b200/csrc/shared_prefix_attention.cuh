@@ -56,6 +56,11 @@ struct AttnArgs {
 // e of an 8-bit cache is at most kMostShift, so that 2^(8 + e) is an fp32 number: scales below 2^-108 lose bits.
 constexpr float kWeightHigh = 10.f, kWeightLimit = 15.f, kMostShift = 118.f;
 
+// Weights of a 16-bit cache are numbers of its type; up to 2^8 (see below), so that in fp16 2^7 times them still is one, and 2^-25,
+// half its least step, is 2^-32 of the largest.
+template <typename M>
+__device__ __forceinline__ constexpr float raw_shift() { return std::is_same<M, __half>::value ? 128.f : 1.f; }
+
 __device__ __forceinline__ float lg2(float x) {
   float y;
   asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -619,7 +624,8 @@ __global__ void __launch_bounds__(kLineWarps * 32, 1) shared_prefix_attention_ke
           const float p0 = ex2(s[n][2 * y] - safe[0]), p1 = ex2(s[n][2 * y + 1] - safe[1]);
           l[0] += p0;
           l[1] += p1;
-          pw[y] = transpose8(kCodes ? Pair<M>::pack(p0 * f[0] * sv[n][y], p1 * f[1] * sv[n][y]) : Pair<M>::pack(p0, p1));
+          pw[y] = transpose8(kCodes ? Pair<M>::pack(p0 * f[0] * sv[n][y], p1 * f[1] * sv[n][y])
+                                    : Pair<M>::pack(p0 * raw_shift<M>(), p1 * raw_shift<M>()));
         }
 #pragma unroll
         for (int c = 0; c < kVc; ++c) {
@@ -671,7 +677,7 @@ __global__ void __launch_bounds__(kLineWarps * 32, 1) shared_prefix_attention_ke
       const int row = 2 * t + r;
       if (row < x.rows) {
         if (g == 0) a.part_ml[part * kItemRows + row] = make_float2(m[r], l[r]);
-        const float back = kCodes ? ex2(-e[r]) : 1.f;
+        const float back = kCodes ? ex2(-e[r]) : 1.f / raw_shift<M>();
         float *dst = a.part_o + (part * kItemRows + row) * D;
 #pragma unroll
         for (int c = 0; c < kVc; ++c)

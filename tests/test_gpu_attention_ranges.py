@@ -5,8 +5,10 @@ Tolerances, per element of a row of queries, with p the softmax weights and u = 
   by at most d, exp2 and the join.  d = (D + 8) * 2^-24 * scale * max_j sum |q||k_j|, and for bf16 queries that became fp16
   numbers D * 2^-29 * scale * max|q| * max|k|: a row's power of two leaves its largest at 2^4 or more, where 2^-25, half the
   least fp16 step, is 2^-29 of it.
-* Weights (of an 8-bit cache: times the value's scale) are fp16 numbers relative to the largest of their row so far, which is
+* Weights of an 8-bit cache, times the value's scale, are fp16 numbers relative to the largest of their row so far, which is
   at 2^6 or more: one below 2^-14 is off by 2^-25, 2^-31 of the largest.  Over n keys n * 2^-31 * max_j p_j max|v_j|.
+* Weights of an fp16 cache are fp16 numbers relative to the largest weight, which is at 2^7 or more, whatever the values are:
+  each is off by 2^-25, so 2^-32 max p, which its value multiplies: 2^-32 max p * sum |v_j|.
 """
 import math
 
@@ -48,8 +50,10 @@ def check_rows(c, out, lse, rows):
         if c["fmt"] != "raw" and c["q"].dtype == BF16:
             d = d + c["dim"] * 2 ** -29 * abs(c["scale"]) * q.abs().max() * kk.abs().max()
         tol = u * (spread + want.abs()) + (2 * d + 64 * 2 ** -24) * spread
-        if c["fmt"] != "raw" or c["q"].dtype == FP16:
+        if c["fmt"] != "raw":
             tol = tol + len(kk) * 2 ** -31 * (p * vv.abs().amax(1)).max()
+        elif c["q"].dtype == FP16:
+            tol = tol + 2 ** -32 * p.max() * vv.abs().sum(0)
         if c["q"].dtype == FP16:
             tol = tol + 2 ** -25                                   # the output's least step
         worst = float(((out[s, head] - want).abs() / tol).max())
@@ -208,3 +212,16 @@ def test_values_of_nearly_the_largest_number(op, cuda_device, fmt, seqs):
     check_all(op, cuda_device, placed_case(fmt, BF16, 128, seqs, 2, n, score, torch.full((n,), 120.0), seed=6))
     size = torch.where(torch.arange(n) % 3 == 0, 100.0, 0.0)
     check_all(op, cuda_device, placed_case(fmt, BF16, 128, seqs, 2, n, score - size, size, seed=7))
+
+
+@pytest.mark.parametrize("seqs", [2, 40])
+def test_very_many_keys_of_very_small_weight(op, cuda_device, seqs):
+    """An fp16 cache: one key with values of 0 takes nearly all weight, 16383 with a weight of 2^-25.5 each make up the result."""
+    n = 16384
+    score, size = torch.full((n,), -25.5), torch.zeros(n)
+    score[5], size[5] = 0, -200
+    c = placed_case("raw", FP16, 64, seqs, 2, n, score, size, seed=9)
+    slots = c["prefix_table"][torch.arange(n) // 16], torch.arange(n) % 16
+    c["v"][slots] = c["v"][slots].abs() + 1                          # of one sign, so that they do not cancel
+    c["v"][slots[0][5], slots[1][5]] = 0
+    check_all(op, cuda_device, c)
