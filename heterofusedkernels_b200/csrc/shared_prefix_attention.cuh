@@ -540,8 +540,9 @@ __global__ void __launch_bounds__(kLineWarps * 32, 1) shared_prefix_attention_ke
             sk = ring.scales[stage][16 * n + 8 * y + g];
             sv[n][y] = ring.scales[stage][kKeys + 16 * n + 8 * y + g];
           }
-          s[n][2 * y] *= kCodes ? by[0] * sk : by[0];
-          s[n][2 * y + 1] *= kCodes ? by[1] * sk : by[1];
+          // (a product of its own: an fma with the maximum would be off from the maximum's own rounding)
+          s[n][2 * y] = __fmul_rn(s[n][2 * y], kCodes ? by[0] * sk : by[0]);
+          s[n][2 * y + 1] = __fmul_rn(s[n][2 * y + 1], kCodes ? by[1] * sk : by[1]);
         }
       constexpr uint32_t kAll = kKeys == 32 ? 0xffffffffu : 0xffffu;
       if (valid != kAll) {
