@@ -34,7 +34,7 @@ INCLUDE = ROOT / "include"
 CAPI_SOURCES = ["hfk_capi.cu", "host_registry.cpp"]
 CAPI_DEPS = ["common.cuh", "kv_swap.cuh", "paged_gather.cuh", "row_gather.cuh", "block_transfer.cuh", "relayout_swap.cuh",
              "kv_migrate.cuh", "kv_format.cuh", "kv_write.cuh", "paged_gather_dequant.cuh", "shared_prefix_attention.cuh",
-             "prefix_tensor.cuh", "cache_ops_host.cuh", "ptr_check.h", "host_util.h"]
+             "prefix_tensor.cuh", "cache_ops_host.cuh", "bounded_wait.h", "ptr_check.h", "host_util.h"]
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

@@ -27,6 +27,7 @@
 // across the rows: the transposed form of the operand).
 #pragma once
 
+#include "bounded_wait.h"
 #include "shared_prefix_attention.cuh"
 
 namespace hfk {
@@ -396,18 +397,15 @@ __global__ void __launch_bounds__(kPtThreads, 1) prefix_tensor_kernel(const __gr
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, *reinterpret_cast<volatile uint32_t *>(&sm.tmem), 0);
+  auto give_up = [&]() {                         // and all the others with this thread
+    raise_status(HFK_DEV_WAIT_TIMEOUT);
+    *reinterpret_cast<volatile int *>(&sm.failed) = 1;
+  };
   auto wait = [&](uint64_t *bar, uint32_t parity) -> bool {
-    if (mbar_try_wait(bar, parity)) return true;
-    const uint64_t t0 = global_timer_ns();
-    while (!mbar_try_wait(bar, parity)) {
-      if (*reinterpret_cast<volatile int *>(&sm.failed)) return false;   // another one gave up: all do
-      if (global_timer_ns() - t0 > kWaitLimitNs) {
-        raise_status(HFK_DEV_WAIT_TIMEOUT);
-        *reinterpret_cast<volatile int *>(&sm.failed) = 1;
-        return false;
-      }
-    }
-    return true;
+    const WaitEnd end = bounded_wait([=] { return mbar_try_wait(bar, parity); }, [] { return global_timer_ns(); },
+                                     [&] { return *reinterpret_cast<volatile int *>(&sm.failed) != 0; }, kWaitLimitNs);
+    if (end == WaitEnd::kRanOut) give_up();
+    return end == WaitEnd::kDone;
   };
 
   auto wait_warp = [&](uint64_t *bar, uint32_t parity) -> bool { return __all_sync(0xffffffffu, wait(bar, parity)); };
@@ -629,8 +627,9 @@ __global__ void __launch_bounds__(kPtThreads, 1) prefix_tensor_kernel(const __gr
         ok = wait_warp(&sm.p_full[j], (n - 1) & 1);
         if (ok) values(j, n - 1);
       }
-      tc_commit(&sm.o_full, leader);                     // also after a failure: nothing is in flight when the CTA ends
-      wait_warp(&sm.o_full, 0);
+      // also after a failure: the products that were issued have read shared memory and written TMEM before the CTA gives them up
+      tc_commit(&sm.o_full, leader);
+      if (!drain([&] { return mbar_try_wait(&sm.o_full, 0); }, [] { return global_timer_ns(); }, kWaitLimitNs)) give_up();
     }
     __syncwarp();
   } else {
