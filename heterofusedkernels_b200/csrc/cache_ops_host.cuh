@@ -280,6 +280,27 @@ static int plan_attention(const hfk_prefix_attention_desc *d, int ctas, AttnPlan
   return HFK_OK;
 }
 
+// What no call with this descriptor, or with fewer sequences, a shorter prefix or narrower block tables, needs more than.  The plan's
+// own size is not monotone: more rows of queries may take fewer runs of the prefix, and what is largest is their product.
+static size_t attention_workspace_bound(const hfk_prefix_attention_desc *d, int ctas) {
+  const int64_t sms = sm_count(), seqs = std::min<int64_t>(d->num_seqs, HFK_MAX_SEQS), rows = seqs * d->group;
+  const int64_t row_tiles = (rows + kItemRows - 1) / kItemRows, own_tiles = (d->group + kItemRows - 1) / kItemRows;
+  // the line: every part of every item, the prefix's items among them up to where they go to the tensor cores
+  const int64_t most_prefix = (kPrefixTensorMinRows + kItemRows - 1) / kItemRows;
+  const int64_t items = seqs * d->kv_heads * own_tiles + (d->prefix_len > 0 ? std::min(row_tiles, most_prefix) * d->kv_heads : 0);
+  const int64_t parts = (ctas > 0 ? std::min<int64_t>(ctas, 65535) : sms * kAttnCtasPerSm) * kLineWarps + items;
+  // the prefix: s runs of r rows of every K/V head, r up to rows; one run, or s <= 2 * room / (kv_heads * ceil(r / 256)) of them
+  int64_t values = 0;
+  if (d->prefix_len > 0 && rows > kPrefixTensorMinRows) {
+    const int64_t room = ctas > 0 ? std::min<int64_t>(ctas, sms) : sms, tiles = (d->prefix_len + kPtKeys - 1) / kPtKeys;
+    const int64_t one = d->kv_heads * rows;
+    values = std::max(one, std::min(2 * room * std::min<int64_t>(rows, 256), tiles * one));
+  }
+  const auto round = [](int64_t n) { return ((size_t)n + 255) & ~(size_t)255; };
+  return 256 + round(parts * kItemRows * sizeof(float2)) + round(parts * kItemRows * d->head_dim * sizeof(float)) +
+         round(values * sizeof(float2)) + round(values * d->head_dim * sizeof(float));
+}
+
 // A launch that may start while the kernel launched before it in the same stream still runs (`early`, where that
 // is one of ours and says so with launch_next).
 template <typename Args>

@@ -894,7 +894,7 @@ int hfk_paged_gather_dequant(const hfk_paged_gather_desc *gather, int kv_format,
 
 size_t hfk_prefix_attention_workspace(const hfk_prefix_attention_desc *desc, int ctas) {
   AttnPlan p = {};
-  return plan_attention(desc, ctas, &p) == HFK_OK ? p.bytes() : 0;
+  return plan_attention(desc, ctas, &p) == HFK_OK ? attention_workspace_bound(desc, ctas) : 0;
 }
 
 int hfk_shared_prefix_attention(const hfk_prefix_attention_desc *desc, int ctas, hfk_stream_t stream) {

@@ -606,7 +606,8 @@ static hfk_prefix_attention_desc attention_desc(const at::Tensor &q, int64_t pre
   return d;
 }
 
-// Bytes of workspace for calls of this shape (a caller that keeps one workspace sizes it for its largest batch).
+// Bytes of workspace for calls of this shape and smaller ones (a caller that keeps one workspace sizes it for its largest batch,
+// longest prefix and the same aiv).
 int64_t shared_prefix_attention_workspace(const at::Tensor &q, int64_t prefixLen, const at::Tensor &blockTables, int64_t blockSize,
                                           int64_t kvHeads, c10::optional<int64_t> aiv) {
   const char *op = "shared_prefix_attention_workspace";

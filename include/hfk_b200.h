@@ -534,8 +534,9 @@ typedef struct hfk_prefix_attention_desc {
   size_t workspace_bytes;
 } hfk_prefix_attention_desc;
 
-/* Bytes of workspace a call with this descriptor needs (pointers are not looked at); 0 when the descriptor is not
- * valid.  Calls that may run at the same time need workspaces of their own. */
+/* Bytes of workspace that suffice for a call with this descriptor (pointers are not looked at) and, with the same ctas, for every
+ * call with fewer sequences, a shorter prefix or a smaller max_blocks_per_seq; 0 when the descriptor is not valid.  Calls that
+ * may run at the same time need workspaces of their own. */
 size_t hfk_prefix_attention_workspace(const hfk_prefix_attention_desc *desc, int ctas);
 
 /* One new token of each sequence attends to the shared prefix and to the sequence's own tokens, one layer:
