@@ -380,7 +380,8 @@ static int attention_impl(const hfk_prefix_attention_desc *d, int ctas, cudaStre
   if (rc != HFK_OK) return rc;
   if (d->num_seqs > 1 && d->block_table_stride < d->max_blocks_per_seq)
     return fail(HFK_ERR_INVALID_ARG, "%s: block_table_stride < max_blocks_per_seq", op);
-  if (!(std::abs(d->scale) <= 3.4e38f)) return fail(HFK_ERR_INVALID_ARG, "%s: scale is not finite", op);
+  // (what the kernels multiply by is the product)
+  if (!std::isfinite(d->scale * kLog2e)) return fail(HFK_ERR_INVALID_ARG, "%s: scale is not finite, or not below 2.3e38", op);
   if (d->num_seqs == 0) return HFK_OK;
   if ((rc = validate_rows(op, "q", d->q)) != HFK_OK) return rc;
   if ((rc = validate_written(op, "out", d->out, d->num_seqs, (int64_t)d->kv_heads * d->group, (int64_t)d->head_dim * 2)) != HFK_OK) return rc;

@@ -529,7 +529,7 @@ typedef struct hfk_prefix_attention_desc {
   int64_t block_size;
   int64_t device_block_stride;
   int64_t num_device_blocks;
-  float scale; /* of the scores; finite */
+  float scale; /* of the scores; finite, below 2.3e38 (its product with log2 e is finite too) */
   void *workspace; /* DEVICE, 256-byte aligned, hfk_prefix_attention_workspace() bytes; nothing in it needs clearing */
   size_t workspace_bytes;
 } hfk_prefix_attention_desc;
