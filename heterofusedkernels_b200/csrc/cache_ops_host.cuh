@@ -353,11 +353,13 @@ static cudaError_t launch_attention(const AttnArgs &a, const AttnPlan &p, unsign
     if ((e = allow_smem(k, smem)) != cudaSuccess) return e;
     if ((e = launch_behind(k, p.tensor, p.ctas, kLineWarps * 32, smem, s, join.a)) != cudaSuccess) return e;
   }
-  const int rows = a.seqs * a.kv_heads * a.group, resident = sm_count() * kJoinWarpsPerSm;
-  if (rows * 16 <= resident) return launch_behind(shared_prefix_join_kernel<T, D, 16>, true, rows, 512, 0, s, join);
-  if (rows * 4 <= resident) return launch_behind(shared_prefix_join_kernel<T, D, 4>, true, rows, 128, 0, s, join);
-  if (rows * 2 <= resident) return launch_behind(shared_prefix_join_kernel<T, D, 2>, true, rows, 64, 0, s, join);
-  return launch_behind(shared_prefix_join_kernel<T, D, 1>, true, rows, 32, 0, s, join);
+  const int rows = a.seqs * a.kv_heads * a.group;
+  switch (join_warps(rows, sm_count() * kJoinWarpsPerSm)) {
+    case 16: return launch_behind(shared_prefix_join_kernel<T, D, 16>, true, rows, 512, 0, s, join);
+    case 4: return launch_behind(shared_prefix_join_kernel<T, D, 4>, true, rows, 128, 0, s, join);
+    case 2: return launch_behind(shared_prefix_join_kernel<T, D, 2>, true, rows, 64, 0, s, join);
+    default: return launch_behind(shared_prefix_join_kernel<T, D, 1>, true, rows, 32, 0, s, join);
+  }
 }
 template <typename T, int kFmt>
 static cudaError_t launch_attention(const AttnArgs &a, int head_dim, const AttnPlan &p, unsigned char *w, cudaStream_t s) {

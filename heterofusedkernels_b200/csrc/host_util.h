@@ -61,6 +61,10 @@ constexpr int kGatherDequantCtasPerSm = 2;
 constexpr int kAttnCtasPerSm = 1;
 // Warps of the join that an SM holds at once (about 72 registers a thread).
 constexpr int kJoinWarpsPerSm = 28;
+// Warps of the join for each of `rows` rows (up to 2^30), so that all of them fit in the `resident` ones.
+constexpr int join_warps(long long rows, long long resident) {
+  return rows * 16 <= resident ? 16 : rows * 4 <= resident ? 4 : rows * 2 <= resident ? 2 : 1;
+}
 // Rows of queries (sequences x query heads of a K/V head) above which the prefix goes to the tensor-core kernel.
 constexpr int kPrefixTensorMinRows = 32;
 // What a CTA of that kernel costs beyond its key tiles, in tiles of about 2.6 us, and how many values of parts (8 bytes to
