@@ -387,16 +387,24 @@ class PagedKVCache:
 
     def attend(self, layer: int, q: torch.Tensor, prefix_table: torch.Tensor, prefix_len: int, block_tables: torch.Tensor,
                seq_lens: torch.Tensor, scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
-               lse: Optional[torch.Tensor] = None, aiv: Optional[int] = None) -> torch.Tensor:
+               lse: Optional[torch.Tensor] = None, aiv: Optional[int] = None,
+               workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Attention of one new token of each sequence, ``q`` ``[num_seqs, query heads, head_dim]``, over the pages of a
         prefix that all sequences share (``prefix_len`` tokens, 0 = none) and the pages of each sequence's own tokens
-        (``seq_lens``, the prefix not counted)."""
+        (``seq_lens``, the prefix not counted).  ``workspace``: see ``attend_workspace``; without it the call takes one from
+        torch's allocator."""
         if out is None:
             out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         torch.ops.pcie_through.shared_prefix_attention(q, out, self.k_caches[layer], self.v_caches[layer], prefix_table,
                                                        prefix_len, block_tables, seq_lens, self.block_size, self.kv_heads,
-                                                       self.kv_format, scale, lse, None, aiv)
+                                                       self.kv_format, scale, lse, workspace, aiv)
         return out
+
+    def attend_workspace(self, q: torch.Tensor, prefix_len: int, block_tables: torch.Tensor, aiv: Optional[int] = None) -> torch.Tensor:
+        """A workspace for ``attend`` of a batch like this one and of all smaller ones (fewer sequences, a shorter prefix, narrower
+        block tables; the same ``aiv``).  One user at a time: calls on two streams need one each."""
+        need = torch.ops.pcie_through.shared_prefix_attention_workspace(q, prefix_len, block_tables, self.block_size, self.kv_heads, aiv)
+        return torch.empty(need, dtype=torch.uint8, device=q.device)
 
     def migrate_to(self, other: "PagedKVCache", src_block_ids, dst_block_ids, aiv: Optional[int] = None,
                    run_on: str = "dst") -> None:
