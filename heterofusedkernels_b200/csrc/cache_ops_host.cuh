@@ -65,7 +65,10 @@ template <typename T, bool kRope, int kLanes, int kUnits>
 static cudaError_t launch_kv_write(const KvWriteArgs &a, int fmt, cudaStream_t s) {
   if (fmt == HFK_KV_E4M3) return launch_kv_write<T, kFmtE4m3, kRope, kLanes, kUnits>(a, s);
   if (fmt == HFK_KV_INT8) return launch_kv_write<T, kFmtInt8, kRope, kLanes, kUnits>(a, s);
-  return launch_kv_write<T, kFmtRaw, kRope, kLanes, kUnits>(a, s);
+  if constexpr (!kRope && kUnits > 1)
+    return cudaErrorInvalidValue;   // write_wide leaves copies to one unit
+  else
+    return launch_kv_write<T, kFmtRaw, kRope, kLanes, kUnits>(a, s);
 }
 template <typename T, bool kRope, int kUnits>
 static cudaError_t launch_kv_write(const KvWriteArgs &a, int fmt, cudaStream_t s) {
@@ -75,7 +78,7 @@ static cudaError_t launch_kv_write(const KvWriteArgs &a, int fmt, cudaStream_t s
 }
 template <typename T, bool kRope>
 static cudaError_t launch_kv_write(const KvWriteArgs &a, int fmt, cudaStream_t s) {
-  return a.rows < kWriteWideRows ? launch_kv_write<T, kRope, 1>(a, fmt, s) : launch_kv_write<T, kRope, 2>(a, fmt, s);
+  return write_wide(a.rows, a.head_dim, kRope, fmt == HFK_KV_RAW) ? launch_kv_write<T, kRope, 2>(a, fmt, s) : launch_kv_write<T, kRope, 1>(a, fmt, s);
 }
 
 static int kv_write_impl(const char *op, const hfk_kv_write_desc *d, const hfk_norm_rope_desc *n, bool rope, cudaStream_t stream) {

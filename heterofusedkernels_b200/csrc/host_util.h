@@ -50,10 +50,23 @@ constexpr int kDefaultStagedLanes = 1;
 constexpr long long kStagedMaxCopyBytes = 64ll << 20;
 // Block migration: 512-thread CTAs per SM (peer loads over NVLink need megabytes in flight).
 constexpr int kMigrateCtasPerSm = 2;
-// kv_write: rows from which a lane takes 32 elements of a row, not 16.  16 finish sooner while every warp is resident and a
-// call lasts as long as one row's chain, 32 take fewer instructions.  Rotated, 48 rows a token, e4m3: 2.42 us with 16 and 2.74
-// with 32 for one token, 3.53 and 3.76 for 256, 5.03 and 4.50 for 512, 13.7 and 12.4 for 2048.
-constexpr unsigned kWriteWideRows = 1u << 14;
+// kv_write: whether a lane takes 32 elements of a row, not 16.  16 finish sooner while every warp is resident and a call lasts as long
+// as one row's chain; 32 take fewer instructions a row, so they pay where a row has much work (a scale and codes, a norm and a
+// rotation) and there are many.  A plain copy has little, and heads up to 64 leave few lanes a row to hide its latency.
+// us with 16 and with 32, bf16, 4 K/V heads, rotated with 16 query heads (rows = heads of all tokens):
+//   head_dim, form        16384 rows    32768       65536       524288
+//   128 to e4m3           2.60, 2.60  3.73, 3.20  5.42, 5.12  34.7, 33.1
+//   128 rotated, e4m3     3.53, 3.80  5.43, 5.02  8.89, 8.76  62.3, 62.6
+//   256 to e4m3           3.79, 3.05  5.44, 4.50  9.58, 8.78  67.4, 62.6
+//   64 to e4m3            2.26, 2.33  2.60, 2.80  3.70, 3.70  18.9, 18.0
+//   64 rotated, e4m3      2.95, 3.49  3.61, 4.22  5.55, 5.70  34.3, 35.3
+//   16 rotated, e4m3      2.94, 3.00  3.56, 3.31  5.51, 4.33  29.1, 22.6
+//   64 copied             2.26, 2.48  2.85, 3.18  4.30, 4.47  22.1, 26.7
+//   128 copied            2.80, 2.92  4.36, 4.03  6.40, 6.46  41.4, 42.8
+//   16 copied             1.96, 1.90  2.15, 2.01  2.78, 2.21  10.6,  6.9
+constexpr bool write_wide(long long rows, int head_dim, bool rope, bool copied) {
+  return (rope || !copied) && rows >= (head_dim > 64 ? 1 << 14 : 1 << 16);
+}
 // Reading an 8-bit cache back: 256-thread CTAs per SM, eight 8-byte loads a lane in flight.  6.9 GB (64 sequences, 4 layers):
 // 1113 us with 2, 1186 with 4, 1157 with 8 and half the loads a lane.
 constexpr int kGatherDequantCtasPerSm = 2;

@@ -49,7 +49,7 @@ struct KvWriteArgs {
 // lane, 70 with 16, 65 with 32; 16384 tokens with rotation of 40 heads, fp16 to e4m3 (379 MB): 135, 80 and 77 to 82 us (the
 // spread between processes).  Loads of the table before the row is waited for: 86 us, for the registers they take.  Two or
 // four rows a thread were slower (85 and 172 us there), and so were CTAs of 256 threads (70 and 81 us with 32 elements).  Few
-// rows take one unit a lane (kWriteWideRows); without rotation that form is held to 32 registers, so that all warps fit.
+// rows, and copies, take one unit a lane (write_wide); without rotation that form is held to 32 registers, so that all warps fit.
 template <typename T, int kFmt, bool kRope, int kLanes, int kUnits, int kThreads>
 __global__ void __launch_bounds__(kThreads, kRope || kUnits > 1 ? 1 : 16) kv_write_kernel(const __grid_constant__ KvWriteArgs a) {
   constexpr int kGroups = kThreads / kLanes;
