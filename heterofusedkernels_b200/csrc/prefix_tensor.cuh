@@ -689,7 +689,9 @@ __global__ void __launch_bounds__(kPtThreads, 1) prefix_tensor_kernel(const __gr
         const int all = shift_to_half(__uint_as_float(high)), e = mixed ? shift_to_half(top[0]) : all;
         const int shared = mixed ? min(-all, kSharedBack) : -all;
         if (threadIdx.x == 0) sm.q_back = power_of_two(shared);
-        if (mixed) row_back = __shfl_sync(0xffffffffu, power_of_two(max(-126, -e - shared)), (lane % kRowsPass) * kChunks + lane / kRowsPass);
+        // (a row 2^166 below the largest has no such factor: its scores are nothing, not 2^40 times what they are)
+        const float undo = -e - shared < -126 ? 0.f : power_of_two(-e - shared);
+        if (mixed) row_back = __shfl_sync(0xffffffffu, undo, (lane % kRowsPass) * kChunks + lane / kRowsPass);
         const float own = power_of_two(e);
 #pragma unroll
         for (int k = 0; k < kPasses; ++k) {

@@ -118,6 +118,20 @@ def test_queries_that_grow_from_row_to_row(op, cuda_device, fmt, scale):
         check_rows(c, out, lse, torch.ones(8, 8, dtype=torch.bool))
 
 
+def test_queries_far_below_their_neighbours(op, cuda_device):
+    """Rows of 2^-112 next to rows of 2^56, keys of 2^66: the small rows' scores are 2^-40, so every key has the same weight."""
+    c = attention_case("e4m3", BF16, 1, 2, 128, 16, 300, [2] * 40, seed=12)
+    o.split_pages(c["k"], 16, 1, 128, "e4m3")[1].mul_(2.0 ** 66)
+    c["q"] = torch.randn(40, 2, 128, generator=gen(3)).to(BF16)
+    c["q"][:, 0] *= 2.0 ** -112
+    c["q"][:, 1] *= 2.0 ** 56
+    rows = torch.zeros(40, 2, dtype=torch.bool)
+    rows[:, 0] = True
+    out, lse = run_attention(op, c, cuda_device)
+    assert status() == 0
+    check_rows(c, out, lse, rows)
+
+
 @pytest.mark.parametrize("seqs", [2, 40])
 @pytest.mark.parametrize("dtype,powers", [(BF16, (8, 20, 25, 31, 40, 70)), (FP16, (8, 13))])
 def test_scores_of_any_magnitude(op, cuda_device, seqs, dtype, powers):
