@@ -13,14 +13,16 @@
 // in its softmax, the tensor cores work on the other: per 128 keys and tile, at head_dim 128, both products take about
 // 1024 clocks of the tensor cores and the 128 x 128 exponentials 1024 clocks of the special function units.
 //
-// Measured: 8 items of 256 rows against 32768 keys, e4m3 (34 GFLOP): 57 us, of which 12 pass before the first tile's
+// Measured: 8 items of 256 rows against 32768 keys, e4m3 (34 GFLOP): 58 to 59 us, of which 12 pass before the first tile's
 // scores and behind the last one's, 33 with the softmax left out (a tile's two products take 1450 clocks, the operands
 // from shared memory being at its bandwidth), the rest is softmax that nothing hides.  Steps to there: 105 us at first;
 // 92 with the queries loaded a row's worth at a time and the parts' rows leaving as bulk copies; 64 with packed fp32
-// arithmetic; 57 with short loops instead of unrolled ones (warps waited for instructions) and four rows a thread.
+// arithmetic; 57 with short loops instead of unrolled ones (warps waited for instructions) and four rows a thread; 58 with
+// powers of two and origins of each row's own and one barrier earlier.
 //
 // o is rescaled only where a row's maximum rises by more than 2^8 above the one in use: weights up to 2^8 are as
-// exact as weights up to 1, and l and o stay in the same units, so nothing is lost.
+// exact as weights up to 1, so nothing is lost.  Of an 8-bit cache also where a row's largest weight times scale rises above
+// what fp16 holds (e); both are looked at in one vote, so a tile in which nothing moves pays two additions a row.
 //
 // Operand layouts: rows of 128 bytes (64 values), 16-byte chunks XORed with the row number mod 8 ("128-byte swizzle"),
 // head_dim 128 as two such halves.  The same bytes serve K (rows = keys, read along the row) and V (rows = keys, read

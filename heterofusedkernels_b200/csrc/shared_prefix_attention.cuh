@@ -10,6 +10,10 @@
 // K/V head, seqs * G of them, and only what follows the prefix is read for each sequence alone.
 // A row without any key (no prefix, length 0) is 0 with lse = -inf.
 //
+// 16-bit cache: weights are rounded to the cache's type, because the product wants operands of one type: 2^-9 (bf16) or 2^-12
+// (fp16) of each weight, with errors of either sign, while l sums them unrounded.  Measured against 64 bits, bf16, thousands of keys:
+// 0.0022 of the result, 0.0017 of which is the result's own rounding.
+//
 // 8-bit cache: codes are exact in fp16, so the products run on codes in fp16; the scale of a key multiplies its score,
 // the scale of a value its weight.  bf16 queries become fp16 numbers times a power of two of their row that brings its largest
 // to 2^14: they have fewer bits than fp16, so only what is 2^29 times smaller than that loses any, 2^-39 of it.
@@ -293,7 +297,7 @@ struct alignas(128) LineRing {
 // a row where the operand layout would have it take two, and V needs no transposition: a lane that holds the same
 // columns of four rows packs its operands with byte permutations.
 //
-// Bound by HBM for long sequences: 8 of 16384 to 131072 tokens, 8 heads of 128, bf16 (2.4 GB) 355 to 375 us, 6.4 to 6.8 TB/s;
+// Bound by HBM for long sequences: 8 of 16384 to 131072 tokens, 8 heads of 128, bf16 (2.4 GB) 355 to 376 us, 6.4 to 6.8 TB/s;
 // for short ones by the chain from a sequence's length over its page ids to its rows (about 5 us), and of 8-bit caches by
 // what eight warps an SM can hide of a tile's latencies (50 MB 18 us).
 template <typename T, int kFmt, int D>

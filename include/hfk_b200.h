@@ -460,6 +460,7 @@ typedef struct hfk_kv_write_desc {
   hfk_rows v;
   void *k_cache; /* one layer's cache, [num_device_blocks] pages */
   void *v_cache;
+  /* (the two caches must not share pages) */
   const void *slot_ids; /* DEVICE [tokens]: block * block_size + place in the block; negative = padding */
   int ids_are_int64;
   int type;      /* HFK_TYPE_BF16 or HFK_TYPE_FP16: of k and v, and of a HFK_KV_RAW cache */
@@ -496,7 +497,8 @@ typedef struct hfk_norm_rope_desc {
 
 /* hfk_kv_write after the norm of each query and key head (x * rsqrt(mean(x^2) + eps) * weight) and the rotation of
  * its first rot_dim elements, in fp32 with one rounding at the end; the rotated queries go to q_out, the keys only
- * to the cache.  A token with a negative slot is padding: neither its q_out row nor a page is written.  A position
+ * to the cache.  A token with a negative slot is padding: neither its q_out row nor a page is written (a new q_out holds there
+ * whatever it held; hfk_shared_prefix_attention of such a row gives a row of no meaning and leaves the others alone).  A position
  * outside the table sets HFK_DEV_BAD_POSITION and its token is skipped.
  * tokens * (q_heads + 2 * kv_heads) < 2^31. */
 int hfk_qk_norm_rope_write(const hfk_kv_write_desc *desc, const hfk_norm_rope_desc *norm_rope, hfk_stream_t stream);
@@ -541,7 +543,16 @@ size_t hfk_prefix_attention_workspace(const hfk_prefix_attention_desc *desc, int
 
 /* One new token of each sequence attends to the shared prefix and to the sequence's own tokens, one layer:
  *   out[s, h*group + g] = softmax(scale * q . [Kprefix[h]; K_s[h]]) [Vprefix[h]; V_s[h]]
- * The prefix is read for all sequences together.  A length outside 0 .. max_blocks_per_seq * block_size is clamped and
+ * The prefix is read for all sequences together.  Scores, maxima, sums and results are held in fp32.  Rounded to fewer bits are:
+ *   the weights, before they are multiplied by the values: to the type of a 16-bit cache (bf16: 2^-9 of each; fp16: 2^-12, and never
+ *   by more than 2^-32 of the row's largest weight); of an 8-bit cache, times the value's scale, to fp16 (2^-12 of each, and never
+ *   by more than 2^-31 of the largest such product of the row, for scales of 2^-108 and more);
+ *   bf16 queries over an 8-bit cache, to fp16 times a power of two (never by more than 2^-29 of the row's largest);
+ *   the result, once, to `type`.
+ * ctas: CTAs of the kernel that reads the sequences' own tokens, 0 = one an SM; the prefix takes at least one for each K/V head and
+ * 256 rows of queries.  prefix_len is a number of the host: a captured graph keeps it, while lengths, tables and pages may
+ * change between replays.
+ * A length outside 0 .. max_blocks_per_seq * block_size is clamped and
  * sets HFK_DEV_BAD_SEQ_LEN; a page id outside the cache sets HFK_DEV_BAD_DEVICE_BLOCK_ID and its keys are left out.
  * A row without keys is 0, its lse -infinity. */
 int hfk_shared_prefix_attention(const hfk_prefix_attention_desc *desc, int ctas, hfk_stream_t stream);
